@@ -49,6 +49,39 @@ class Fp16LinearParams(C.Structure):
     ]
 
 
+class Int8TokenLinearParams(C.Structure):
+    """struct trtamd_int8_token_linear_params (include/trtamd_encoder_ops.h)."""
+    _fields_ = [
+        ("a", c_p), ("w", c_p), ("token_scale", c_p), ("channel_scale", c_p), ("bias", c_p), ("out", c_p),
+        ("T", i32), ("K", i32), ("N", i32), ("epilogue", i32),
+    ]
+
+
+class Int8DynamicLinearParams(C.Structure):
+    """struct trtamd_int8_dynamic_linear_params (include/trtamd_encoder_ops.h)."""
+    _fields_ = [
+        ("a", c_p), ("a_stride", i64), ("w", c_p), ("channel_scale", c_p), ("bias", c_p), ("out", c_p),
+        ("workspace", c_p), ("workspace_bytes", C.c_size_t),
+        ("T", i32), ("K", i32), ("N", i32), ("epilogue", i32),
+    ]
+
+
+class QkNormRotaryParams(C.Structure):
+    """struct trtamd_qk_norm_rotary_params (include/trtamd_encoder_ops.h)."""
+    _fields_ = [
+        ("q", c_p), ("k", c_p), ("q_out", c_p), ("k_out", c_p),
+        ("q_token_stride", i64), ("q_head_stride", i64), ("k_token_stride", i64), ("k_head_stride", i64),
+        ("q_out_token_stride", i64), ("q_out_head_stride", i64), ("k_out_token_stride", i64), ("k_out_head_stride", i64),
+        ("T", i32), ("q_heads", i32), ("k_heads", i32), ("d", i32),
+        ("norm", i32), ("eps", f32),
+        ("q_weight", c_p), ("k_weight", c_p), ("q_bias", c_p), ("k_bias", c_p),
+        ("rotary_dim", i32), ("adjacent_pairs", i32),
+        ("frequencies", c_p), ("positions", c_p),
+        ("axes", i32), ("axes_cycled", i32), ("sections", i32 * 4),
+    ]
+
+
+QK_NORM_NONE, QK_NORM_RMS, QK_NORM_LAYER = 0, 1, 2
 LINEAR_AFFINE, LINEAR_GELU, LINEAR_RAW_INT32, LINEAR_AFFINE_FP16 = 0, 1, 2, 3
 UNFUSED_ROUTE_ONE_LAUNCH, UNFUSED_ROUTE_THREE_LAUNCHES, UNFUSED_ROUTE_BY_SHAPE = 0, 1, 99
 
@@ -145,6 +178,11 @@ _SIGS = {
     "trtamd_zero_padding_2d": (C.c_int, [c_p, i32, c_p, i32, i32, c_p]),
     "trtamd_int8_linear": (C.c_int, [c_p, C.POINTER(Int8LinearParams)]),
     "trtamd_fp16_linear": (C.c_int, [c_p, C.POINTER(Fp16LinearParams)]),
+    "trtamd_quantize_fp16_per_token": (C.c_int, [c_p, i32, i32, c_p, i64, c_p, c_p]),
+    "trtamd_int8_token_linear": (C.c_int, [c_p, C.POINTER(Int8TokenLinearParams)]),
+    "trtamd_int8_dynamic_linear_workspace_size": (C.c_size_t, [i32, i32, i32]),
+    "trtamd_int8_dynamic_linear": (C.c_int, [c_p, C.POINTER(Int8DynamicLinearParams)]),
+    "trtamd_qk_norm_rotary": (C.c_int, [c_p, i32, C.POINTER(QkNormRotaryParams)]),
     "trtamd_encoder_create": (c_p, [C.POINTER(EncoderConfig)]),
     "trtamd_encoder_destroy": (None, [c_p]),
     "trtamd_encoder_set_embedding": (C.c_int, [c_p, C.POINTER(EncoderEmbedding)]),
@@ -167,7 +205,9 @@ TEST_HOOK_SYMBOLS = ["trtamd_fused_mha_run_debug", "trtamd_test_set_tuning", "tr
 # Entry points declared in include/trtamd_bert_kernels.h are the rest of the table.
 # Entry points declared in include/trtamd_encoder_ops.h.
 ENCODER_OPS_SYMBOLS = ["trtamd_int8_linear", "trtamd_fp16_linear", "trtamd_int8_linear_to_interleaved", "trtamd_int8_interleaved_to_linear",
-                       "trtamd_quantize_fp16_to_interleaved", "trtamd_dequantize_interleaved_to_fp16"]
+                       "trtamd_quantize_fp16_to_interleaved", "trtamd_dequantize_interleaved_to_fp16",
+                       "trtamd_quantize_fp16_per_token", "trtamd_int8_token_linear",
+                       "trtamd_int8_dynamic_linear_workspace_size", "trtamd_int8_dynamic_linear", "trtamd_qk_norm_rotary"]
 # Entry points declared in include/trtamd_encoder_runtime.h.
 ENCODER_RUNTIME_SYMBOLS = ["trtamd_encoder_create", "trtamd_encoder_destroy", "trtamd_encoder_set_embedding",
                            "trtamd_encoder_set_layer", "trtamd_encoder_workspace_size", "trtamd_encoder_enqueue",

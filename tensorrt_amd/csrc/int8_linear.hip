@@ -53,19 +53,38 @@ enum Epilogue
     // FP16 operands (trtamd_fp16_linear): the same kernels with v_mfma_f32_32x32x16_f16 and binary32 accumulators
     kF16_AFFINE = 4,
     kF16_GELU = 5,
-    kF16_RAW = 6 // the binary32 accumulators (partial sums of fp16_linear_partial)
+    kF16_RAW = 6, // the binary32 accumulators (partial sums of fp16_linear_partial)
+    // INT8 operands, FP16 results with a scale for each token too (trtamd_int8_token_linear)
+    kTOKEN = 7,
+    kTOKEN_GELU = 8
 };
+
+constexpr bool f16_operands(int epi)
+{
+    return epi == kF16_AFFINE || epi == kF16_GELU || epi == kF16_RAW;
+}
+
+constexpr bool token_scaled(int epi)
+{
+    return epi == kTOKEN || epi == kTOKEN_GELU;
+}
+
+// FP16 results from operands of one layout.
+constexpr bool f16_rows(int epi)
+{
+    return epi == kF16_AFFINE || epi == kF16_GELU || token_scaled(epi);
+}
 
 // INT8 operands accumulate in INT32, FP16 operands in binary32.  Either way a lane feeds 16 bytes of a row per
 // operand and MFMA step (16 INT8 or 8 FP16 values of k), a fragment is 32 rows x 32 bytes, and the result has the
 // same 32 x 32 accumulator layout, so the tiling, the LDS layout and the load schedule are shared.
 template <int EPI>
-using AccT = std::conditional_t<(EPI >= kF16_AFFINE), f32x16, i32x16>;
+using AccT = std::conditional_t<f16_operands(EPI), f32x16, i32x16>;
 
 template <int EPI>
 __device__ __forceinline__ AccT<EPI> mma(i32x4 const a, i32x4 const b, AccT<EPI> const c)
 {
-    if constexpr (EPI >= kF16_AFFINE)
+    if constexpr (f16_operands(EPI))
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(bits_as<f16x8>(a), bits_as<f16x8>(b), c, 0, 0, 0);
     }
@@ -80,7 +99,7 @@ struct LinearArgs
     int8_t const* a;
     int8_t const* w;
     float const* alpha;
-    float const* beta;
+    float const* beta; // token-scaled epilogues: may be null, for zeros
     void* out;
     int T, K, N; // K: bytes of k per row (elements for INT8, twice the elements for FP16)
     float qOut;
@@ -93,6 +112,7 @@ struct LinearArgs
     int perPart;   // pieces: 32-byte k-slabs (interleaved operands) or stages of 64 or 128 bytes of each
     FastDiv panelDiv, perPanelDiv; // tiles: by panel and tokMain * panel
     WeightPrefetch prefetch; // by the workgroups behind mainTiles of the interleaved tile and piece kernels
+    float const* tokenScale; // token-scaled epilogues
 };
 
 // gelu(y) = y * Phi(y) = max(y, 0) - |y| * Phi(-|y|).  log2(Phi(-a)) is smooth and nearly quadratic, so
@@ -109,6 +129,41 @@ __device__ inline float gelu_erf(float y)
     p = fmaf(p, a, -1.129245639e+00f);
     p = fmaf(p, a, -1.003531814e+00f);
     return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
+}
+
+// The same for FP16 results, which need Phi(-a) to a relative error (y Phi(y) is small, not rounded away, for negative y):
+// a polynomial of degree 7 for log2(Phi(-a)) that is off by 4.5e-6 at most on [0, 5.5], behind which the result is below
+// half of the smallest binary16.  Within 4e-6 of the exact value where that is a normal binary16, 2.5e-10 elsewhere.  The leading coefficient is
+// negative, so the term vanishes for larger a; a NaN stays one (through a).
+__device__ inline float gelu_f16(float y)
+{
+    float const a = fabsf(y);
+    float p = fmaf(a, -1.793455226e-06f, 6.090417810e-05f);
+    p = fmaf(p, a, -9.260290535e-04f);
+    p = fmaf(p, a, 8.493757807e-03f);
+    p = fmaf(p, a, -5.393784493e-02f);
+    p = fmaf(p, a, -4.584805071e-01f);
+    p = fmaf(p, a, -1.151246786e+00f);
+    p = fmaf(p, a, -9.999954700e-01f);
+    return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
+}
+
+// The result of a token-scaled layer: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
+template <int EPI>
+__device__ __forceinline__ float token_result(int const acc, float const ts, float const al, float const be)
+{
+    float const y = fmaf((float) acc * ts, al, be);
+    return EPI == kTOKEN_GELU ? gelu_f16(y) : y;
+}
+
+template <int EPI>
+__device__ __forceinline__ float token_scale(LinearArgs const& p, int const t)
+{
+    if constexpr (token_scaled(EPI))
+    {
+        return p.tokenScale[min(t, p.T - 1)];
+    }
+    return 1.f;
 }
 
 // One operand fragment of v_mfma_i32_32x32x32_i8 is 32 rows x 32 k-bytes; lane l feeds row l%32,
@@ -175,9 +230,10 @@ __device__ __forceinline__ BlockScales load_block_scales(float const* sAlpha, fl
     return s;
 }
 
-// The FP16 results of a 32 x 32 block: 16 consecutive channels, 16 (l/32) .. +15, of token l%32 per lane.
+// The FP16 results of a 32 x 32 block: 16 consecutive channels, 16 (l/32) .. +15, of token l%32 per lane (ts: its scale).
 template <int EPI>
-__device__ __forceinline__ void pack_half_block(AccT<EPI> const& acc, BlockScales const& sc, u32x4& first, u32x4& second)
+__device__ __forceinline__ void pack_half_block(
+    AccT<EPI> const& acc, BlockScales const& sc, float const ts, u32x4& first, u32x4& second)
 {
     u32x2 w[4];
 #pragma unroll
@@ -187,8 +243,15 @@ __device__ __forceinline__ void pack_half_block(AccT<EPI> const& acc, BlockScale
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            float const y = fmaf((float) acc[4 * g + e], sc.al[g][e], sc.be[g][e]);
-            h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
+            if constexpr (token_scaled(EPI))
+            {
+                h[e] = (f16) token_result<EPI>(acc[4 * g + e], ts, sc.al[g][e], sc.be[g][e]);
+            }
+            else
+            {
+                float const y = fmaf((float) acc[4 * g + e], sc.al[g][e], sc.be[g][e]);
+                h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
+            }
         }
         w[g] = __builtin_bit_cast(u32x2, h);
     }
@@ -204,7 +267,7 @@ __device__ __forceinline__ void pack_half_block(AccT<EPI> const& acc, BlockScale
 
 template <bool IL_OUT, int EPI, bool FULL = false, bool THROUGH = false>
 __device__ __forceinline__ void store_block_scaled(
-    LinearArgs const& p, AccT<EPI> const& acc, int const c0, int const tb, BlockScales const& sc)
+    LinearArgs const& p, AccT<EPI> const& acc, int const c0, int const tb, BlockScales const& sc, float const ts = 1.f)
 {
     int const lane = threadIdx.x & 63;
     int const hi = lane >> 5;
@@ -224,10 +287,10 @@ __device__ __forceinline__ void store_block_scaled(
             }
         }
     }
-    else if constexpr (EPI >= kF16_AFFINE || EPI == kHALF)
+    else if constexpr (f16_rows(EPI) || EPI == kHALF)
     {
         u32x4 first, second;
-        pack_half_block<EPI>(acc, sc, first, second);
+        pack_half_block<EPI>(acc, sc, ts, first, second);
         if (live)
         {
             f16* dst = static_cast<f16*>(p.out) + (size_t) t * p.N + c0 + 16 * hi;
@@ -276,7 +339,19 @@ template <bool IL_OUT, int EPI, bool FULL = false, bool THROUGH = false>
 __device__ __forceinline__ void store_block(
     LinearArgs const& p, AccT<EPI> const& acc, int const c0, int const tb, float const* sAlpha, float const* sBeta)
 {
-    store_block_scaled<IL_OUT, EPI, FULL, THROUGH>(p, acc, c0, tb, load_block_scales<EPI>(sAlpha, sBeta));
+    store_block_scaled<IL_OUT, EPI, FULL, THROUGH>(p, acc, c0, tb, load_block_scales<EPI>(sAlpha, sBeta),
+        token_scale<EPI>(p, tb + (int) (threadIdx.x & 31)));
+}
+
+// The offset of channel n.
+template <int EPI>
+__device__ __forceinline__ float offset_of(LinearArgs const& p, int const n)
+{
+    if constexpr (token_scaled(EPI))
+    {
+        return p.beta ? p.beta[n] : 0.f;
+    }
+    return p.beta[n];
 }
 
 // Epilogue of one workgroup tile.
@@ -446,7 +521,7 @@ __device__ __forceinline__ void linear_tile(
         {
             int const n = min(n0 + c, p.N - 1);
             sAlpha[c] = p.alpha[n];
-            sBeta[c] = p.beta[n];
+            sBeta[c] = offset_of<EPI>(p, n);
         }
     }
 
@@ -609,7 +684,7 @@ __device__ __forceinline__ void linear_tile_run(
     {
         int const n = min(n0 + ch, p.N - 1);
         scales(0, 0)[ch] = p.alpha[n];
-        scales(0, 1)[ch] = p.beta[n];
+        scales(0, 1)[ch] = offset_of<EPI>(p, n);
     }
     int const nk = p.K / 64; // even, >= 2
     fetch(Set0{}, oaC, obC, 0);
@@ -629,7 +704,7 @@ __device__ __forceinline__ void linear_tile_run(
         {
             int const n = min(n1 + ch, p.N - 1);
             nextAlpha = p.alpha[n];
-            nextBeta = p.beta[n];
+            nextBeta = offset_of<EPI>(p, n);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -1107,23 +1182,28 @@ __device__ __forceinline__ void linear_piece64(
     }
 }
 
-// The scales and offsets of the four channels that a lane of a piece stores: requested with the operands, since a trip to
+// The scales and offsets of the four channels that a lane of a piece stores, and the scale of its token t: requested with the operands, since a trip to
 // memory behind the sums is as long as everything else behind the operands' (see linear_piece_kernel).
 struct QuadScales
 {
     f32x4 al, be;
+    float ts;
 };
 
 template <int EPI>
-__device__ __forceinline__ QuadScales load_quad_scales(LinearArgs const& p, int const c)
+__device__ __forceinline__ QuadScales load_quad_scales(LinearArgs const& p, int const c, int const t)
 {
     QuadScales s{};
     if constexpr (EPI != kRAW && EPI != kF16_RAW)
     {
         int const at = min(c, p.N - 4);
         s.al = *reinterpret_cast<f32x4 const*>(p.alpha + at);
-        s.be = *reinterpret_cast<f32x4 const*>(p.beta + at);
+        if (!token_scaled(EPI) || p.beta)
+        {
+            s.be = *reinterpret_cast<f32x4 const*>(p.beta + at);
+        }
     }
+    s.ts = token_scale<EPI>(p, t);
     return s;
 }
 
@@ -1146,14 +1226,21 @@ __device__ __forceinline__ void store_quad(
     {
         return;
     }
-    if constexpr (EPI >= kF16_AFFINE)
+    if constexpr (f16_rows(EPI))
     {
         f16x4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            float const y = fmaf(acc[e], al[e], be[e]);
-            h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
+            if constexpr (token_scaled(EPI))
+            {
+                h[e] = (f16) token_result<EPI>(acc[e], sc.ts, al[e], be[e]);
+            }
+            else
+            {
+                float const y = fmaf(acc[e], al[e], be[e]);
+                h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
+            }
         }
         *reinterpret_cast<f16x4*>(static_cast<f16*>(p.out) + (size_t) t * p.N + c) = h;
     }
@@ -1368,10 +1455,21 @@ __device__ __forceinline__ void linear_tile_dma(
     auto fetch_scales = [&](int at) {
         if (wave < 2 && lane < BM / 4)
         {
+            if (token_scaled(EPI) && wave == 1 && p.beta == nullptr)
+            {
+                *reinterpret_cast<f32x4*>(lds + at + kBigTile * 4 + lane * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
+                return;
+            }
             float const* from = (wave == 0 ? p.alpha : p.beta) + min(n0 + lane * 4, p.N - 4);
             load_to_lds16(from, ldsBase + (uint32_t) (at + wave * kBigTile * 4));
         }
     };
+    float ts[NT]; // of this lane's tokens, requested before everything else: the wait for stage 0 covers them
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+    {
+        ts[j] = token_scale<EPI>(p, t0 + (wn * NT + j) * 32 + (lane & 31));
+    }
     if constexpr (!kLate)
     {
         fetch_scales(RING * STAGE); // requested first, so the wait for stage 0 covers them
@@ -1440,7 +1538,7 @@ __device__ __forceinline__ void linear_tile_dma(
     first_halves(No{});
     phase(Odd{}, No{}, 0, 0, NoLoads{}, 0, 0);
     constexpr int kRow = MT * 64 + 16; // bytes; 16 of padding spread the rows over the banks
-    constexpr bool kStaged = EPI >= kF16_AFFINE && NWAVES * 32 * kRow <= STAGE;
+    constexpr bool kStaged = f16_rows(EPI) && NWAVES * 32 * kRow <= STAGE;
     if constexpr (kLate || kStaged)
     {
         wait_vmcnt<0>();
@@ -1468,7 +1566,7 @@ __device__ __forceinline__ void linear_tile_dma(
             for (int i = 0; i < MT; ++i)
             {
                 u32x4 first, second;
-                pack_half_block<EPI>(acc[i][j], sc[i], first, second);
+                pack_half_block<EPI>(acc[i][j], sc[i], ts[j], first, second);
                 u32x4* dst = reinterpret_cast<u32x4*>(own + (lane & 31) * kRow + i * 64 + (lane >> 5) * 32);
                 dst[0] = first;
                 dst[1] = second;
@@ -1505,11 +1603,11 @@ __device__ __forceinline__ void linear_tile_dma(
             constexpr bool through = IL_OUT && (EPI == kAFFINE || EPI == kGELU);
             if (full)
             {
-                store_block_scaled<IL_OUT, EPI, true, through>(p, acc[i][j], n0 + cl, tb, sc);
+                store_block_scaled<IL_OUT, EPI, true, through>(p, acc[i][j], n0 + cl, tb, sc, ts[j]);
             }
             else
             {
-                store_block_scaled<IL_OUT, EPI, false, through>(p, acc[i][j], n0 + cl, tb, sc);
+                store_block_scaled<IL_OUT, EPI, false, through>(p, acc[i][j], n0 + cl, tb, sc, ts[j]);
             }
         }
     }
@@ -1670,7 +1768,8 @@ __global__ __launch_bounds__(512, PER_SIMD) void linear_piece_kernel(uint64_t co
     }
     uint32_t const slabA = (uint32_t) p.N * 32u, slabB = (uint32_t) p.T * 32u;
     static_assert(CB * TB * 4 <= NW, "a quarter of a block for each wavefront at most");
-    QuadScales const scales = load_quad_scales<EPI>(p, n0 + (wave / (4 * TB)) * 32 + 8 * (wave & 3) + 4 * half);
+    QuadScales const scales = load_quad_scales<EPI>(
+        p, n0 + (wave / (4 * TB)) * 32 + 8 * (wave & 3) + 4 * half, t0 + ((wave >> 2) % TB) * 32 + row);
     // this workgroup's k-slabs, and the consecutive ones of this wavefront
     int const slabs = min(p.K / 32, (kpart + 1) * p.perPart);
     int const per = ceil_div(p.perPart, NW), first = kpart * p.perPart + wave * per;
@@ -1731,7 +1830,7 @@ __global__ __launch_bounds__(512, PER_SIMD) void linear_piece_kernel(uint64_t co
             }
         }
     }
-    using Acc4 = std::conditional_t<(EPI >= kF16_AFFINE), f32x4, i32x4>;
+    using Acc4 = std::conditional_t<f16_operands(EPI), f32x4, i32x4>;
     // partial accumulators: [wavefront][block][four registers][lane], 16 bytes per lane and access
     Acc4* const part = reinterpret_cast<Acc4*>(lds);
 #pragma unroll
@@ -1807,7 +1906,7 @@ __global__ __launch_bounds__(NW * 64, PER_SIMD) void linear_piece_dma_kernel(uin
     for (int v = 0; v < kOwn; ++v)
     {
         int const u = v * NW + wave;
-        scales[v] = load_quad_scales<EPI>(p, n0 + (u / (4 * TB)) * 32 + 8 * (u & 3) + 4 * half);
+        scales[v] = load_quad_scales<EPI>(p, n0 + (u / (4 * TB)) * 32 + 8 * (u & 3) + 4 * half, t0 + ((u >> 2) % TB) * 32 + row);
     }
     int const nk = min(p.K / (32 * KS), (kpart + 1) * p.perPart); // stages up to the end of this workgroup's
     int const per = ceil_div(p.perPart, NW), first = kpart * p.perPart + wave * per;
@@ -1888,7 +1987,7 @@ __global__ __launch_bounds__(NW * 64, PER_SIMD) void linear_piece_dma_kernel(uin
         multiply(slot);
         slot = slot == RING - 1 ? 0 : slot + 1;
     });
-    using Acc4 = std::conditional_t<(EPI >= kF16_AFFINE), f32x4, i32x4>;
+    using Acc4 = std::conditional_t<f16_operands(EPI), f32x4, i32x4>;
     __builtin_amdgcn_s_waitcnt(0xC07F);
 #pragma unroll
     for (int i = 0; i < CB; ++i)
@@ -2350,11 +2449,12 @@ int launch_shape(hipStream_t stream, LinearArgs a)
     int const persistent = tuning(Tuning::kLinearPersistent);
     int const direct = tuning(Tuning::kLinearDirect);
     constexpr int kMaxPanel = 8; // 8 x 256 channels x K = 1024 of weights is half of an XCD's 4 MB L2
-    if constexpr (IL_W == IL_IN && (EPI == kAFFINE || EPI == kGELU || EPI == kF16_AFFINE || EPI == kF16_GELU))
+    if constexpr (IL_W == IL_IN && (EPI == kAFFINE || EPI == kGELU || f16_rows(EPI)))
     {
         if (persistent && direct)
         {
-            int const plan = plan_behind_large_tiles<IL_W>(a, smallTiles, EPI == kGELU || EPI == kF16_GELU);
+            int const plan = plan_behind_large_tiles<IL_W>(
+                a, smallTiles, EPI == kGELU || EPI == kF16_GELU || EPI == kTOKEN_GELU);
             if (plan != kLargeTiles) // numbers its tiles itself
             {
                 return launch_plan<IL_W, IL_OUT, EPI>(stream, a, plan);
@@ -2522,6 +2622,72 @@ int check_fp16(trtamd_fp16_linear_params const* p)
     return TRTAMD_STATUS_SUCCESS;
 }
 
+LinearArgs args_of(trtamd_int8_token_linear_params const& p)
+{
+    LinearArgs a{};
+    a.a = p.a;
+    a.w = p.w;
+    a.alpha = p.channel_scale;
+    a.beta = p.bias;
+    a.tokenScale = p.token_scale;
+    a.out = p.out;
+    a.T = p.T;
+    a.K = p.K;
+    a.N = p.N;
+    a.qOut = 1.f;
+    a.panel = 1;
+    return a;
+}
+
+int check_token(trtamd_int8_token_linear_params const* p)
+{
+    if (p == nullptr)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: null pointer");
+    }
+    if (p->T < 0 || p->K <= 0 || p->N <= 0 || p->K % 64 != 0 || p->N % 32 != 0)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM,
+            "int8_token_linear: T=%d K=%d N=%d (K must be a multiple of 64, N of 32)", p->T, p->K, p->N);
+    }
+    if (p->epilogue != TRTAMD_LINEAR_AFFINE && p->epilogue != TRTAMD_LINEAR_GELU)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: unknown epilogue %d", p->epilogue);
+    }
+    if (p->T == 0)
+    {
+        return TRTAMD_STATUS_SUCCESS; // tensors without a token may have no address
+    }
+    if (p->a == nullptr || p->w == nullptr || p->token_scale == nullptr || p->channel_scale == nullptr || p->out == nullptr)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: null pointer");
+    }
+    if ((int64_t) p->T * p->K >= (int64_t) 1 << 31 || (int64_t) p->N * p->K >= (int64_t) 1 << 31)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "int8_token_linear: operand of 2 GiB or more");
+    }
+    if (!aligned16(p->a) || !aligned16(p->w) || !aligned16(p->out) || !aligned16(p->channel_scale) || !aligned16(p->bias)
+        || (reinterpret_cast<uintptr_t>(p->token_scale) & 3u) != 0)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM,
+            "int8_token_linear: pointers must be 16-byte aligned (token_scale: 4)");
+    }
+    return TRTAMD_STATUS_SUCCESS;
+}
+
+int run_token(trtamd_stream_t stream, trtamd_int8_token_linear_params const* p)
+{
+    int const checked = check_token(p);
+    if (checked != TRTAMD_STATUS_SUCCESS || p->T == 0)
+    {
+        return checked;
+    }
+    LinearArgs const a = args_of(*p);
+    hipStream_t const st = as_stream(stream);
+    return p->epilogue == TRTAMD_LINEAR_GELU ? launch_shape<false, false, false, kTOKEN_GELU>(st, a)
+                                             : launch_shape<false, false, false, kTOKEN>(st, a);
+}
+
 int run_fp16(trtamd_stream_t stream, trtamd_fp16_linear_params const* p)
 {
     int const checked = check_fp16(p);
@@ -2618,6 +2784,11 @@ int fp16_linear_check(trtamd_fp16_linear_params const& p)
     return check_fp16(&p);
 }
 
+int int8_token_linear_check(trtamd_int8_token_linear_params const& p)
+{
+    return check_token(&p);
+}
+
 } // namespace trtamd
 
 extern "C" int trtamd_test_linear_plan(int32_t interleaved, int32_t T, int32_t row_bytes, int32_t N, int32_t gelu)
@@ -2648,4 +2819,9 @@ extern "C" int trtamd_int8_linear(trtamd_stream_t stream, trtamd_int8_linear_par
 extern "C" int trtamd_fp16_linear(trtamd_stream_t stream, trtamd_fp16_linear_params const* p)
 {
     return trtamd::run_fp16(stream, p);
+}
+
+extern "C" int trtamd_int8_token_linear(trtamd_stream_t stream, trtamd_int8_token_linear_params const* p)
+{
+    return trtamd::run_token(stream, p);
 }

@@ -40,6 +40,8 @@ int int8_linear_partial(trtamd_stream_t stream, trtamd_int8_linear_params const&
 int fp16_linear_partial(trtamd_stream_t stream, trtamd_fp16_linear_params const& p, int parts, float* partial);
 // The checks of trtamd_fp16_linear without its launch, for a pass that is refused before its first launch.
 int fp16_linear_check(trtamd_fp16_linear_params const& p);
+// The same of trtamd_int8_token_linear, for trtamd_int8_dynamic_linear.
+int int8_token_linear_check(trtamd_int8_token_linear_params const& p);
 
 // trtamd_skipln_interleaved_{small,large}_hface with the input given as the partial sums of an affine INT8 layer (alpha,
 // beta as in trtamd_int8_linear_params): the same bytes as the layer's output through memory would give.

@@ -1,0 +1,488 @@
+// Norms of queries and keys for each head and the rotation of their pairs by position, one pass over Q and K.
+//
+//   y = x | x / sqrt(mean(x^2) + eps) w | (x - mean) / sqrt(var + eps) w + b        over the d values of a head
+//   (a, b) -> (a cos(p f) - b sin(p f), b cos(p f) + a sin(p f))                    for its rotary_dim / 2 pairs
+//
+// HBM streaming: each value is read and written once.
+#include "device_utils.hpp"
+#include "host_utils.hpp"
+#include "trtamd_encoder_ops.h"
+
+namespace trtamd
+{
+namespace
+{
+
+struct Side
+{
+    void const* in;
+    void* out;
+    int64_t inToken, inHead, outToken, outHead;
+    float const* weight;
+    float const* bias;
+};
+
+struct RotaryArgs
+{
+    Side side[2]; // queries, keys
+    int T, qHeads, heads, d; // heads: of queries and keys
+    int norm;
+    float eps;
+    int half, adjacent; // half: pairs
+    float const* frequencies;
+    int32_t const* positions;
+    int axes, cycled;
+    int sections[TRTAMD_ROTARY_MAX_AXES];
+    FastDiv headsDiv;
+};
+
+__device__ inline int axis_of(RotaryArgs const& p, int pair)
+{
+    if (p.axes == 1)
+    {
+        return 0;
+    }
+    if (p.cycled)
+    {
+        int const turn = pair / p.axes, axis = pair - turn * p.axes;
+        int left = 0;
+#pragma unroll
+        for (int a = 0; a < TRTAMD_ROTARY_MAX_AXES; ++a)
+        {
+            left = a == axis ? p.sections[a] : left;
+        }
+        return turn < left ? axis : 0;
+    }
+    int axis = 0, end = 0;
+#pragma unroll
+    for (int a = 0; a + 1 < TRTAMD_ROTARY_MAX_AXES; ++a)
+    {
+        end += p.sections[a]; // 0 behind the last axis
+        axis += a + 1 < p.axes && pair >= end ? 1 : 0;
+    }
+    return axis;
+}
+
+// cos and sin of position * frequency: the angle in turns, reduced to half a turn in binary64 (binary32 has none of the
+// fraction left at far positions), then the library's function of that in binary32.
+__device__ inline void cos_sin(int32_t position, float frequency, float& c, float& s)
+{
+    constexpr double kInverseTwoPi = 0.15915494309189533577;
+    double const turns = (double) position * (double) frequency * kInverseTwoPi;
+    sincospif(2.f * (float) (turns - rint(turns)), &s, &c);
+}
+
+// V values of T as binary32.
+template <int V, typename T>
+__device__ inline void load_values(T const* p, float (&v)[V])
+{
+    if constexpr (V == 1)
+    {
+        v[0] = (float) *p;
+    }
+    else
+    {
+        typedef T Vec __attribute__((ext_vector_type(V)));
+        Vec const x = *reinterpret_cast<Vec const*>(p);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+        {
+            v[e] = (float) x[e];
+        }
+    }
+}
+
+template <int V, typename T>
+__device__ inline void store_values(T* p, float const (&v)[V])
+{
+    if constexpr (V == 1)
+    {
+        *p = (T) v[0];
+    }
+    else
+    {
+        typedef T Vec __attribute__((ext_vector_type(V)));
+        Vec x;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+        {
+            x[e] = (T) v[e];
+        }
+        *reinterpret_cast<Vec*>(p) = x;
+    }
+}
+
+// A lane's share of a head: two chunks of V values.  Pairs of distant values are the same places of chunks rotary_dim / 2
+// apart, adjacent ones lie in two chunks one behind the other, as does what is not rotated.
+struct Slot
+{
+    int at[2]; // where the chunks are; at[1] < 0: there is no second one
+    int pair;  // its first pair; V of them (those from `half` on are not rotated)
+};
+
+template <int V, bool ADJACENT>
+__device__ inline Slot slot_of(RotaryArgs const& p, int slot)
+{
+    int first, second, pair;
+    int const pairSlots = p.half / V;
+    if (!ADJACENT && slot < pairSlots)
+    {
+        first = slot * V;
+        second = first + p.half;
+        pair = first;
+    }
+    else
+    {
+        int const base = ADJACENT ? 0 : 2 * p.half, n = ADJACENT ? slot : slot - pairSlots;
+        first = base + 2 * V * n;
+        second = first + V;
+        pair = ADJACENT ? V * n : p.half;
+    }
+    return {{first < p.d ? first : -1, second < p.d ? second : -1}, pair};
+}
+
+// Groups of G lanes take a head each.  NS slots a lane (V = 1: heads of more than 128 values).
+template <typename T, int V, int NS, int G, bool ADJACENT>
+__global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
+{
+    uint32_t const row = blockIdx.x * (256 / G) + threadIdx.x / G;
+    uint32_t const rows = (uint32_t) p.T * (uint32_t) p.heads;
+    uint32_t const live = min(row, rows - 1);
+    uint32_t const t = live / p.headsDiv;
+    int const h = (int) (live - t * p.headsDiv.d);
+    Side const& side = p.side[h < p.qHeads ? 0 : 1];
+    int const head = h < p.qHeads ? h : h - p.qHeads;
+    T const* in = static_cast<T const*>(side.in) + (int64_t) t * side.inToken + (int64_t) head * side.inHead;
+    T* out = static_cast<T*>(side.out) + (int64_t) t * side.outToken + (int64_t) head * side.outHead;
+
+    float x[NS][2][V];
+    Slot slots[NS];
+    float sum = 0.f, squares = 0.f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+    {
+        slots[n] = slot_of<V, ADJACENT>(p, (int) (threadIdx.x % G) + n * G);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+        {
+            int const at = slots[n].at[c];
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+            {
+                x[n][c][e] = 0.f;
+            }
+            if (at >= 0)
+            {
+                load_values<V>(in + at, x[n][c]);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+            {
+                sum += x[n][c][e];
+                squares = fmaf(x[n][c][e], x[n][c][e], squares);
+            }
+        }
+    }
+    auto const add = [](float a, float b) { return a + b; };
+    if (p.norm != TRTAMD_QK_NORM_NONE)
+    {
+        float const n = (float) p.d;
+        float mean = 0.f;
+        if (p.norm == TRTAMD_QK_NORM_LAYER)
+        {
+            mean = group_allreduce<G>(sum, add) / n;
+            squares = 0.f;
+#pragma unroll
+            for (int k = 0; k < NS; ++k)
+            {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                    {
+                        float const dev = slots[k].at[c] >= 0 ? x[k][c][e] - mean : 0.f;
+                        squares = fmaf(dev, dev, squares);
+                    }
+                }
+            }
+        }
+        float const scale = 1.f / sqrtf(group_allreduce<G>(squares, add) / n + p.eps);
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+        {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+            {
+                int const at = slots[k].at[c];
+                if (at < 0)
+                {
+                    continue;
+                }
+                float w[V], b[V];
+                load_values<V>(side.weight + at, w);
+                if (p.norm == TRTAMD_QK_NORM_LAYER)
+                {
+                    load_values<V>(side.bias + at, b);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    float const y = (x[k][c][e] - mean) * scale;
+                    x[k][c][e] = p.norm == TRTAMD_QK_NORM_LAYER ? fmaf(y, w[e], b[e]) : y * w[e];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+    {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+        {
+            int const pair = slots[k].pair + e;
+            if (pair < p.half)
+            {
+                float c, s;
+                cos_sin(p.positions[(int64_t) axis_of(p, pair) * p.T + t], p.frequencies[pair], c, s);
+                float& a = ADJACENT ? x[k][2 * e / V][2 * e % V] : x[k][0][e];
+                float& b = ADJACENT ? x[k][(2 * e + 1) / V][(2 * e + 1) % V] : x[k][1][e];
+                float const ra = a * c - b * s, rb = b * c + a * s;
+                a = ra;
+                b = rb;
+            }
+        }
+    }
+    if (row >= rows)
+    {
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+    {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+        {
+            if (slots[k].at[c] >= 0)
+            {
+                store_values<V>(out + slots[k].at[c], x[k][c]);
+            }
+        }
+    }
+}
+
+template <typename T, int V, int NS, int G>
+int launch_group(hipStream_t stream, RotaryArgs const& a, bool adjacent)
+{
+    dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, 256 / G));
+    if (adjacent)
+    {
+        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, true>), grid, dim3(256), 0, stream, a);
+    }
+    else
+    {
+        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, false>), grid, dim3(256), 0, stream, a);
+    }
+    return check_launch("qk_norm_rotary_kernel");
+}
+
+// Slots of a head: pairs of chunks.
+int slots_of(RotaryArgs const& a, int V)
+{
+    return a.adjacent ? ceil_div(a.d, 2 * V) : a.half / V + ceil_div(a.d - 2 * a.half, 2 * V);
+}
+
+template <typename T, int V>
+int launch_width(hipStream_t stream, RotaryArgs const& a)
+{
+    int const slots = slots_of(a, V);
+    bool const adj = a.adjacent != 0;
+    if constexpr (V == 1)
+    {
+        return slots <= 64 ? launch_group<T, V, 1, 64>(stream, a, adj) : launch_group<T, V, 2, 64>(stream, a, adj);
+    }
+    else
+    {
+        if (slots <= 4)
+        {
+            return launch_group<T, V, 1, 4>(stream, a, adj);
+        }
+        if (slots <= 8)
+        {
+            return launch_group<T, V, 1, 8>(stream, a, adj);
+        }
+        if (slots <= 16)
+        {
+            return launch_group<T, V, 1, 16>(stream, a, adj);
+        }
+        return launch_group<T, V, 1, 32>(stream, a, adj);
+    }
+}
+
+// Whether chunks of V values start at multiples of their size everywhere.
+template <typename T>
+bool fits(RotaryArgs const& a, int V)
+{
+    auto const aligned = [](void const* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; };
+    bool ok = a.d % V == 0 && (a.adjacent || a.half % V == 0);
+    for (int i = 0; i < 2; ++i)
+    {
+        if (i == 0 ? a.qHeads == 0 : a.heads == a.qHeads)
+        {
+            continue;
+        }
+        Side const& s = a.side[i];
+        ok = ok && aligned(s.in, V * sizeof(T)) && aligned(s.out, V * sizeof(T)) && s.inToken % V == 0 && s.inHead % V == 0
+            && s.outToken % V == 0 && s.outHead % V == 0 && aligned(s.weight, 16) && aligned(s.bias, 16);
+    }
+    return ok;
+}
+
+template <typename T>
+int launch_type(hipStream_t stream, RotaryArgs const& a)
+{
+    if constexpr (sizeof(T) == 2)
+    {
+        if (fits<T>(a, 8))
+        {
+            return launch_width<T, 8>(stream, a);
+        }
+    }
+    return fits<T>(a, 4) ? launch_width<T, 4>(stream, a) : launch_width<T, 1>(stream, a);
+}
+
+int bad(char const* what)
+{
+    return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: %s", what);
+}
+
+int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
+{
+    if (type != 0 && type != 1)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: data type %d (0 = FP32, 1 = FP16)", type);
+    }
+    if (p == nullptr)
+    {
+        return bad("null pointer");
+    }
+    if (p->T < 0 || p->q_heads < 0 || p->k_heads < 0 || p->d < 1 || p->d > TRTAMD_ROTARY_MAX_HEAD)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: T=%d q_heads=%d k_heads=%d d=%d (d of 1 to %d)", p->T,
+            p->q_heads, p->k_heads, p->d, (int) TRTAMD_ROTARY_MAX_HEAD);
+    }
+    if (p->norm < TRTAMD_QK_NORM_NONE || p->norm > TRTAMD_QK_NORM_LAYER)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: unknown norm %d", p->norm);
+    }
+    if (p->norm != TRTAMD_QK_NORM_NONE && !(p->eps >= 0.f))
+    {
+        return bad("eps must not be negative");
+    }
+    if (p->rotary_dim < 0 || p->rotary_dim > p->d || p->rotary_dim % 2 != 0)
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: rotary_dim=%d (even, 0 to d=%d)", p->rotary_dim, p->d);
+    }
+    bool const rotates = p->rotary_dim > 0, norms = p->norm != TRTAMD_QK_NORM_NONE;
+    if (!rotates && !norms)
+    {
+        return bad("neither a norm nor a rotation");
+    }
+    size_t const size = type == 1 ? 2 : 4;
+    for (int i = 0; i < 2; ++i)
+    {
+        bool const q = i == 0;
+        if ((q ? p->q_heads : p->k_heads) == 0 || p->T == 0) // tensors without a token may have no address
+        {
+            continue;
+        }
+        void const* const data[2] = {q ? p->q : p->k, q ? p->q_out : p->k_out};
+        float const* const vectors[2] = {q ? p->q_weight : p->k_weight, q ? p->q_bias : p->k_bias};
+        if (data[0] == nullptr || data[1] == nullptr || (norms && vectors[0] == nullptr)
+            || (p->norm == TRTAMD_QK_NORM_LAYER && vectors[1] == nullptr))
+        {
+            return bad("null pointer");
+        }
+        for (int j = 0; j < 2; ++j)
+        {
+            if (reinterpret_cast<uintptr_t>(data[j]) % size != 0 || reinterpret_cast<uintptr_t>(vectors[j]) % 4 != 0)
+            {
+                return bad("pointers must be aligned to their values");
+            }
+        }
+    }
+    if (rotates)
+    {
+        if (p->T > 0 && (p->frequencies == nullptr || p->positions == nullptr))
+        {
+            return bad("null pointer");
+        }
+        if (reinterpret_cast<uintptr_t>(p->frequencies) % 4 != 0 || reinterpret_cast<uintptr_t>(p->positions) % 4 != 0)
+        {
+            return bad("pointers must be aligned to their values");
+        }
+        if (p->axes < 1 || p->axes > TRTAMD_ROTARY_MAX_AXES)
+        {
+            return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: axes=%d (1 to %d)", p->axes, (int) TRTAMD_ROTARY_MAX_AXES);
+        }
+        int const pairs = p->rotary_dim / 2;
+        int64_t sum = 0;
+        for (int i = 0; i < p->axes && p->axes > 1; ++i)
+        {
+            int const n = p->sections[i];
+            sum += n;
+            // the last turn of an axis has to be a pair
+            if (n < 0 || n > pairs || (p->axes_cycled && i > 0 && n > 0 && (n - 1) * p->axes + i >= pairs))
+            {
+                return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: sections[%d]=%d of %d pairs", i, n, pairs);
+            }
+        }
+        if (p->axes > 1 && sum != pairs)
+        {
+            return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: sections of %lld pairs, rotary_dim has %d", (long long) sum, pairs);
+        }
+    }
+    if ((int64_t) p->T * ((int64_t) p->q_heads + p->k_heads) >= (int64_t) 1 << 31)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: 2^31 heads or more");
+    }
+    return TRTAMD_STATUS_SUCCESS;
+}
+
+} // namespace
+} // namespace trtamd
+
+using namespace trtamd;
+
+extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, trtamd_qk_norm_rotary_params const* p)
+{
+    int const st = check(data_type, p);
+    if (st != TRTAMD_STATUS_SUCCESS || p->T == 0 || p->q_heads + p->k_heads == 0)
+    {
+        return st;
+    }
+    RotaryArgs a{};
+    bool const norms = p->norm != TRTAMD_QK_NORM_NONE, layer = p->norm == TRTAMD_QK_NORM_LAYER;
+    a.side[0] = {p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride,
+        norms ? p->q_weight : nullptr, layer ? p->q_bias : nullptr};
+    a.side[1] = {p->k, p->k_out, p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride,
+        norms ? p->k_weight : nullptr, layer ? p->k_bias : nullptr};
+    a.T = p->T;
+    a.qHeads = p->q_heads;
+    a.heads = p->q_heads + p->k_heads;
+    a.d = p->d;
+    a.norm = p->norm;
+    a.eps = p->eps;
+    a.half = p->rotary_dim / 2;
+    a.adjacent = p->adjacent_pairs != 0;
+    a.frequencies = p->frequencies;
+    a.positions = p->positions;
+    a.axes = p->axes;
+    a.cycled = p->axes_cycled != 0;
+    for (int i = 0; i < p->axes && p->axes > 1 && a.half > 0; ++i)
+    {
+        a.sections[i] = p->sections[i];
+    }
+    a.headsDiv = fast_div((uint32_t) a.heads);
+    return data_type == 1 ? launch_type<f16>(as_stream(stream), a) : launch_type<float>(as_stream(stream), a);
+}

@@ -1,0 +1,371 @@
+"""Quantisation with a scale for each token and the INT8 linear layers on it, against the definitions in binary64.
+
+Tolerances.  The quantised values are exact, and so is the scale (one binary32 division).  A layer's result is formed in binary32: the
+accumulator's conversion, its products with the two scales and the addition of the bias round at most four times, each to 2^-24 of the
+product p or of the sum (which is no more than |p| + |bias|); GELU's slope is at most 1.13, and its polynomial is within 4.1e-6 of the value
+or 2.5e-10.  One rounding to binary16 follows: half a step, 2^-11 of the value or 2^-25, whichever is more."""
+import ctypes as C
+
+import numpy as np
+import pytest
+from scipy.special import ndtr
+
+from helpers import dev, dev_empty, host, ptr, rng, stream, sync
+from tensorrt_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def api():
+    return capi.api()
+
+
+def activations(r, T, K):
+    x = r.standard_normal((T, K)) * np.exp(0.5 * r.standard_normal((T, 1)))
+    x[:, r.random(K) < 0.02] *= 10
+    return x.astype(np.float16)
+
+
+def quantised(x):
+    """(values, scales) of the definition; rows that are not finite become zeros with scale NaN."""
+    wide = x.astype(np.float64)
+    amax = np.abs(wide).max(1)
+    finite = np.isfinite(amax)
+    safe = np.where(finite & (amax > 0), amax, 1.0)
+    q = np.rint(np.where(finite[:, None], wide, 0.0) * 127 / safe[:, None]).astype(np.int8)
+    return q, np.where(finite, amax.astype(np.float32) / np.float32(127), np.float32(np.nan))
+
+
+def run_quantise(api, x, view=None, s=None):
+    T, K = x.shape
+    d = dev(x) if view is None else view
+    q, scales = dev_empty((T + 1, K), np.int8, fill=77), dev_empty((T + 1,), np.float32, fill=-7)
+    api.check(api.quantize_fp16_per_token(s or stream(), T, K, ptr(d), d.stride(0), ptr(q), ptr(scales)))
+    sync()
+    q, scales = host(q), host(scales)
+    assert (q[T] == 77).all() and scales[T] == -7, "something behind the last token was written"
+    return q[:T], scales[:T]
+
+
+def reference(q, scales, w, channel, bias, gelu):
+    """(result, tolerance)."""
+    p = (q.astype(np.float64) @ w.astype(np.float64).T) * scales.astype(np.float64)[:, None] * channel.astype(np.float64)
+    b = np.zeros(w.shape[0]) if bias is None else bias.astype(np.float64)
+    y = p + b
+    off = 4 * 2.0 ** -24 * (np.abs(p) + np.abs(b))
+    if gelu:
+        y, off = y * ndtr(y), 1.13 * off
+        off += 4.1e-6 * np.abs(y) + 2.5e-10
+    return y, off + np.maximum(2.0 ** -11 * (np.abs(y) + off), 2.0 ** -25)
+
+
+def assert_within(got, want, tol, what=""):
+    got = got.astype(np.float64)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (f"{what}: {bad.sum()} of {bad.size} outside, first at {np.argwhere(bad)[0]}: "
+                           f"{got[bad][0]} for {want[bad][0]} +- {tol[bad][0]}")
+
+
+def weights(r, N, K):
+    w = r.integers(-127, 128, (N, K)).astype(np.int8)
+    channel = (r.uniform(0.5, 1.5, N) / (73 * np.sqrt(K))).astype(np.float32)
+    return w, channel, (0.3 * r.standard_normal(N)).astype(np.float32)
+
+
+def params(cls, T, K, N, gelu, w, channel, bias, out, **more):
+    p = cls(w=ptr(w), channel_scale=ptr(channel), bias=ptr(bias), out=ptr(out), T=T, K=K, N=N,
+            epilogue=capi.LINEAR_GELU if gelu else capi.LINEAR_AFFINE)
+    for k, v in more.items():
+        setattr(p, k, v)
+    return p
+
+
+class Layer:
+    """Device operands of one layer; the output has a row behind its last one that must stay as it is."""
+
+    def __init__(self, api, T, K, N, gelu=False, bias=True, seed=0, x=None):
+        r = rng([T, K, N, seed])
+        self.api, self.sizes, self.gelu = api, (T, K, N), gelu
+        self.x = activations(r, T, K) if x is None else x
+        self.w, self.channel, b = weights(r, N, K)
+        self.bias = b if bias else None
+        self.dx, self.dw, self.dc = dev(self.x), dev(self.w), dev(self.channel)
+        self.db = dev(self.bias) if bias else None
+
+    def want(self):
+        q, scales = quantised(self.x)
+        return reference(q, scales, self.w, self.channel, self.bias, self.gelu)
+
+    def out(self):
+        return dev_empty((self.sizes[0] + 1, self.sizes[2]), np.float16, fill=-7)
+
+    def token(self, out, s=None):
+        q, scales = quantised(self.x)
+        self.dq, self.ds = dev(q), dev(scales)
+        p = params(capi.Int8TokenLinearParams, *self.sizes, self.gelu, self.dw, self.dc, self.db, out, a=ptr(self.dq),
+                   token_scale=ptr(self.ds))
+        self.api.check(self.api.int8_token_linear(s or stream(), C.byref(p)))
+
+    def workspace(self):
+        return dev_empty((self.api.int8_dynamic_linear_workspace_size(*self.sizes),), np.uint8, fill=0xAB)
+
+    def dynamic(self, out, ws, s=None, view=None):
+        x = self.dx if view is None else view
+        p = params(capi.Int8DynamicLinearParams, *self.sizes, self.gelu, self.dw, self.dc, self.db, out, a=ptr(x),
+                   a_stride=x.stride(0), workspace=ptr(ws), workspace_bytes=ws.numel())
+        self.api.check(self.api.int8_dynamic_linear(s or stream(), C.byref(p)))
+
+
+def bits(t):
+    return host(t).view(np.uint16)
+
+
+# ---- the quantiser -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("C_", [32, 64, 96, 256, 480, 512, 544, 768, 1024, 1056, 2048, 2080, 4096, 4128, 8192, 8224, 16384, 33024])
+@pytest.mark.parametrize("T", [1, 2, 3, 5, 37])
+def test_quantiser(api, T, C_):
+    x = activations(rng(T * 100000 + C_), T, C_)
+    got, want = run_quantise(api, x), quantised(x)
+    assert np.array_equal(got[0], want[0])
+    assert np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("T,C_", [(4099, 96), (1000, 1024), (777, 4096), (20011, 64)])
+def test_quantiser_many_tokens(api, T, C_):
+    x = activations(rng(T + C_), T, C_)
+    got, want = run_quantise(api, x), quantised(x)
+    assert np.array_equal(got[0], want[0])
+    assert np.array_equal(got[1], want[1])
+
+
+def test_quantiser_ties_and_every_pair_of_maximum_and_value(api):
+    """Half-way quotients are those of the definition: for many maxima, every finite binary16 value up to the maximum."""
+    r = rng(5)
+    values = np.arange(0x7c00, dtype=np.uint16).view(np.float16)
+    maxima = np.concatenate([values[r.integers(1, 0x7c00, 60)], values[[1, 2, 3, 1023, 1024, 0x7bff]],
+                             np.float16([127, 254, 127 / 1024, 1, 0.5, 63.5, 95.25])])
+    for top in maxima:
+        x = values[values <= top]
+        x = np.concatenate([x, -x, np.zeros(-2 * len(x) % 32, np.float16)])
+        x = np.stack([x, x[::-1]])
+        got, want = run_quantise(api, x), quantised(x)
+        assert np.array_equal(got[0], want[0]), top
+        assert np.array_equal(got[1], want[1]), top
+
+
+@pytest.mark.parametrize("C_", [64, 768, 4096, 20000])
+def test_quantiser_zeros_and_values_that_are_not_finite(api, C_):
+    x = activations(rng(C_), 11, C_)
+    x[1] = 0
+    x[3, C_ - 1] = np.nan
+    x[4, 0] = np.inf
+    x[6, C_ // 2] = -np.inf
+    x[7] = -0.0
+    x[8] = 0
+    x[8, 5] = 2.0 ** -24
+    x[9] = np.nan
+    x[10] = 65504
+    q, s = run_quantise(api, x)
+    wq, ws = quantised(x)
+    assert np.array_equal(q, wq)
+    assert np.array_equal(s.view(np.uint32)[np.isfinite(ws)], ws.view(np.uint32)[np.isfinite(ws)])
+    assert np.isnan(s[[3, 4, 6, 9]]).all() and s[1] == s[7] == 0
+
+
+def test_quantiser_of_strided_rows(api):
+    """Rows that lie between others: the middle of a wider tensor, and every second row."""
+    wide = activations(rng(3), 54, 1600)
+    d = dev(wide)
+    for view, x in ((d[:, 512:512 + 1024], wide[:, 512:512 + 1024]), (d[::2, 8:8 + 96], wide[::2, 8:8 + 96])):
+        got, want = run_quantise(api, np.ascontiguousarray(x), view), quantised(x)
+        assert np.array_equal(got[0], want[0])
+        assert np.array_equal(got[1], want[1])
+
+
+def test_quantiser_beyond_32_bits(api):
+    """More than 2^32 bytes of input and 2^31 of output."""
+    import torch
+    T, C_ = 70001, 32768
+    x = torch.zeros((T, C_), dtype=torch.float16, device="cuda")
+    tail = activations(rng(9), 3, C_)
+    x[-3:] = dev(tail)
+    q = torch.full((T, C_), 77, dtype=torch.int8, device="cuda")
+    scales = torch.empty((T,), dtype=torch.float32, device="cuda")
+    api.check(api.quantize_fp16_per_token(stream(), T, C_, ptr(x), C_, ptr(q), ptr(scales)))
+    sync()
+    want = quantised(tail)
+    assert np.array_equal(host(q[-3:]), want[0]) and np.array_equal(host(scales[-3:]), want[1])
+    assert not q[:-3].any() and not scales[:-3].any()
+
+
+# ---- the layers --------------------------------------------------------------------------------------------------
+
+SHAPES = [(1, 64, 32), (1, 1024, 1024), (2, 768, 2304), (3, 4096, 1024), (4, 128, 4096), (5, 192, 96), (7, 1088, 544), (8, 1024, 4096),
+          (9, 512, 512), (16, 4096, 1024), (17, 64, 4128), (31, 128, 64), (33, 320, 160), (40, 4096, 1024), (64, 768, 768), (100, 1024, 288),
+          (129, 192, 32), (257, 1024, 1024), (777, 768, 2304), (1000, 4096, 1024), (2049, 384, 1536), (4099, 1024, 4096)]
+
+
+@pytest.mark.parametrize("T,K,N", SHAPES)
+@pytest.mark.parametrize("gelu,bias", [(False, True), (False, False), (True, True), (True, False)])
+def test_layers(api, T, K, N, gelu, bias):
+    layer = Layer(api, T, K, N, gelu, bias)
+    want, tol = layer.want()
+    one, two = layer.out(), layer.out()
+    layer.token(one)
+    layer.dynamic(two, layer.workspace())
+    sync()
+    assert_within(host(one)[:T], want, tol, f"token {T} {K} {N}")
+    assert (host(one)[T] == -7).all() and (host(two)[T] == -7).all(), "something behind the last token was written"
+    assert np.array_equal(bits(one), bits(two)), "the two entry points differ"
+
+
+PLANS = range(1, 15)
+
+
+@pytest.mark.parametrize("T,K,N", [(300, 256, 288), (130, 192, 160), (61, 128, 96)])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_every_plan_gives_the_same_bits(api, T, K, N, gelu):
+    layer = Layer(api, T, K, N, gelu)
+    want, tol = layer.want()
+    first = layer.out()
+    layer.token(first)
+    sync()
+    assert_within(host(first)[:T], want, tol)
+    try:
+        for plan in PLANS:
+            api.check(api.test_set_tuning(b"TRTAMD_LINEAR_PLAN", plan))
+            out = layer.out()
+            layer.token(out)
+            sync()
+            assert np.array_equal(bits(out), bits(first)), f"plan {plan}"
+        api.check(api.test_reset_tuning(b"TRTAMD_LINEAR_PLAN"))
+        for switch in (b"TRTAMD_LINEAR_DIRECT", b"TRTAMD_LINEAR_PERSISTENT"):
+            api.check(api.test_set_tuning(switch, 0))
+            out = layer.out()
+            layer.token(out)
+            sync()
+            assert np.array_equal(bits(out), bits(first)), switch
+            api.check(api.test_reset_tuning(switch))
+    finally:
+        for switch in (b"TRTAMD_LINEAR_PLAN", b"TRTAMD_LINEAR_DIRECT", b"TRTAMD_LINEAR_PERSISTENT"):
+            api.test_reset_tuning(switch)
+
+
+@pytest.mark.parametrize("T,K,N", [(6, 1024, 1024), (70, 256, 96), (700, 1024, 1024)])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_tokens_that_are_not_finite_stay_by_themselves(api, T, K, N, gelu):
+    x = activations(rng(T), T, K)
+    x[1, 3], x[T - 1, K - 1], x[2] = np.nan, -np.inf, 0
+    layer = Layer(api, T, K, N, gelu, x=x)
+    want, tol = layer.want()
+    one, two = layer.out(), layer.out()
+    layer.token(one)
+    layer.dynamic(two, layer.workspace())
+    sync()
+    for out in (host(one)[:T], host(two)[:T]):
+        assert np.isnan(out[[1, T - 1]]).all()
+        rows = [t for t in range(T) if t not in (1, T - 1)]
+        assert_within(out[rows], want[rows], tol[rows])
+
+
+def test_large_accumulators(api):
+    """Sums beyond 2^24, which a binary32 no longer holds exactly, and the largest in either direction."""
+    T, K, N = 3, 8192, 64
+    x = np.full((T, K), 3, np.float16)
+    x[1] = -3
+    x[2, ::2] = -1
+    layer = Layer(api, T, K, N, x=x)
+    layer.w = np.full((N, K), 127, np.int8)
+    layer.w[1::2] = -127
+    layer.w[5, :77] = 1
+    layer.channel = np.full(N, 2e-5, np.float32)
+    layer.dw, layer.dc = dev(layer.w), dev(layer.channel)
+    want, tol = layer.want()
+    out = layer.out()
+    layer.dynamic(out, layer.workspace())
+    sync()
+    assert_within(host(out)[:T], want, tol)
+
+
+def test_results_beyond_binary16_are_infinities(api):
+    layer = Layer(api, 4, 128, 64)
+    layer.channel = np.full(64, 1e4, np.float32)
+    layer.dc = dev(layer.channel)
+    want, _ = layer.want()
+    out = layer.out()
+    layer.dynamic(out, layer.workspace())
+    sync()
+    got = host(out)[:4]
+    large = np.abs(want) > 70000
+    assert large.any() and np.array_equal(got[large], np.sign(want[large]) * np.inf)
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 1024, 512), (90, 256, 288), (1500, 512, 256)])
+def test_strided_tokens(api, T, K, N):
+    import torch
+    layer = Layer(api, T, K, N)
+    wide = torch.full((T, 2 * K + 8), float("nan"), dtype=torch.float16, device="cuda")
+    wide[:, 8:8 + K] = layer.dx
+    one, two = layer.out(), layer.out()
+    layer.dynamic(one, layer.workspace())
+    layer.dynamic(two, layer.workspace(), view=wide[:, 8:8 + K])
+    sync()
+    assert np.array_equal(bits(one), bits(two))
+
+
+@pytest.mark.parametrize("T,K,N", [(33, 1024, 2048), (3, 768, 512)])
+def test_a_token_does_not_depend_on_its_neighbours(api, T, K, N):
+    """Each token by itself, through the kernels of single tokens, gives the bits it has in the batch."""
+    layer = Layer(api, T, K, N, gelu=True)
+    out = layer.out()
+    layer.dynamic(out, layer.workspace())
+    for t in (0, 1, T - 1):
+        single = Layer(api, 1, K, N, gelu=True, x=layer.x[t:t + 1])
+        single.w, single.dw, single.dc, single.db = layer.w, layer.dw, layer.dc, layer.db
+        alone = single.out()
+        single.dynamic(alone, single.workspace())
+        sync()
+        assert np.array_equal(bits(alone)[0], bits(out)[t]), t
+
+
+def test_two_calls_at_once_on_streams_of_their_own(api):
+    import torch
+    layers = [Layer(api, 600, 1024, 1024, seed=1), Layer(api, 2, 2048, 1024, gelu=True, seed=2)]
+    want = [l.out() for l in layers]
+    for l, o in zip(layers, want):
+        l.dynamic(o, l.workspace())
+    sync()
+    streams, outs, spaces = [torch.cuda.Stream() for _ in layers], [l.out() for l in layers], [l.workspace() for l in layers]
+    sync()
+    for _ in range(10):
+        for l, o, ws, s in zip(layers, outs, spaces, streams):
+            l.dynamic(o, ws, s.cuda_stream)
+    sync()
+    for o, w in zip(outs, want):
+        assert np.array_equal(bits(o), bits(w))
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 1024, 1024), (12, 1024, 1024), (500, 768, 768)])
+def test_captured_and_replayed(api, T, K, N):
+    """A captured call follows what its input holds at each replay, with eager calls on the same operands between the replays."""
+    import torch
+    layer = Layer(api, T, K, N, gelu=True)
+    out, eager, ws, other = layer.out(), layer.out(), layer.workspace(), layer.workspace()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    sync()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            layer.dynamic(out, ws, side.cuda_stream)
+    for replay in range(3):
+        layer.x = activations(rng(replay + 50), T, K)
+        layer.dx.copy_(dev(layer.x))
+        out.fill_(-7)
+        layer.dynamic(eager, other)
+        graph.replay()
+        sync()
+        assert np.array_equal(bits(out), bits(eager)), replay
+        want, tol = layer.want()
+        assert_within(host(out)[:T], want, tol)
+    del graph
