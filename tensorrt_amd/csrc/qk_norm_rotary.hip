@@ -33,7 +33,8 @@ struct RotaryArgs
     int32_t const* positions;
     int axes, cycled;
     int sections[TRTAMD_ROTARY_MAX_AXES];
-    FastDiv headsDiv;
+    FastDiv headsDiv, halfDiv;
+    int pitch; // of the cosines and sines of a token in LDS: pairs in whole chunks
 };
 
 __device__ inline int axis_of(RotaryArgs const& p, int pair)
@@ -74,7 +75,7 @@ __device__ inline void cos_sin(int32_t position, float frequency, float& c, floa
 
 // V values of T as binary32.
 template <int V, typename T>
-__device__ inline void load_values(T const* p, float (&v)[V])
+__device__ __forceinline__ void load_values(T const* p, float (&v)[V])
 {
     if constexpr (V == 1)
     {
@@ -141,14 +142,18 @@ __device__ inline Slot slot_of(RotaryArgs const& p, int slot)
     return {{first < p.d ? first : -1, second < p.d ? second : -1}, pair};
 }
 
-// Groups of G lanes take a head each.  NS slots a lane (V = 1: heads of more than 128 values).
+// A workgroup takes 256 / G rows (a row: a head of a token), G lanes each, NS slots a lane (V = 1: heads of more than 128 values).  Rows are
+// numbered token by token, so its rows are heads of few tokens: their cosines and sines are worked out once, a thread each,
+// while the rows are on their way, and shared through LDS.
 template <typename T, int V, int NS, int G, bool ADJACENT>
 __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 {
-    uint32_t const row = blockIdx.x * (256 / G) + threadIdx.x / G;
+    constexpr int kRows = 256 / G;
+    extern __shared__ __attribute__((aligned(16))) float lds[]; // [token][cosines | sines][pairs], pairs padded to whole chunks
     uint32_t const rows = (uint32_t) p.T * (uint32_t) p.heads;
+    uint32_t const first = blockIdx.x * (uint32_t) kRows, row = first + threadIdx.x / G;
     uint32_t const live = min(row, rows - 1);
-    uint32_t const t = live / p.headsDiv;
+    uint32_t const t0 = first / p.headsDiv, t = live / p.headsDiv;
     int const h = (int) (live - t * p.headsDiv.d);
     Side const& side = p.side[h < p.qHeads ? 0 : 1];
     int const head = h < p.qHeads ? h : h - p.qHeads;
@@ -157,7 +162,6 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 
     float x[NS][2][V];
     Slot slots[NS];
-    float sum = 0.f, squares = 0.f;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
     {
@@ -175,23 +179,29 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
             {
                 load_values<V>(in + at, x[n][c]);
             }
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-            {
-                sum += x[n][c][e];
-                squares = fmaf(x[n][c][e], x[n][c][e], squares);
-            }
         }
+    }
+    if (p.half > 0)
+    {
+        uint32_t const tokens = min(first + (uint32_t) kRows - 1, rows - 1) / p.headsDiv - t0 + 1;
+        for (uint32_t i = threadIdx.x; i < tokens * (uint32_t) p.half; i += 256)
+        {
+            uint32_t const token = i / p.halfDiv;
+            int const pair = (int) (i - token * p.halfDiv.d);
+            float c, s;
+            cos_sin(p.positions[(int64_t) axis_of(p, pair) * p.T + (t0 + token)], p.frequencies[pair], c, s);
+            lds[token * 2 * p.pitch + pair] = c;
+            lds[(token * 2 + 1) * p.pitch + pair] = s;
+        }
+        __syncthreads();
     }
     auto const add = [](float a, float b) { return a + b; };
     if (p.norm != TRTAMD_QK_NORM_NONE)
     {
-        float const n = (float) p.d;
         float mean = 0.f;
         if (p.norm == TRTAMD_QK_NORM_LAYER)
         {
-            mean = group_allreduce<G>(sum, add) / n;
-            squares = 0.f;
+            float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < NS; ++k)
             {
@@ -201,13 +211,28 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 #pragma unroll
                     for (int e = 0; e < V; ++e)
                     {
-                        float const dev = slots[k].at[c] >= 0 ? x[k][c][e] - mean : 0.f;
-                        squares = fmaf(dev, dev, squares);
+                        sum += x[k][c][e];
                     }
                 }
             }
+            mean = group_allreduce<G>(sum, add) / (float) p.d;
         }
-        float const scale = 1.f / sqrtf(group_allreduce<G>(squares, add) / n + p.eps);
+        float squares = 0.f;
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+        {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+            {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    x[k][c][e] = slots[k].at[c] >= 0 ? x[k][c][e] - mean : 0.f;
+                    squares = fmaf(x[k][c][e], x[k][c][e], squares);
+                }
+            }
+        }
+        float const scale = 1.f / sqrtf(group_allreduce<G>(squares, add) / (float) p.d + p.eps);
 #pragma unroll
         for (int k = 0; k < NS; ++k)
         {
@@ -228,7 +253,7 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 #pragma unroll
                 for (int e = 0; e < V; ++e)
                 {
-                    float const y = (x[k][c][e] - mean) * scale;
+                    float const y = x[k][c][e] * scale;
                     x[k][c][e] = p.norm == TRTAMD_QK_NORM_LAYER ? fmaf(y, w[e], b[e]) : y * w[e];
                 }
             }
@@ -237,19 +262,22 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 #pragma unroll
     for (int k = 0; k < NS; ++k)
     {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
+        int const pair = slots[k].pair;
+        if (pair < p.half)
         {
-            int const pair = slots[k].pair + e;
-            if (pair < p.half)
+            // chunks of V pairs begin at multiples of V; what lies behind the last pair of one (adjacent pairs) is not used
+            float c[V], s[V];
+            load_values<V>(lds + (t - t0) * 2 * p.pitch + pair, c);
+            load_values<V>(lds + ((t - t0) * 2 + 1) * p.pitch + pair, s);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
             {
-                float c, s;
-                cos_sin(p.positions[(int64_t) axis_of(p, pair) * p.T + t], p.frequencies[pair], c, s);
                 float& a = ADJACENT ? x[k][2 * e / V][2 * e % V] : x[k][0][e];
                 float& b = ADJACENT ? x[k][(2 * e + 1) / V][(2 * e + 1) % V] : x[k][1][e];
-                float const ra = a * c - b * s, rb = b * c + a * s;
-                a = ra;
-                b = rb;
+                float const ra = a * c[e] - b * s[e], rb = b * c[e] + a * s[e];
+                bool const turned = !ADJACENT || pair + e < p.half;
+                a = turned ? ra : a;
+                b = turned ? rb : b;
             }
         }
     }
@@ -272,16 +300,20 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 }
 
 template <typename T, int V, int NS, int G>
-int launch_group(hipStream_t stream, RotaryArgs const& a, bool adjacent)
+int launch_group(hipStream_t stream, RotaryArgs a, bool adjacent)
 {
-    dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, 256 / G));
+    constexpr int kRows = 256 / G;
+    dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, kRows));
+    a.pitch = ceil_div(a.half, V < 4 ? 4 : V) * (V < 4 ? 4 : V);
+    // the rows of a workgroup are heads of no more tokens than this
+    unsigned const lds = (unsigned) (2 * a.pitch * (ceil_div(kRows - 1, a.heads) + 1)) * sizeof(float);
     if (adjacent)
     {
-        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, true>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, true>), grid, dim3(256), lds, stream, a);
     }
     else
     {
-        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, false>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, false>), grid, dim3(256), lds, stream, a);
     }
     return check_launch("qk_norm_rotary_kernel");
 }
@@ -484,5 +516,6 @@ extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, 
         a.sections[i] = p->sections[i];
     }
     a.headsDiv = fast_div((uint32_t) a.heads);
+    a.halfDiv = fast_div((uint32_t) (a.half > 0 ? a.half : 1));
     return data_type == 1 ? launch_type<f16>(as_stream(stream), a) : launch_type<float>(as_stream(stream), a);
 }
