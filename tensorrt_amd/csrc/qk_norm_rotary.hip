@@ -27,7 +27,7 @@ struct RotaryArgs
     Side side[2]; // queries, keys
     int T, qHeads, heads, d; // heads: of queries and keys
     int norm;
-    float eps;
+    float eps, inverseD;
     int half, adjacent; // half: pairs
     float const* frequencies;
     int32_t const* positions;
@@ -73,23 +73,31 @@ __device__ inline void cos_sin(int32_t position, float frequency, float& c, floa
     sincospif(2.f * (float) (turns - rint(turns)), &s, &c);
 }
 
-// V values of T as binary32.
-template <int V, typename T>
-__device__ __forceinline__ void load_values(T const* p, float (&v)[V])
+template <typename T, int V>
+struct Chunk
+{
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+
+template <typename T>
+struct Chunk<T, 1>
+{
+    typedef T type;
+};
+
+template <typename T, int V>
+using ChunkT = typename Chunk<T, V>::type;
+
+template <int V, typename C>
+__device__ __forceinline__ float element(C const& c, int e)
 {
     if constexpr (V == 1)
     {
-        v[0] = (float) *p;
+        return (float) c;
     }
     else
     {
-        typedef T Vec __attribute__((ext_vector_type(V)));
-        Vec const x = *reinterpret_cast<Vec const*>(p);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-        {
-            v[e] = (float) x[e];
-        }
+        return (float) c[e];
     }
 }
 
@@ -145,7 +153,7 @@ __device__ inline Slot slot_of(RotaryArgs const& p, int slot)
 // A workgroup takes 256 / G rows (a row: a head of a token), G lanes each, NS slots a lane (V = 1: heads of more than 128 values).  Rows are
 // numbered token by token, so its rows are heads of few tokens: their cosines and sines are worked out once, a thread each,
 // while the rows are on their way, and shared through LDS.
-template <typename T, int V, int NS, int G, bool ADJACENT>
+template <typename T, int V, int NS, int G, bool ADJACENT, int NORM>
 __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 {
     constexpr int kRows = 256 / G;
@@ -154,14 +162,38 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
     uint32_t const first = blockIdx.x * (uint32_t) kRows, row = first + threadIdx.x / G;
     uint32_t const live = min(row, rows - 1);
     uint32_t const t0 = first / p.headsDiv, t = live / p.headsDiv;
-    int const h = (int) (live - t * p.headsDiv.d);
-    Side const& side = p.side[h < p.qHeads ? 0 : 1];
-    int const head = h < p.qHeads ? h : h - p.qHeads;
-    T const* in = static_cast<T const*>(side.in) + (int64_t) t * side.inToken + (int64_t) head * side.inHead;
-    T* out = static_cast<T*>(side.out) + (int64_t) t * side.outToken + (int64_t) head * side.outHead;
+    // Loads come back in the order in which they are asked for: first what the angles need, which are worked out while the rest
+    // is on its way.
+    uint32_t const angles = p.half > 0 ? (min(first + (uint32_t) kRows - 1, rows - 1) / p.headsDiv - t0 + 1) * (uint32_t) p.half : 0;
+    struct Angle
+    {
+        uint32_t token;
+        int pair;
+        int32_t position;
+        float frequency;
+    };
+    auto const load_angle = [&](uint32_t i) {
+        Angle a;
+        a.token = i / p.halfDiv;
+        a.pair = (int) (i - a.token * p.halfDiv.d);
+        a.frequency = p.frequencies[a.pair];
+        a.position = p.positions[(int64_t) axis_of(p, a.pair) * p.T + (t0 + a.token)];
+        return a;
+    };
+    Angle angle = {};
+    if (threadIdx.x < angles)
+    {
+        angle = load_angle(threadIdx.x);
+    }
 
-    float x[NS][2][V];
+    int const h = (int) (live - t * p.headsDiv.d);
+    bool const isQuery = h < p.qHeads;
+    Side const& side = p.side[isQuery ? 0 : 1];
+    int const head = isQuery ? h : h - p.qHeads;
+    T const* in = static_cast<T const*>(side.in) + (int64_t) t * side.inToken + (int64_t) head * side.inHead;
     Slot slots[NS];
+    ChunkT<T, V> raw[NS][2];
+    ChunkT<float, V> weight[NS][2], bias[NS][2];
 #pragma unroll
     for (int n = 0; n < NS; ++n)
     {
@@ -169,95 +201,74 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
         {
-            int const at = slots[n].at[c];
+            // a lane without a chunk reads the first one instead of waiting behind a branch
+            raw[n][c] = *reinterpret_cast<ChunkT<T, V> const*>(in + max(slots[n].at[c], 0));
+        }
+    }
 #pragma unroll
-            for (int e = 0; e < V; ++e)
+    for (int n = 0; NORM != TRTAMD_QK_NORM_NONE && n < NS; ++n)
+    {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+        {
+            weight[n][c] = *reinterpret_cast<ChunkT<float, V> const*>(side.weight + max(slots[n].at[c], 0));
+            if constexpr (NORM == TRTAMD_QK_NORM_LAYER)
             {
-                x[n][c][e] = 0.f;
-            }
-            if (at >= 0)
-            {
-                load_values<V>(in + at, x[n][c]);
+                bias[n][c] = *reinterpret_cast<ChunkT<float, V> const*>(side.bias + max(slots[n].at[c], 0));
             }
         }
     }
-    if (p.half > 0)
+    if (angles > 0) // uniform
     {
-        uint32_t const tokens = min(first + (uint32_t) kRows - 1, rows - 1) / p.headsDiv - t0 + 1;
-        for (uint32_t i = threadIdx.x; i < tokens * (uint32_t) p.half; i += 256)
+        for (uint32_t i = threadIdx.x; i < angles; i += 256)
         {
-            uint32_t const token = i / p.halfDiv;
-            int const pair = (int) (i - token * p.halfDiv.d);
+            if (i >= 256)
+            {
+                angle = load_angle(i);
+            }
             float c, s;
-            cos_sin(p.positions[(int64_t) axis_of(p, pair) * p.T + (t0 + token)], p.frequencies[pair], c, s);
-            lds[token * 2 * p.pitch + pair] = c;
-            lds[(token * 2 + 1) * p.pitch + pair] = s;
+            cos_sin(angle.position, angle.frequency, c, s);
+            float* const to = lds + angle.token * 2 * p.pitch + angle.pair;
+            to[0] = c;
+            to[p.pitch] = s;
         }
         __syncthreads();
     }
-    auto const add = [](float a, float b) { return a + b; };
-    if (p.norm != TRTAMD_QK_NORM_NONE)
+
+    float x[NS][2][V];
+    auto const each = [&](auto f) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+        {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+            {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    f(x[n][c][e], n, c, e);
+                }
+            }
+        }
+    };
+    each([&](float& v, int n, int c, int e) { v = slots[n].at[c] >= 0 ? element<V>(raw[n][c], e) : 0.f; });
+    if constexpr (NORM != TRTAMD_QK_NORM_NONE)
     {
-        float mean = 0.f;
-        if (p.norm == TRTAMD_QK_NORM_LAYER)
+        auto const add = [](float a, float b) { return a + b; };
+        if constexpr (NORM == TRTAMD_QK_NORM_LAYER)
         {
             float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < NS; ++k)
-            {
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                    {
-                        sum += x[k][c][e];
-                    }
-                }
-            }
-            mean = group_allreduce<G>(sum, add) / (float) p.d;
+            each([&](float& v, int, int, int) { sum += v; });
+            float const mean = group_allreduce<G>(sum, add) * p.inverseD;
+            each([&](float& v, int n, int c, int) { v = slots[n].at[c] >= 0 ? v - mean : 0.f; });
         }
         float squares = 0.f;
-#pragma unroll
-        for (int k = 0; k < NS; ++k)
-        {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-            {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                {
-                    x[k][c][e] = slots[k].at[c] >= 0 ? x[k][c][e] - mean : 0.f;
-                    squares = fmaf(x[k][c][e], x[k][c][e], squares);
-                }
-            }
-        }
-        float const scale = 1.f / sqrtf(group_allreduce<G>(squares, add) / (float) p.d + p.eps);
-#pragma unroll
-        for (int k = 0; k < NS; ++k)
-        {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-            {
-                int const at = slots[k].at[c];
-                if (at < 0)
-                {
-                    continue;
-                }
-                float w[V], b[V];
-                load_values<V>(side.weight + at, w);
-                if (p.norm == TRTAMD_QK_NORM_LAYER)
-                {
-                    load_values<V>(side.bias + at, b);
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                {
-                    float const y = x[k][c][e] * scale;
-                    x[k][c][e] = p.norm == TRTAMD_QK_NORM_LAYER ? fmaf(y, w[e], b[e]) : y * w[e];
-                }
-            }
-        }
+        each([&](float& v, int, int, int) { squares = fmaf(v, v, squares); });
+        float const scale = rsqrtf(fmaf(group_allreduce<G>(squares, add), p.inverseD, p.eps));
+        each([&](float& v, int n, int c, int e) {
+            float const w = element<V>(weight[n][c], e);
+            v = NORM == TRTAMD_QK_NORM_LAYER ? fmaf(v * scale, w, element<V>(bias[n][c], e)) : v * scale * w;
+        });
     }
 #pragma unroll
     for (int k = 0; k < NS; ++k)
@@ -266,15 +277,16 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
         if (pair < p.half)
         {
             // chunks of V pairs begin at multiples of V; what lies behind the last pair of one (adjacent pairs) is not used
-            float c[V], s[V];
-            load_values<V>(lds + (t - t0) * 2 * p.pitch + pair, c);
-            load_values<V>(lds + ((t - t0) * 2 + 1) * p.pitch + pair, s);
+            float const* const from = lds + (t - t0) * 2 * p.pitch + pair;
+            ChunkT<float, V> const cosines = *reinterpret_cast<ChunkT<float, V> const*>(from);
+            ChunkT<float, V> const sines = *reinterpret_cast<ChunkT<float, V> const*>(from + p.pitch);
 #pragma unroll
             for (int e = 0; e < V; ++e)
             {
                 float& a = ADJACENT ? x[k][2 * e / V][2 * e % V] : x[k][0][e];
                 float& b = ADJACENT ? x[k][(2 * e + 1) / V][(2 * e + 1) % V] : x[k][1][e];
-                float const ra = a * c[e] - b * s[e], rb = b * c[e] + a * s[e];
+                float const c = element<V>(cosines, e), s = element<V>(sines, e);
+                float const ra = a * c - b * s, rb = b * c + a * s;
                 bool const turned = !ADJACENT || pair + e < p.half;
                 a = turned ? ra : a;
                 b = turned ? rb : b;
@@ -285,6 +297,7 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
     {
         return;
     }
+    T* out = static_cast<T*>(side.out) + (int64_t) t * side.outToken + (int64_t) head * side.outHead;
 #pragma unroll
     for (int k = 0; k < NS; ++k)
     {
@@ -299,22 +312,25 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
     }
 }
 
+// One of the kernels for the norms.
+template <typename T, int V, int NS, int G, bool ADJACENT>
+auto kernel_of(int norm)
+{
+    return norm == TRTAMD_QK_NORM_NONE ? qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_NONE>
+        : norm == TRTAMD_QK_NORM_RMS  ? qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_RMS>
+                                      : qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_LAYER>;
+}
+
 template <typename T, int V, int NS, int G>
-int launch_group(hipStream_t stream, RotaryArgs a, bool adjacent)
+int launch_group(hipStream_t stream, RotaryArgs a)
 {
     constexpr int kRows = 256 / G;
     dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, kRows));
     a.pitch = ceil_div(a.half, V < 4 ? 4 : V) * (V < 4 ? 4 : V);
     // the rows of a workgroup are heads of no more tokens than this
     unsigned const lds = (unsigned) (2 * a.pitch * (ceil_div(kRows - 1, a.heads) + 1)) * sizeof(float);
-    if (adjacent)
-    {
-        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, true>), grid, dim3(256), lds, stream, a);
-    }
-    else
-    {
-        hipLaunchKernelGGL((qk_norm_rotary_kernel<T, V, NS, G, false>), grid, dim3(256), lds, stream, a);
-    }
+    auto const kernel = a.adjacent ? kernel_of<T, V, NS, G, true>(a.norm) : kernel_of<T, V, NS, G, false>(a.norm);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a);
     return check_launch("qk_norm_rotary_kernel");
 }
 
@@ -328,26 +344,25 @@ template <typename T, int V>
 int launch_width(hipStream_t stream, RotaryArgs const& a)
 {
     int const slots = slots_of(a, V);
-    bool const adj = a.adjacent != 0;
     if constexpr (V == 1)
     {
-        return slots <= 64 ? launch_group<T, V, 1, 64>(stream, a, adj) : launch_group<T, V, 2, 64>(stream, a, adj);
+        return slots <= 64 ? launch_group<T, V, 1, 64>(stream, a) : launch_group<T, V, 2, 64>(stream, a);
     }
     else
     {
         if (slots <= 4)
         {
-            return launch_group<T, V, 1, 4>(stream, a, adj);
+            return launch_group<T, V, 1, 4>(stream, a);
         }
         if (slots <= 8)
         {
-            return launch_group<T, V, 1, 8>(stream, a, adj);
+            return launch_group<T, V, 1, 8>(stream, a);
         }
-        if (slots <= 16)
+        if constexpr (V == 4) // 16 chunks of 8 pairs of values are 256
         {
-            return launch_group<T, V, 1, 16>(stream, a, adj);
+            return slots <= 16 ? launch_group<T, V, 1, 16>(stream, a) : launch_group<T, V, 1, 32>(stream, a);
         }
-        return launch_group<T, V, 1, 32>(stream, a, adj);
+        return launch_group<T, V, 1, 16>(stream, a);
     }
 }
 
@@ -505,6 +520,7 @@ extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, 
     a.d = p->d;
     a.norm = p->norm;
     a.eps = p->eps;
+    a.inverseD = 1.f / (float) p->d;
     a.half = p->rotary_dim / 2;
     a.adjacent = p->adjacent_pairs != 0;
     a.frequencies = p->frequencies;
