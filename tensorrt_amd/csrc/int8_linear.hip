@@ -29,6 +29,7 @@
 #include "device_utils.hpp"
 #include "host_utils.hpp"
 #include "network_ops.hpp"
+#include "token_ops.hpp"
 #include "trtamd_encoder_ops.h"
 #include "trtamd_test_hooks.h"
 
@@ -131,31 +132,6 @@ __device__ inline float gelu_erf(float y)
     return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
 }
 
-// The same for FP16 results, which need Phi(-a) to a relative error (y Phi(y) is small, not rounded away, for negative y):
-// a polynomial of degree 7 for log2(Phi(-a)) that is off by 4.5e-6 at most on [0, 5.5], behind which the result is below
-// half of the smallest binary16.  Within 4e-6 of the exact value where that is a normal binary16, 2.5e-10 elsewhere.  The leading coefficient is
-// negative, so the term vanishes for larger a; a NaN stays one (through a).
-__device__ inline float gelu_f16(float y)
-{
-    float const a = fabsf(y);
-    float p = fmaf(a, -1.793455226e-06f, 6.090417810e-05f);
-    p = fmaf(p, a, -9.260290535e-04f);
-    p = fmaf(p, a, 8.493757807e-03f);
-    p = fmaf(p, a, -5.393784493e-02f);
-    p = fmaf(p, a, -4.584805071e-01f);
-    p = fmaf(p, a, -1.151246786e+00f);
-    p = fmaf(p, a, -9.999954700e-01f);
-    return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
-}
-
-// The result of a token-scaled layer: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
-template <int EPI>
-__device__ __forceinline__ float token_result(int const acc, float const ts, float const al, float const be)
-{
-    float const y = fmaf((float) acc * ts, al, be);
-    return EPI == kTOKEN_GELU ? gelu_f16(y) : y;
-}
-
 template <int EPI>
 __device__ __forceinline__ float token_scale(LinearArgs const& p, int const t)
 {
@@ -245,7 +221,7 @@ __device__ __forceinline__ void pack_half_block(
         {
             if constexpr (token_scaled(EPI))
             {
-                h[e] = (f16) token_result<EPI>(acc[4 * g + e], ts, sc.al[g][e], sc.be[g][e]);
+                h[e] = (f16) token_result<EPI == kTOKEN_GELU>(acc[4 * g + e], ts, sc.al[g][e], sc.be[g][e]);
             }
             else
             {
@@ -1234,7 +1210,7 @@ __device__ __forceinline__ void store_quad(
         {
             if constexpr (token_scaled(EPI))
             {
-                h[e] = (f16) token_result<EPI>(acc[e], sc.ts, al[e], be[e]);
+                h[e] = (f16) token_result<EPI == kTOKEN_GELU>(acc[e], sc.ts, al[e], be[e]);
             }
             else
             {

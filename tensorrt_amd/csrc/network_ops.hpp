@@ -42,6 +42,10 @@ int fp16_linear_partial(trtamd_stream_t stream, trtamd_fp16_linear_params const&
 int fp16_linear_check(trtamd_fp16_linear_params const& p);
 // The same of trtamd_int8_token_linear, for trtamd_int8_dynamic_linear.
 int int8_token_linear_check(trtamd_int8_token_linear_params const& p);
+// The checks of trtamd_quantize_fp16_per_token, as those of `what`, and its launch without them.
+int token_quantize_check(
+    char const* what, int32_t T, int32_t C, void const* in, int64_t stride, void const* out, void const* scales);
+int token_quantize(trtamd_stream_t stream, int32_t T, int32_t C, trtamd_half_t const* in, int64_t stride, int8_t* out, float* scales);
 
 // trtamd_skipln_interleaved_{small,large}_hface with the input given as the partial sums of an affine INT8 layer (alpha,
 // beta as in trtamd_int8_linear_params): the same bytes as the layer's output through memory would give.

@@ -1,0 +1,105 @@
+// What the kernels of INT8 arithmetic with a scale for each token share: the quantiser's steps and the layers' results.
+#pragma once
+
+#include "device_utils.hpp"
+
+namespace trtamd
+{
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+constexpr uint32_t kF16Inf = 0x7c00u;
+
+// The larger of the absolute values' bits in each half: as integers they are ordered as the values are, with infinity and
+// the NaNs above all others, so that a row's maximum says whether it holds any.
+__device__ inline u16x2 max_abs(u16x2 m, uint32_t pair)
+{
+    return __builtin_elementwise_max(m, bits_as<u16x2>(pair & 0x7fff7fffu));
+}
+
+// What a row is divided by: q = 127 x / amax, with 1 / amax at hand.  amax = 0 stands for rows whose values all become 0.
+struct RowScale
+{
+    float amax, inverse;
+};
+
+__device__ inline RowScale row_scale(uint32_t bits, float& scale)
+{
+    float const amax = (float) bits_as<f16>((uint16_t) bits);
+    bool const finite = bits < kF16Inf;
+    scale = finite ? __fdiv_rn(amax, 127.f) : __builtin_nanf("");
+    return finite && bits ? RowScale{amax, __fdiv_rn(1.f, amax)} : RowScale{0.f, 0.f};
+}
+
+// The quotient is corrected by its exact remainder, which makes it the correctly rounded one (Markstein's step): 127 x
+// is exact, and so is what is half way between two integers, which the product with a rounded reciprocal misses now and then
+// (amax / 2 is a common value, and is 63.5).  What is not half way is further from it than this rounding moves it: 127 x / amax has
+// 11-bit operands.  Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the lowest byte.
+__device__ inline uint32_t quantized_bits(float x, RowScale const& r)
+{
+    float const n = x * 127.f;
+    float const y = n * r.inverse;
+    return bits_as<uint32_t>(fmaf(fmaf(-y, r.amax, n), r.inverse, y) + 12582912.f);
+}
+
+// The lowest bytes of four dwords in one.
+__device__ inline uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    uint32_t const ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), cd = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return ab | cd << 16;
+}
+
+__device__ inline u32x2 quantize8(f16x8 v, RowScale const& r)
+{
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        // 0 * NaN and 0 * infinity: a row that holds them has no quotients
+        b[e] = r.amax > 0.f ? quantized_bits((float) v[e], r) : 0u;
+    }
+    return {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+}
+
+__device__ inline uint32_t wave_max_bits(u16x2 m)
+{
+    uint32_t const both = max((uint32_t) m[0], (uint32_t) m[1]);
+    return group_allreduce<kWaveSize>(both, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
+__device__ inline u16x2 max_abs(u16x2 m, u32x4 const& v)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+    {
+        m = max_abs(m, v[e]);
+    }
+    return m;
+}
+
+// GELU for FP16 results: gelu(y) = max(y, 0) - |y| Phi(-|y|), with Phi(-a) to a relative error (y Phi(y) is small, not rounded away, for negative y):
+// a polynomial of degree 7 for log2(Phi(-a)) that is off by 4.5e-6 at most on [0, 5.5], behind which the result is below
+// half of the smallest binary16.  Within 4e-6 of the exact value where that is a normal binary16, 2.5e-10 elsewhere.  The leading coefficient is
+// negative, so the term vanishes for larger a; a NaN stays one (through a).
+__device__ inline float gelu_f16(float y)
+{
+    float const a = fabsf(y);
+    float p = fmaf(a, -1.793455226e-06f, 6.090417810e-05f);
+    p = fmaf(p, a, -9.260290535e-04f);
+    p = fmaf(p, a, 8.493757807e-03f);
+    p = fmaf(p, a, -5.393784493e-02f);
+    p = fmaf(p, a, -4.584805071e-01f);
+    p = fmaf(p, a, -1.151246786e+00f);
+    p = fmaf(p, a, -9.999954700e-01f);
+    return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
+}
+
+// The result of a token-scaled layer: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
+template <bool GELU>
+__device__ __forceinline__ float token_result(int const acc, float const ts, float const al, float const be)
+{
+    float const y = fmaf((float) acc * ts, al, be);
+    return GELU ? gelu_f16(y) : y;
+}
+
+} // namespace trtamd
