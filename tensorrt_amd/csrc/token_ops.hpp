@@ -17,29 +17,35 @@ __device__ inline u16x2 max_abs(u16x2 m, uint32_t pair)
     return __builtin_elementwise_max(m, bits_as<u16x2>(pair & 0x7fff7fffu));
 }
 
-// What a row is divided by: q = 127 x / amax, with 1 / amax at hand.  amax = 0 stands for rows whose values all become 0.
+// What a row's values are multiplied by, 127 / amax in two parts: the second is what the first is off by, so a product with both is the
+// quotient rounded once.  A quotient half way between two integers therefore comes out as such (a product with one rounded
+// factor misses now and then, and amax / 2 is a common value: 63.5), and any other is further from half way than a rounding
+// moves it: 127 x / amax has operands of 11 bits.
 struct RowScale
 {
-    float amax, inverse;
+    float high, low;
 };
 
+// From the bits of amax.  Rows of zeros have factors of 0, and so have rows with an infinity or a NaN.  The scale, amax / 127, is rounded
+// correctly: a product with 1 / 127, corrected by its exact remainder.
 __device__ inline RowScale row_scale(uint32_t bits, float& scale)
 {
     float const amax = (float) bits_as<f16>((uint16_t) bits);
     bool const finite = bits < kF16Inf;
-    scale = finite ? __fdiv_rn(amax, 127.f) : __builtin_nanf("");
-    return finite && bits ? RowScale{amax, __fdiv_rn(1.f, amax)} : RowScale{0.f, 0.f};
+    constexpr float k127th = 1.f / 127.f;
+    float const s = amax * k127th;
+    scale = finite ? fmaf(fmaf(-s, 127.f, amax), k127th, s) : __builtin_nanf("");
+    float const inverse = __builtin_amdgcn_rcpf(amax);
+    float const high = 127.f * inverse;
+    return finite && bits ? RowScale{high, fmaf(-high, amax, 127.f) * inverse} : RowScale{0.f, 0.f};
 }
 
-// The quotient is corrected by its exact remainder, which makes it the correctly rounded one (Markstein's step): 127 x
-// is exact, and so is what is half way between two integers, which the product with a rounded reciprocal misses now and then
-// (amax / 2 is a common value, and is 63.5).  What is not half way is further from it than this rounding moves it: 127 x / amax has
-// 11-bit operands.  Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the lowest byte.
-__device__ inline uint32_t quantized_bits(float x, RowScale const& r)
+// Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the lowest byte.  What is not a number (an infinity or a NaN times
+// the factors of its row, 0) has zeros there.
+__device__ inline uint32_t quantized_bits(f16 x, RowScale const& r)
 {
-    float const n = x * 127.f;
-    float const y = n * r.inverse;
-    return bits_as<uint32_t>(fmaf(fmaf(-y, r.amax, n), r.inverse, y) + 12582912.f);
+    float const low = fmaf((float) x, r.low, 0.f); // as a multiply-add it takes the binary16 as it is
+    return bits_as<uint32_t>(fmaf((float) x, r.high, low) + 12582912.f);
 }
 
 // The lowest bytes of four dwords in one.
@@ -55,8 +61,7 @@ __device__ inline u32x2 quantize8(f16x8 v, RowScale const& r)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
     {
-        // 0 * NaN and 0 * infinity: a row that holds them has no quotients
-        b[e] = r.amax > 0.f ? quantized_bits((float) v[e], r) : 0u;
+        b[e] = quantized_bits(v[e], r);
     }
     return {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
 }

@@ -221,6 +221,32 @@ def test_layers(api, T, K, N, gelu, bias):
     assert np.array_equal(bits(one), bits(two)), "the two entry points differ"
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 5, 8, 15, 16, 17, 31, 32, 33, 47, 64, 65])
+@pytest.mark.parametrize("K", [64, 128, 192, 576, 960, 1024, 1088, 1152, 2048, 2112, 4032, 4096, 4160, 8192])
+@pytest.mark.parametrize("N", [32, 224])
+def test_few_tokens(api, T, K, N):
+    """Both sides of every length up to which few tokens go in one launch."""
+    layer = Layer(api, T, K, N, gelu=N == 32, bias=K % 128 == 0)
+    want, tol = layer.want()
+    one, two, ws = layer.out(), layer.out(), layer.workspace()
+    layer.token(one)
+    layer.dynamic(two, ws)
+    sync()
+    assert_within(host(one)[:T], want, tol)
+    assert np.array_equal(bits(one), bits(two))
+
+
+def test_few_tokens_of_many_channels(api):
+    for T, N in ((1, 8160), (1, 8192), (3, 8224), (16, 16384), (5, 30528)):
+        layer = Layer(api, T, 128, N)
+        want, tol = layer.want()
+        out = layer.out()
+        layer.dynamic(out, layer.workspace())
+        sync()
+        assert_within(host(out)[:T], want, tol, f"{T} {N}")
+        assert (host(out)[T] == -7).all()
+
+
 PLANS = range(1, 15)
 
 
