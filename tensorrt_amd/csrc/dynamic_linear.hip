@@ -152,13 +152,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void dynamic_few_kernel(uint64_t co
             {
                 sum += part[i][b][lane];
             }
-            f16x4 h;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-            {
-                h[e] = (f16) token_result<GELU>(sum[e], scale[b], al[e], be[e]);
-            }
-            *reinterpret_cast<f16x4*>(out + (size_t) t * N + n0 + 4 * group) = h;
+            *reinterpret_cast<u32x2*>(out + (size_t) t * N + n0 + 4 * group) = token_results<GELU>(sum, scale[b], al, be);
         }
     }
 }

@@ -43,6 +43,7 @@ namespace trtamd
 namespace
 {
 
+constexpr int64_t kLastLevelCache = 256 << 20; // bytes
 constexpr int kBigTile = 256; // channels and tokens of the large workgroup tile
 
 enum Epilogue
@@ -114,6 +115,7 @@ struct LinearArgs
     FastDiv panelDiv, perPanelDiv; // tiles: by panel and tokMain * panel
     WeightPrefetch prefetch; // by the workgroups behind mainTiles of the interleaved tile and piece kernels
     float const* tokenScale; // token-scaled epilogues
+    bool streaming;          // likewise: results past the last-level cache (see store_rows)
 };
 
 // gelu(y) = y * Phi(y) = max(y, 0) - |y| * Phi(-|y|).  log2(Phi(-a)) is smooth and nearly quadratic, so
@@ -172,6 +174,26 @@ __device__ __forceinline__ void store_out(void* p, V const& v)
     }
 }
 
+// 16 bytes per lane of whole lines at a scalar address and a lane's offset, through the L2; `streaming`: past the last-level cache too.  Results
+// that it cannot hold would only push each other out of it: 33289 tokens x 1024 -> 4096 (273 MB), 186 us through it and 165 past it,
+// with the quantiser that reads them 247 either way; below that the reader pays more than is gained (16384 tokens, 134 MB: 92 / 78
+// alone, 120 / 124 with the reader).  Inline assembly as in store_through_l2.
+__device__ __forceinline__ void store_rows(void* base, uint32_t laneOffset, u32x4 const& v, bool streaming)
+{
+    uint64_t const b = reinterpret_cast<uint64_t>(base);
+    uint32_t const lo = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) b);
+    uint32_t const hi = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (b >> 32));
+    uint64_t const ub = ((uint64_t) hi << 32) | lo;
+    if (streaming)
+    {
+        asm volatile("global_store_dwordx4 %0, %1, %2 nt\n\ts_nop 1" ::"v"(laneOffset), "v"(v), "s"(ub) : "memory");
+    }
+    else
+    {
+        asm volatile("global_store_dwordx4 %0, %1, %2 sc1\n\ts_nop 1" ::"v"(laneOffset), "v"(v), "s"(ub) : "memory");
+    }
+}
+
 // The 16 scale / offset pairs a lane needs for one 32-channel block (channels 8g + 4 (l/32) + e of the block), read
 // from the tile's vectors in LDS.  For the affine INT8 epilogue the offsets already carry the 128 of the unsigned
 // byte conversion.  A block's scales serve every token block of the same channels, so callers that walk several
@@ -215,19 +237,18 @@ __device__ __forceinline__ void pack_half_block(
 #pragma unroll
     for (int g = 0; g < 4; ++g)
     {
+        if constexpr (token_scaled(EPI))
+        {
+            i32x4 const a = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+            w[g] = token_results<EPI == kTOKEN_GELU>(a, ts, sc.al[g], sc.be[g]);
+            continue;
+        }
         f16x4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            if constexpr (token_scaled(EPI))
-            {
-                h[e] = (f16) token_result<EPI == kTOKEN_GELU>(acc[4 * g + e], ts, sc.al[g][e], sc.be[g][e]);
-            }
-            else
-            {
-                float const y = fmaf((float) acc[4 * g + e], sc.al[g][e], sc.be[g][e]);
-                h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
-            }
+            float const y = fmaf((float) acc[4 * g + e], sc.al[g][e], sc.be[g][e]);
+            h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
         }
         w[g] = __builtin_bit_cast(u32x2, h);
     }
@@ -1202,21 +1223,18 @@ __device__ __forceinline__ void store_quad(
     {
         return;
     }
-    if constexpr (f16_rows(EPI))
+    if constexpr (token_scaled(EPI))
+    {
+        *reinterpret_cast<u32x2*>(static_cast<f16*>(p.out) + (size_t) t * p.N + c) = token_results<EPI == kTOKEN_GELU>(acc, sc.ts, al, be);
+    }
+    else if constexpr (f16_rows(EPI))
     {
         f16x4 h;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            if constexpr (token_scaled(EPI))
-            {
-                h[e] = (f16) token_result<EPI == kTOKEN_GELU>(acc[e], sc.ts, al[e], be[e]);
-            }
-            else
-            {
-                float const y = fmaf(acc[e], al[e], be[e]);
-                h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
-            }
+            float const y = fmaf(acc[e], al[e], be[e]);
+            h[e] = (f16) (EPI == kF16_GELU ? gelu_erf(y) : y);
         }
         *reinterpret_cast<f16x4*>(static_cast<f16*>(p.out) + (size_t) t * p.N + c) = h;
     }
@@ -1549,6 +1567,25 @@ __device__ __forceinline__ void linear_tile_dma(
             }
             constexpr int kChunks = MT * 4; // 16-byte pieces of a row
             int const tb = t0 + (wn * NT + j) * 32;
+            if constexpr (token_scaled(EPI))
+            {
+                // a lane's pieces lie whole groups of rows apart: their addresses are one offset and scalar steps
+                constexpr int kRows = 64 / kChunks;
+                int const r = lane / kChunks, ch = lane % kChunks;
+                bool const whole = tb + 32 <= p.T && nw + MT * 32 <= p.N; // uniform
+                uint32_t const laneOff = ((uint32_t) r * (uint32_t) p.N + (uint32_t) ch * 8u) * 2u;
+                f16* rows = static_cast<f16*>(p.out) + (size_t) tb * p.N + nw;
+#pragma unroll
+                for (int q = 0; q < kChunks / 2; ++q, rows += (size_t) kRows * p.N)
+                {
+                    u32x4 const v = *reinterpret_cast<u32x4 const*>(own + (q * kRows + r) * kRow + ch * 16);
+                    if (whole || (tb + q * kRows + r < p.T && nw + ch * 8 < p.N))
+                    {
+                        store_rows(rows, laneOff, v, p.streaming);
+                    }
+                }
+                continue;
+            }
 #pragma unroll
             for (int q = 0; q < kChunks / 2; ++q)
             {
@@ -2606,6 +2643,7 @@ LinearArgs args_of(trtamd_int8_token_linear_params const& p)
     a.alpha = p.channel_scale;
     a.beta = p.bias;
     a.tokenScale = p.token_scale;
+    a.streaming = (int64_t) p.T * p.N * (int64_t) sizeof(trtamd_half_t) > kLastLevelCache;
     a.out = p.out;
     a.T = p.T;
     a.K = p.K;

@@ -99,12 +99,30 @@ __device__ inline float gelu_f16(float y)
     return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
 }
 
-// The result of a token-scaled layer: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
-template <bool GELU>
-__device__ __forceinline__ float token_result(int const acc, float const ts, float const al, float const be)
+// The result of a token-scaled layer for four consecutive channels of a token: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
+// Converted in pairs: one by one the compiler now and then makes the multiply-add and the conversion one instruction, and a token's bits would
+// depend on the kernel.
+template <bool GELU, typename Acc4>
+__device__ __forceinline__ u32x2 token_results(Acc4 const& acc, float const ts, f32x4 const& al, f32x4 const& be)
 {
-    float const y = fmaf((float) acc * ts, al, be);
-    return GELU ? gelu_f16(y) : y;
+    u32x2 r;
+#pragma unroll
+    for (int pair = 0; pair < 2; ++pair)
+    {
+        f32x2 y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+        {
+            int const c = 2 * pair + e;
+            y[e] = fmaf((float) acc[c] * ts, al[c], be[c]);
+            if constexpr (GELU)
+            {
+                y[e] = gelu_f16(y[e]);
+            }
+        }
+        r[pair] = bits_as<uint32_t>(__builtin_convertvector(y, f16x2));
+    }
+    return r;
 }
 
 } // namespace trtamd
