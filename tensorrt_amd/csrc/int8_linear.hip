@@ -1532,7 +1532,9 @@ __device__ __forceinline__ void linear_tile_dma(
     first_halves(No{});
     phase(Odd{}, No{}, 0, 0, NoLoads{}, 0, 0);
     constexpr int kRow = MT * 64 + 16; // bytes; 16 of padding spread the rows over the banks
-    constexpr bool kStaged = f16_rows(EPI) && NWAVES * 32 * kRow <= STAGE;
+    constexpr bool kOneSlot = NWAVES * 32 * kRow <= STAGE;
+    constexpr bool kStaged
+        = f16_rows(EPI) && (kOneSlot || (token_scaled(EPI) && !kLate && NWAVES * 32 * kRow <= RING * STAGE));
     if constexpr (kLate || kStaged)
     {
         wait_vmcnt<0>();
@@ -1545,7 +1547,7 @@ __device__ __forceinline__ void linear_tile_dma(
     // stores of 16-byte pieces need the L2 to put them together, and cost 5 to 9 of the 44 us of feed-forward 1).
     if constexpr (kStaged)
     {
-        uint8_t* const own = lds + slot * STAGE + wave * (32 * kRow);
+        uint8_t* const own = lds + (kOneSlot ? slot * STAGE : 0) + wave * (32 * kRow); // nobody needs any slot any more
         int const nw = n0 + wm * MT * 32;
         BlockScales sc[MT];
 #pragma unroll
@@ -2138,12 +2140,24 @@ constexpr TileCost kTileCosts[3][kLinearPlans] = {
     {{}, {128, 256, 2, 2.06f, 2.05f, 0.430f, 0.64f, 1.50f, 1.22f, 0.62f}, {128, 128, 2, 1.93f, 1.06f, 0.292f, 0.41f, 1.30f, 1.10f, 0.53f},
         {64, 128, 3, 2.49f, 0.32f, 0.188f, 0.21f, 1.27f, 1.14f, 0.52f}, {64, 64, 4, 2.29f, 0.30f, 0.138f, 0.13f, 0.94f, 0.89f, 0.47f},
         {}, {}, {}, {32, 64, 1, 2.88f, 0.30f, 0.071f, 0.05f, 0.57f, 1.91f, 0.80f}, {32, 32, 1, 2.38f, 0.34f, 0.053f, 0.13f, 1.48f, 1.49f, 0.68f}}};
+// Token-scaled layers whose rows end within a line: all of their tiles store whole rows, and there are three more of them.  Fitted to launches by
+// themselves (graph replays, three sets of operands in turn), 720 sizes of 1 to 33289 tokens, rows of 64 to 4032 bytes, 64 to 5120
+// channels, with and without GELU: 2.0 % more than the best of the nine plans in the mean on 180 other sizes too, where the constants and tiles
+// of the layers above take 4.0 %, and 9 % from 2000 tokens on (33289 x 960 -> 4096: 247 us, now 157 in 256 x 256 tiles).
+constexpr TileCost kTokenTileCosts[kLinearPlans] = {{}, {128, 256, 2, 0.46f, 4.62f, 0.301f, 2.14f, 0.69f, 0.81f, 0.56f, 1.14f},
+    {128, 128, 2, 2.16f, 1.54f, 0.186f, 0.86f, 0.71f, 0.86f, 0.55f, 0.96f}, {64, 128, 3, 2.87f, 0.72f, 0.097f, 0.42f, 0.71f, 0.82f, 0.39f, 1.68f},
+    {64, 64, 4, 3.15f, 0.33f, 0.086f, 0.16f, 0.70f, 0.81f, 0.65f, 0.82f}, {}, {}, {},
+    {32, 64, 1, 2.82f, 0.82f, 0.035f, 0.09f, 0.01f, 1.35f, 0.68f, 2.03f, 0.10f}, {32, 32, 1, 3.09f, 0.53f, 0.018f, 0.08f, 2.01f, 1.32f, 0.51f, 2.90f, 0.15f},
+    {256, 256, 1, 0.01f, 6.13f, 0.522f, 3.89f, 0.00f, 1.13f, 0.70f, 0.50f, 0.17f},
+    {256, 192, 1, 0.12f, 5.10f, 0.458f, 3.17f, 2.54f, 1.01f, 0.67f, 0.56f, 0.02f},
+    {128, 192, 2, 2.27f, 2.40f, 0.272f, 1.62f, 0.64f, 0.88f, 0.74f, 0.68f, 0.05f}};
 
 // The costs of a launch's plans.
 template <bool IL>
 TileCost const* tile_costs(LinearArgs const& a)
 {
-    return kTileCosts[IL ? 1 : a.K % 128 == 0 ? 0 : 2];
+    bool const whole = a.K % 128 == 0;
+    return a.tokenScale && !whole ? kTokenTileCosts : kTileCosts[IL ? 1 : whole ? 0 : 2];
 }
 
 inline float tile_time(TileCost const& c, LinearArgs const& a, bool gelu)
@@ -2271,6 +2285,16 @@ int launch_plan(hipStream_t stream, LinearArgs a, int plan)
     else if (a.K % 128 != 0)
     {
         // rows that end within a line: stages of 64 bytes
+        if constexpr (token_scaled(EPI))
+        {
+            switch (plan)
+            {
+            case kTile256x256: return run(linear_tile_kernel<IL, IL_OUT, EPI, 4, 2, 2, 4, 4, 2>, 512);
+            case kTile256x192: return run(linear_tile_kernel<IL, IL_OUT, EPI, 4, 2, 2, 3, 5, 2>, 512);
+            case kTile128x192: return run(linear_tile_kernel<IL, IL_OUT, EPI, 2, 2, 2, 3, 4, 2>, 256);
+            default: break;
+            }
+        }
         switch (plan)
         {
         case kTile128x256: return run(linear_tile_kernel<IL, IL_OUT, EPI, 2, 4, 2, 2, 3, 4>, 512);
@@ -2370,7 +2394,7 @@ int choose_plan(LinearArgs const& a, int64_t smallTiles, bool gelu)
 {
     struct Choice
     {
-        int T, K, N, mainTiles, pieces, gelu, setting, plan;
+        int T, K, N, mainTiles, pieces, gelu, setting, plan, token;
         int64_t smallTiles;
     };
     constexpr int kChoices = 16;
@@ -2383,7 +2407,7 @@ int choose_plan(LinearArgs const& a, int64_t smallTiles, bool gelu)
     for (Choice const& c : choices)
     {
         if (c.T == a.T && c.K == a.K && c.N == a.N && c.gelu == (int) gelu && c.mainTiles == mainTiles && c.pieces == pieces
-            && c.smallTiles == behind && c.setting == setting)
+            && c.smallTiles == behind && c.setting == setting && c.token == (a.tokenScale != nullptr))
         {
             return c.plan;
         }
@@ -2391,7 +2415,8 @@ int choose_plan(LinearArgs const& a, int64_t smallTiles, bool gelu)
     ++gLinearEstimates;
     Choice& c = choices[oldest];
     oldest = (oldest + 1) % kChoices;
-    c = {a.T, a.K, a.N, mainTiles, pieces, (int) gelu, setting, cheapest_plan<IL>(a, smallTiles, gelu, setting), behind};
+    c = {a.T, a.K, a.N, mainTiles, pieces, (int) gelu, setting, cheapest_plan<IL>(a, smallTiles, gelu, setting), a.tokenScale != nullptr,
+        behind};
     return c.plan;
 }
 

@@ -204,7 +204,7 @@ def test_quantiser_beyond_32_bits(api):
 
 SHAPES = [(1, 64, 32), (1, 1024, 1024), (2, 768, 2304), (3, 4096, 1024), (4, 128, 4096), (5, 192, 96), (7, 1088, 544), (8, 1024, 4096),
           (9, 512, 512), (16, 4096, 1024), (17, 64, 4128), (31, 128, 64), (33, 320, 160), (40, 4096, 1024), (64, 768, 768), (100, 1024, 288),
-          (129, 192, 32), (257, 1024, 1024), (777, 768, 2304), (1000, 4096, 1024), (2049, 384, 1536), (4099, 1024, 4096)]
+          (129, 192, 32), (257, 1024, 1024), (777, 768, 2304), (1000, 4096, 1024), (2049, 384, 1536), (4099, 1024, 4096), (5003, 960, 4096), (2600, 832, 2304)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
@@ -250,7 +250,7 @@ def test_few_tokens_of_many_channels(api):
 PLANS = range(1, 15)
 
 
-@pytest.mark.parametrize("T,K,N", [(300, 256, 288), (130, 192, 160), (61, 128, 96)])
+@pytest.mark.parametrize("T,K,N", [(300, 256, 288), (300, 192, 320), (130, 192, 160), (61, 128, 96), (520, 64, 544)])
 @pytest.mark.parametrize("gelu", [False, True])
 def test_every_plan_gives_the_same_bits(api, T, K, N, gelu):
     layer = Layer(api, T, K, N, gelu)
