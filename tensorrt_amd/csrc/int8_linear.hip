@@ -43,7 +43,7 @@ namespace trtamd
 namespace
 {
 
-constexpr int64_t kLastLevelCache = 256 << 20; // bytes
+constexpr int64_t kStreamedBytes = 64 << 20; // a quarter of the last-level cache: see store_rows
 constexpr int kBigTile = 256; // channels and tokens of the large workgroup tile
 
 enum Epilogue
@@ -175,9 +175,11 @@ __device__ __forceinline__ void store_out(void* p, V const& v)
 }
 
 // 16 bytes per lane of whole lines at a scalar address and a lane's offset, through the L2; `streaming`: past the last-level cache too.  Results
-// that it cannot hold would only push each other out of it: 33289 tokens x 1024 -> 4096 (273 MB), 186 us through it and 165 past it,
-// with the quantiser that reads them 247 either way; below that the reader pays more than is gained (16384 tokens, 134 MB: 92 / 78
-// alone, 120 / 124 with the reader).  Inline assembly as in store_through_l2.
+// of a size that it cannot hold beside what else a layer touches only push each other out of it: 33289 tokens x 1024 -> 4096 (273 MB)
+// 186 us through it and 165 past it, x 1024 -> 1024 (68 MB) 49 and 42.  What reads them next gives most of that back, and for smaller ones
+// more (the layer and the quantiser that reads it, 4963 x 768 -> 2304, 23 MB: 19.8 through, 20.4 past).  Four such layers with their quantisers
+// and norms, results above 64 MiB past the cache: 33289 tokens of 1024 (4096) values 539 -> 528 us, of 768 (2304) 308 -> 302, of 512 (2048) 211 -> 207;
+// 16384 of 1024 259 -> 260, 9000 of them 154 -> 156, 20000 of 512 129 -> 132.  Inline assembly as in store_through_l2.
 __device__ __forceinline__ void store_rows(void* base, uint32_t laneOffset, u32x4 const& v, bool streaming)
 {
     uint64_t const b = reinterpret_cast<uint64_t>(base);
@@ -2668,7 +2670,7 @@ LinearArgs args_of(trtamd_int8_token_linear_params const& p)
     a.alpha = p.channel_scale;
     a.beta = p.bias;
     a.tokenScale = p.token_scale;
-    a.streaming = (int64_t) p.T * p.N * (int64_t) sizeof(trtamd_half_t) > kLastLevelCache;
+    a.streaming = (int64_t) p.T * p.N * (int64_t) sizeof(trtamd_half_t) > kStreamedBytes;
     a.out = p.out;
     a.T = p.T;
     a.K = p.K;
