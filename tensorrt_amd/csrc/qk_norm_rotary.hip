@@ -102,7 +102,7 @@ __device__ __forceinline__ float element(C const& c, int e)
 }
 
 template <int V, typename T>
-__device__ inline void store_values(T* p, float const (&v)[V])
+__device__ __forceinline__ void store_values(T* p, float const (&v)[V])
 {
     if constexpr (V == 1)
     {
@@ -110,18 +110,27 @@ __device__ inline void store_values(T* p, float const (&v)[V])
     }
     else
     {
-        typedef T Vec __attribute__((ext_vector_type(V)));
-        Vec x;
+        // converted in pairs, which is one instruction each
+        typedef T Pair __attribute__((ext_vector_type(2)));
+        ChunkT<T, V> x;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+        for (int e = 0; e < V; e += 2)
         {
-            x[e] = (T) v[e];
+            Pair const two = __builtin_convertvector((f32x2{v[e], v[e + 1]}), Pair);
+            x[e] = two[0];
+            x[e + 1] = two[1];
         }
-        *reinterpret_cast<Vec*>(p) = x;
+        *reinterpret_cast<ChunkT<T, V>*>(p) = x;
     }
 }
 
-// A lane's share of a head: two chunks of V values.  Pairs of distant values are the same places of chunks rotary_dim / 2
+// Values of a head per lane: one slot, or of narrow chunks as many as make 8.
+constexpr int lane_values(int V)
+{
+    return V == 8 ? 16 : 8;
+}
+
+// A slot of a head: two chunks of V values.  Pairs of distant values are the same places of chunks rotary_dim / 2
 // apart, adjacent ones lie in two chunks one behind the other, as does what is not rotated.
 struct Slot
 {
@@ -150,13 +159,13 @@ __device__ inline Slot slot_of(RotaryArgs const& p, int slot)
     return {{first < p.d ? first : -1, second < p.d ? second : -1}, pair};
 }
 
-// A workgroup takes 256 / G rows (a row: a head of a token), G lanes each, NS slots a lane (V = 1: heads of more than 128 values).  Rows are
-// numbered token by token, so its rows are heads of few tokens: their cosines and sines are worked out once, a thread each,
-// while the rows are on their way, and shared through LDS.
-template <typename T, int V, int NS, int G, bool ADJACENT, int NORM>
+// A workgroup takes 256 / G rows (a row: a head of a token), G lanes each.  Rows are numbered token by token, so its
+// rows are heads of few tokens: their cosines and sines are worked out once, a thread each, while the rows are on their way, and
+// shared through LDS.
+template <typename T, int V, int G, bool ADJACENT, int NORM>
 __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 {
-    constexpr int kRows = 256 / G;
+    constexpr int kRows = 256 / G, NS = lane_values(V) / (2 * V);
     extern __shared__ __attribute__((aligned(16))) float lds[]; // [token][cosines | sines][pairs], pairs padded to whole chunks
     uint32_t const rows = (uint32_t) p.T * (uint32_t) p.heads;
     uint32_t const first = blockIdx.x * (uint32_t) kRows, row = first + threadIdx.x / G;
@@ -236,6 +245,7 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
     }
 
     float x[NS][2][V];
+    // f on every value; and the sum of f over those that the lane has, chunk by chunk
     auto const each = [&](auto f) {
 #pragma unroll
         for (int n = 0; n < NS; ++n)
@@ -251,24 +261,38 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
             }
         }
     };
-    each([&](float& v, int n, int c, int e) { v = slots[n].at[c] >= 0 ? element<V>(raw[n][c], e) : 0.f; });
-    if constexpr (NORM != TRTAMD_QK_NORM_NONE)
-    {
-        auto const add = [](float a, float b) { return a + b; };
-        if constexpr (NORM == TRTAMD_QK_NORM_LAYER)
+    auto const total = [&](auto f) {
+        float all = 0.f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
         {
-            float sum = 0.f;
-            each([&](float& v, int, int, int) { sum += v; });
-            float const mean = group_allreduce<G>(sum, add) * p.inverseD;
-            each([&](float& v, int n, int c, int) { v = slots[n].at[c] >= 0 ? v - mean : 0.f; });
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+            {
+                float chunk = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    chunk = f(chunk, x[n][c][e]);
+                }
+                all += slots[n].at[c] >= 0 ? chunk : 0.f;
+            }
         }
-        float squares = 0.f;
-        each([&](float& v, int, int, int) { squares = fmaf(v, v, squares); });
-        float const scale = rsqrtf(fmaf(group_allreduce<G>(squares, add), p.inverseD, p.eps));
-        each([&](float& v, int n, int c, int e) {
-            float const w = element<V>(weight[n][c], e);
-            v = NORM == TRTAMD_QK_NORM_LAYER ? fmaf(v * scale, w, element<V>(bias[n][c], e)) : v * scale * w;
-        });
+        return group_allreduce<G>(all, [](float a, float b) { return a + b; });
+    };
+    auto const square = [](float sum, float v) { return fmaf(v, v, sum); };
+    each([&](float& v, int n, int c, int e) { v = element<V>(raw[n][c], e); });
+    if constexpr (NORM == TRTAMD_QK_NORM_RMS)
+    {
+        float const scale = rsqrtf(fmaf(total(square), p.inverseD, p.eps));
+        each([&](float& v, int n, int c, int e) { v = v * element<V>(weight[n][c], e) * scale; });
+    }
+    if constexpr (NORM == TRTAMD_QK_NORM_LAYER)
+    {
+        float const mean = total([](float sum, float v) { return sum + v; }) * p.inverseD;
+        each([&](float& v, int, int, int) { v -= mean; });
+        float const scale = rsqrtf(fmaf(total(square), p.inverseD, p.eps));
+        each([&](float& v, int n, int c, int e) { v = fmaf(v * scale, element<V>(weight[n][c], e), element<V>(bias[n][c], e)); });
     }
 #pragma unroll
     for (int k = 0; k < NS; ++k)
@@ -313,15 +337,15 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 }
 
 // One of the kernels for the norms.
-template <typename T, int V, int NS, int G, bool ADJACENT>
+template <typename T, int V, int G, bool ADJACENT>
 auto kernel_of(int norm)
 {
-    return norm == TRTAMD_QK_NORM_NONE ? qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_NONE>
-        : norm == TRTAMD_QK_NORM_RMS  ? qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_RMS>
-                                      : qk_norm_rotary_kernel<T, V, NS, G, ADJACENT, TRTAMD_QK_NORM_LAYER>;
+    return norm == TRTAMD_QK_NORM_NONE ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_NONE>
+        : norm == TRTAMD_QK_NORM_RMS  ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_RMS>
+                                      : qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_LAYER>;
 }
 
-template <typename T, int V, int NS, int G>
+template <typename T, int V, int G>
 int launch_group(hipStream_t stream, RotaryArgs a)
 {
     constexpr int kRows = 256 / G;
@@ -329,40 +353,45 @@ int launch_group(hipStream_t stream, RotaryArgs a)
     a.pitch = ceil_div(a.half, V < 4 ? 4 : V) * (V < 4 ? 4 : V);
     // the rows of a workgroup are heads of no more tokens than this
     unsigned const lds = (unsigned) (2 * a.pitch * (ceil_div(kRows - 1, a.heads) + 1)) * sizeof(float);
-    auto const kernel = a.adjacent ? kernel_of<T, V, NS, G, true>(a.norm) : kernel_of<T, V, NS, G, false>(a.norm);
+    auto const kernel = a.adjacent ? kernel_of<T, V, G, true>(a.norm) : kernel_of<T, V, G, false>(a.norm);
     hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a);
     return check_launch("qk_norm_rotary_kernel");
 }
 
-// Slots of a head: pairs of chunks.
-int slots_of(RotaryArgs const& a, int V)
+// The lanes of a head: its slots (pairs of chunks), NS a lane.
+int lanes_of(RotaryArgs const& a, int V)
 {
-    return a.adjacent ? ceil_div(a.d, 2 * V) : a.half / V + ceil_div(a.d - 2 * a.half, 2 * V);
+    int const slots = a.adjacent ? ceil_div(a.d, 2 * V) : a.half / V + ceil_div(a.d - 2 * a.half, 2 * V);
+    return ceil_div(slots, lane_values(V) / (2 * V));
 }
 
 template <typename T, int V>
 int launch_width(hipStream_t stream, RotaryArgs const& a)
 {
-    int const slots = slots_of(a, V);
-    if constexpr (V == 1)
+    int const lanes = lanes_of(a, V);
+    if constexpr (V >= 4)
     {
-        return slots <= 64 ? launch_group<T, V, 1, 64>(stream, a) : launch_group<T, V, 2, 64>(stream, a);
+        if (lanes <= 2)
+        {
+            return launch_group<T, V, 2>(stream, a);
+        }
+        if (lanes <= 4)
+        {
+            return launch_group<T, V, 4>(stream, a);
+        }
+    }
+    if (lanes <= 8)
+    {
+        return launch_group<T, V, 8>(stream, a);
+    }
+    static_assert(TRTAMD_ROTARY_MAX_HEAD <= 32 * lane_values(1) && TRTAMD_ROTARY_MAX_HEAD <= 16 * lane_values(8), "lanes enough");
+    if constexpr (V == 8)
+    {
+        return launch_group<T, V, 16>(stream, a);
     }
     else
     {
-        if (slots <= 4)
-        {
-            return launch_group<T, V, 1, 4>(stream, a);
-        }
-        if (slots <= 8)
-        {
-            return launch_group<T, V, 1, 8>(stream, a);
-        }
-        if constexpr (V == 4) // 16 chunks of 8 pairs of values are 256
-        {
-            return slots <= 16 ? launch_group<T, V, 1, 16>(stream, a) : launch_group<T, V, 1, 32>(stream, a);
-        }
-        return launch_group<T, V, 1, 16>(stream, a);
+        return lanes <= 16 ? launch_group<T, V, 16>(stream, a) : launch_group<T, V, 32>(stream, a);
     }
 }
 
@@ -395,7 +424,7 @@ int launch_type(hipStream_t stream, RotaryArgs const& a)
             return launch_width<T, 8>(stream, a);
         }
     }
-    return fits<T>(a, 4) ? launch_width<T, 4>(stream, a) : launch_width<T, 1>(stream, a);
+    return fits<T>(a, 4) ? launch_width<T, 4>(stream, a) : fits<T>(a, 2) ? launch_width<T, 2>(stream, a) : launch_width<T, 1>(stream, a);
 }
 
 int bad(char const* what)
