@@ -85,7 +85,8 @@ TRTAMD_API int trtamd_fp16_linear(trtamd_stream_t stream, trtamd_fp16_linear_par
 /* amax[t] = max_c |in[t][c]|;  scales[t] = amax[t] / 127;  out[t][c] = round_half_even(in[t][c] * 127 / amax[t]), exact
  * (the quotient is rounded once, ties as such).  A token of zeros has scale 0 and zeros.  A token that holds an infinity
  * or a NaN has scale NaN and zeros, so that whatever is computed from it is NaN, and nothing else is.
- * in [T][C] with in_stride elements between rows (a multiple of 8, no less than C); out [T][C]; C % 32 == 0. */
+ * in [T][C] with in_stride elements between rows (a multiple of 8, no less than C); out [T][C]; C % 32 == 0; T < 2^24 and C < 2^30.
+ * As everywhere below, what a call writes overlaps nothing that it reads. */
 TRTAMD_API int trtamd_quantize_fp16_per_token(trtamd_stream_t stream, int32_t T, int32_t C, trtamd_half_t const* in,
     int64_t in_stride, int8_t* out, float* scales);
 
@@ -107,8 +108,8 @@ typedef struct trtamd_int8_token_linear_params
 TRTAMD_API int trtamd_int8_token_linear(trtamd_stream_t stream, trtamd_int8_token_linear_params const* params);
 
 /* The two in one call, for a layer whose input no other layer takes: the same bits as trtamd_quantize_fp16_per_token and
- * trtamd_int8_token_linear behind it.  The quantised tokens stay in the workspace (16-byte aligned; calls that may overlap
- * need one each). */
+ * trtamd_int8_token_linear behind it (few tokens: in one launch, which leaves the workspace alone).  The quantised tokens go to the
+ * workspace (16-byte aligned; calls that may overlap need one each). */
 typedef struct trtamd_int8_dynamic_linear_params
 {
     trtamd_half_t const* a;     /* [T][K] */
@@ -153,7 +154,8 @@ enum
  * q and k are read at q + t * q_token_stride + head * q_head_stride (elements), each head's d values in a row, and written
  * to q_out and k_out in the same way: the packed layouts of the attention plugins ([token][head][q|k|v][d] has token strides
  * of 3 N d and head strides of 3 d) as well as tensors of their own, with fewer heads of k than of q or none.  q_out = q with the
- * same strides works in place; other overlaps of what is written with anything else in the call are not allowed. */
+ * same strides works in place; other overlaps of what is written with anything else in the call are not allowed.  T * (q_heads + k_heads)
+ * < 2^26. */
 typedef struct trtamd_qk_norm_rotary_params
 {
     void const* q;

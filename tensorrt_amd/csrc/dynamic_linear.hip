@@ -220,7 +220,7 @@ extern "C" int trtamd_int8_dynamic_linear(trtamd_stream_t stream, trtamd_int8_dy
     int8_t* const quantized = static_cast<int8_t*>(p->workspace);
     float* const scales = p->T > 0 ? reinterpret_cast<float*>(quantized + quantized_bytes(p->T, p->K)) : nullptr;
     trtamd_int8_token_linear_params const q = {quantized, p->w, scales, p->channel_scale, p->bias, p->out, p->T, p->K, p->N, p->epilogue};
-    int st = int8_token_linear_check(q);
+    int st = int8_token_linear_check("int8_dynamic_linear", q);
     st = st ? st : token_quantize_check("int8_dynamic_linear", p->T, p->K, p->a, p->a_stride, quantized, scales);
     if (st || p->T == 0)
     {

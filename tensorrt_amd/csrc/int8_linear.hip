@@ -2680,20 +2680,20 @@ LinearArgs args_of(trtamd_int8_token_linear_params const& p)
     return a;
 }
 
-int check_token(trtamd_int8_token_linear_params const* p)
+int check_token(char const* what, trtamd_int8_token_linear_params const* p)
 {
     if (p == nullptr)
     {
-        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: null pointer");
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: null pointer", what);
     }
     if (p->T < 0 || p->K <= 0 || p->N <= 0 || p->K % 64 != 0 || p->N % 32 != 0)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM,
-            "int8_token_linear: T=%d K=%d N=%d (K must be a multiple of 64, N of 32)", p->T, p->K, p->N);
+            "%s: T=%d K=%d N=%d (K must be a multiple of 64, N of 32)", what, p->T, p->K, p->N);
     }
     if (p->epilogue != TRTAMD_LINEAR_AFFINE && p->epilogue != TRTAMD_LINEAR_GELU)
     {
-        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: unknown epilogue %d", p->epilogue);
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: unknown epilogue %d", what, p->epilogue);
     }
     if (p->T == 0)
     {
@@ -2701,24 +2701,24 @@ int check_token(trtamd_int8_token_linear_params const* p)
     }
     if (p->a == nullptr || p->w == nullptr || p->token_scale == nullptr || p->channel_scale == nullptr || p->out == nullptr)
     {
-        return set_error(TRTAMD_STATUS_BAD_PARAM, "int8_token_linear: null pointer");
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: null pointer", what);
     }
     if ((int64_t) p->T * p->K >= (int64_t) 1 << 31 || (int64_t) p->N * p->K >= (int64_t) 1 << 31)
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "int8_token_linear: operand of 2 GiB or more");
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: operand of 2 GiB or more", what);
     }
     if (!aligned16(p->a) || !aligned16(p->w) || !aligned16(p->out) || !aligned16(p->channel_scale) || !aligned16(p->bias)
         || (reinterpret_cast<uintptr_t>(p->token_scale) & 3u) != 0)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM,
-            "int8_token_linear: pointers must be 16-byte aligned (token_scale: 4)");
+            "%s: pointers must be 16-byte aligned (token_scale: 4)", what);
     }
     return TRTAMD_STATUS_SUCCESS;
 }
 
 int run_token(trtamd_stream_t stream, trtamd_int8_token_linear_params const* p)
 {
-    int const checked = check_token(p);
+    int const checked = check_token("int8_token_linear", p);
     if (checked != TRTAMD_STATUS_SUCCESS || p->T == 0)
     {
         return checked;
@@ -2825,9 +2825,9 @@ int fp16_linear_check(trtamd_fp16_linear_params const& p)
     return check_fp16(&p);
 }
 
-int int8_token_linear_check(trtamd_int8_token_linear_params const& p)
+int int8_token_linear_check(char const* what, trtamd_int8_token_linear_params const& p)
 {
-    return check_token(&p);
+    return check_token(what, &p);
 }
 
 } // namespace trtamd

@@ -40,8 +40,8 @@ int int8_linear_partial(trtamd_stream_t stream, trtamd_int8_linear_params const&
 int fp16_linear_partial(trtamd_stream_t stream, trtamd_fp16_linear_params const& p, int parts, float* partial);
 // The checks of trtamd_fp16_linear without its launch, for a pass that is refused before its first launch.
 int fp16_linear_check(trtamd_fp16_linear_params const& p);
-// The same of trtamd_int8_token_linear, for trtamd_int8_dynamic_linear.
-int int8_token_linear_check(trtamd_int8_token_linear_params const& p);
+// The same of trtamd_int8_token_linear, as those of `what`.
+int int8_token_linear_check(char const* what, trtamd_int8_token_linear_params const& p);
 // The checks of trtamd_quantize_fp16_per_token, as those of `what`, and its launch without them.
 int token_quantize_check(
     char const* what, int32_t T, int32_t C, void const* in, int64_t stride, void const* out, void const* scales);

@@ -518,9 +518,9 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
             return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: sections of %lld pairs, rotary_dim has %d", (long long) sum, pairs);
         }
     }
-    if ((int64_t) p->T * ((int64_t) p->q_heads + p->k_heads) >= (int64_t) 1 << 31)
+    if ((int64_t) p->T * ((int64_t) p->q_heads + p->k_heads) >= (int64_t) 1 << 26)
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: 2^31 heads or more");
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: 2^26 heads of tokens or more"); // a launch has 2^32 threads
     }
     return TRTAMD_STATUS_SUCCESS;
 }

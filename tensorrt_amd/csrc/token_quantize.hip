@@ -122,9 +122,9 @@ int token_quantize_check(
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: null pointer", what);
     }
-    if (T >= 1 << 24)
+    if (T >= 1 << 24 || C >= 1 << 30)
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: 2^24 tokens or more", what); // 2^32 threads
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: 2^24 tokens or 2^30 values of one or more", what); // a launch has 2^32 threads
     }
     if (!aligned16(in) || !aligned16(out) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)
     {

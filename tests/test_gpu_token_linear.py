@@ -296,6 +296,19 @@ def test_tokens_that_are_not_finite_stay_by_themselves(api, T, K, N, gelu):
         assert_within(out[rows], want[rows], tol[rows])
 
 
+@pytest.mark.parametrize("T,K,N", [(33333, 64, 1056), (33000, 128, 1024), (9001, 192, 4128)])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_results_past_the_cache(api, T, K, N, gelu):
+    """Results of more than 64 MiB, in whole tiles and with ends in either direction."""
+    layer = Layer(api, T, K, N, gelu)
+    want, tol = layer.want()
+    out = layer.out()
+    layer.dynamic(out, layer.workspace())
+    sync()
+    assert_within(host(out)[:T], want, tol)
+    assert (host(out)[T] == -7).all()
+
+
 def test_large_accumulators(api):
     """Sums beyond 2^24, which a binary32 no longer holds exactly, and the largest in either direction."""
     T, K, N = 3, 8192, 64
