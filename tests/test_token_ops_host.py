@@ -1,9 +1,14 @@
 """What the token-scaled INT8 layers and the norm-and-rotation pass refuse, and that they do so before anything is launched:
 no GPU is needed here, and no address that is given is ever read."""
 import ctypes as C
+import os
+import re
 
+import numpy as np
 import pytest
+from scipy.special import ndtr
 
+import tensorrt_amd
 from tensorrt_amd import capi
 
 A = 0x10000  # an aligned address
@@ -122,3 +127,23 @@ def test_workspace_size(api):
         assert size(T, K, N) >= T * K + 4 * T
         # what is one byte short is refused
         refused(api, api.int8_dynamic_linear(None, dynamic(T=T, K=K, N=N, a_stride=K, workspace_bytes=size(T, K, N) - 1)), "workspace")
+
+
+def test_gelu_polynomial():
+    """The polynomial of gelu_f16 as it stands in the source, evaluated in binary32 as the kernels do: what the layers' tolerances count on."""
+    path = os.path.join(os.path.dirname(tensorrt_amd.__file__), "csrc", "token_ops.hpp")
+    body = open(path).read().split("float gelu_f16(float y)")[1].split("return fmaf(-a")[0]
+    c = [np.float32(v) for v in re.findall(r"(-?\d\.\d+e[-+]\d+)f", body)]
+    assert len(c) == 6 and c[0] < 0
+    y = np.linspace(-12, 12, 480001).astype(np.float32)
+    a = np.abs(y).astype(np.float64)
+    p = np.full(y.shape, c[0])
+    for v in c[1:]:  # the products are exact in binary64, so this rounds once, as an fma
+        p = (p.astype(np.float64) * a + np.float64(v)).astype(np.float32)
+    got = np.maximum(y, 0).astype(np.float64) - a * np.exp2(p.astype(np.float64)).astype(np.float32)
+    want = y * ndtr(y.astype(np.float64))
+    assert (np.abs(got - want) <= np.where(np.abs(want) >= 2.0 ** -14, 8.5e-5 * np.abs(want), 5.2e-9)).all()
+    # behind the interval the term vanishes
+    far = 10.0 ** np.arange(1, 9)
+    poly = np.polyval([float(v) for v in c], far)
+    assert (poly < -70).all() and (np.diff(poly) < 0).all()
