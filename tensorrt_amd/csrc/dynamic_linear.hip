@@ -1,5 +1,5 @@
-// INT8 linear layers on FP16 activations that are quantised token by token: the quantiser and the token-scaled layer behind it, or for
-// few tokens both in one launch.
+// INT8 linear layers on FP16 activations that are quantised token by token: the quantiser and the token-scaled layer behind it,
+// or for few tokens both in one launch.
 #include "device_utils.hpp"
 #include "host_utils.hpp"
 #include "network_ops.hpp"
@@ -13,12 +13,12 @@ namespace
 
 // ---- Few tokens ----
 //
-// A launch of its own for the quantiser is as long as the layer itself (1024 -> 4096 channels, one token: 2.5 of 5.1 us, and 3 us of the
-// host), so every workgroup quantises all tokens for itself.  What bounds it is one trip to memory for the weights, which are
-// requested before the tokens are looked at.
+// A launch of its own for the quantiser is as long as the layer itself (1024 -> 4096 channels, one token: 2.5 of 5.1 us, and 3
+// us of the host), so every workgroup quantises all tokens for itself.  What bounds it is one trip to memory for the weights,
+// which are requested before the tokens are looked at.
 //
-// A workgroup has 16 output channels and 16 TB tokens.  Its eight wavefronts share k: wavefront w multiplies the stretches w, w + 8, ..
-// of 128 values with v_mfma_i32_16x16x64_i8, whose operands are 16 values of one row per lane: weights, and tokens that
+// A workgroup has 16 output channels and 16 TB tokens.  Its eight wavefronts share k: wavefront w multiplies the stretches w, w
+// + 8, .. of 128 values with v_mfma_i32_16x16x64_i8, whose operands are 16 values of one row per lane: weights, and tokens that
 // the lane has quantised itself.  They meet twice in LDS, for the tokens' maxima and for the sums.
 constexpr int kFewWaves = 8;
 constexpr int kFewK = 128 * kFewWaves; // values of k in one stretch of each wavefront
@@ -34,10 +34,10 @@ __global__ __launch_bounds__(kFewWaves * 64) void dynamic_few_kernel(uint64_t co
     int const row = lane & 15, group = lane >> 4;
     int const n0 = (int) blockIdx.x * 16;
 
-    // Both operands' lanes hold the values 16 group .. +15 of either half of a stretch.  Loads come back in order, and the tokens are needed
-    // first.  Columns behind the last token are the last one's; their sums are not used.  What lies behind the last value is the
-    // last half of a stretch again, which is loaded (the maxima stay what they are) and not multiplied: no load stands
-    // behind a branch.
+    // Both operands' lanes hold the values 16 group .. +15 of either half of a stretch.  Loads come back in order, and the
+    // tokens are needed first.  Columns behind the last token are the last one's; their sums are not used.  What lies behind
+    // the last value is the last half of a stretch again, which is loaded (the maxima stay what they are) and not multiplied:
+    // no load stands behind a branch.
     f16 const* const a = global_ptr<f16 const>(aAddress) + group * 16;
     int8_t const* const w = global_ptr<int8_t const>(wAddress) + (size_t) (n0 + row) * K + group * 16;
     auto const k_of = [&](int d, int h) { return (wave + d * kFewWaves) * 128 + h * 64; };
@@ -157,10 +157,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void dynamic_few_kernel(uint64_t co
     }
 }
 
-// Where one launch takes about as long as two on the GPU or less (the host's 3 us are saved either way): 32768 values at most and no more
-// weights than one round of workgroups has, in two blocks of tokens only rows of one stretch and no more workgroups than CUs.  us, graph replays, one launch / two: 1 x 1024 -> 4096 3.4 / 5.2, 16 x 1024 -> 4096
-// 4.1 / 5.3, 1 x 4096 -> 1024 6.4 / 6.8, 8 x 4096 -> 1024 7.7 / 7.2, 16 x 2048 -> 1024 5.5 / 5.9, 32 x 1024 -> 4096 5.7 / 5.5; not taken:
-// 16 x 4096 -> 1024 9.1 / 7.1, 32 x 2048 -> 1024 8.4 / 6.2, 32 x 1024 -> 8192 7.9 / 5.5, 64 x 1024 -> 4096 8.9 / 5.7, 1 x 4096 -> 16384 17.5 / 14.4.
+// Where one launch takes about as long as two on the GPU or less (the host's 3 us are saved either way): 32768 values at most
+// and no more weights than one round of workgroups has, in two blocks of tokens only rows of one stretch and no more workgroups
+// than CUs.  us, graph replays, one launch / two: 1 x 1024 -> 4096 3.4 / 5.2, 16 x 1024 -> 4096 4.1 / 5.3, 1 x 4096 -> 1024 6.4
+// / 6.8, 8 x 4096 -> 1024 7.7 / 7.2, 16 x 2048 -> 1024 5.5 / 5.9, 32 x 1024 -> 4096 5.7 / 5.5; not taken: 16 x 4096 -> 1024 9.1
+// / 7.1, 32 x 2048 -> 1024 8.4 / 6.2, 32 x 1024 -> 8192 7.9 / 5.5, 64 x 1024 -> 4096 8.9 / 5.7, 1 x 4096 -> 16384 17.5 / 14.4.
 bool few_tokens(trtamd_int8_dynamic_linear_params const& p)
 {
     if (p.T <= 16)

@@ -174,12 +174,13 @@ __device__ __forceinline__ void store_out(void* p, V const& v)
     }
 }
 
-// 16 bytes per lane of whole lines at a scalar address and a lane's offset, through the L2; `streaming`: past the last-level cache too.  Results
-// of a size that it cannot hold beside what else a layer touches only push each other out of it: 33289 tokens x 1024 -> 4096 (273 MB)
-// 186 us through it and 165 past it, x 1024 -> 1024 (68 MB) 49 and 42.  What reads them next gives most of that back, and for smaller ones
-// more (the layer and the quantiser that reads it, 4963 x 768 -> 2304, 23 MB: 19.8 through, 20.4 past).  Four such layers with their quantisers
-// and norms, results above 64 MiB past the cache: 33289 tokens of 1024 (4096) values 539 -> 528 us, of 768 (2304) 308 -> 302, of 512 (2048) 211 -> 207;
-// 16384 of 1024 259 -> 260, 9000 of them 154 -> 156, 20000 of 512 129 -> 132.  Inline assembly as in store_through_l2.
+// 16 bytes per lane of whole lines at a scalar address and a lane's offset, through the L2; `streaming`: past the last-level
+// cache too.  Results of a size that it cannot hold beside what else a layer touches only push each other out of it: 33289
+// tokens x 1024 -> 4096 (273 MB) 186 us through it and 165 past it, x 1024 -> 1024 (68 MB) 49 and 42.  What reads them next
+// gives most of that back, and for smaller ones more (the layer and the quantiser that reads it, 4963 x 768 -> 2304, 23 MB:
+// 19.8 through, 20.4 past).  Whole layers (projection, feed-forward layers, their quantisers and norms), results above 64 MiB
+// past the cache: 33289 tokens of 1024 (4096) values 539 -> 528 us, of 768 (2304) 308 -> 302, of 512 (2048) 211 -> 207; 16384
+// of 1024 259 -> 260, 9000 of them 154 -> 156, 20000 of 512 129 -> 132.  Inline assembly as in store_through_l2.
 __device__ __forceinline__ void store_rows(void* base, uint32_t laneOffset, u32x4 const& v, bool streaming)
 {
     uint64_t const b = reinterpret_cast<uint64_t>(base);
@@ -1181,8 +1182,9 @@ __device__ __forceinline__ void linear_piece64(
     }
 }
 
-// The scales and offsets of the four channels that a lane of a piece stores, and the scale of its token t: requested with the operands, since a trip to
-// memory behind the sums is as long as everything else behind the operands' (see linear_piece_kernel).
+// The scales and offsets of the four channels that a lane of a piece stores, and the scale of its token t: requested with the
+// operands, since a trip to memory behind the sums is as long as everything else behind the operands' (see
+// linear_piece_kernel).
 struct QuadScales
 {
     f32x4 al, be;
@@ -2142,10 +2144,11 @@ constexpr TileCost kTileCosts[3][kLinearPlans] = {
     {{}, {128, 256, 2, 2.06f, 2.05f, 0.430f, 0.64f, 1.50f, 1.22f, 0.62f}, {128, 128, 2, 1.93f, 1.06f, 0.292f, 0.41f, 1.30f, 1.10f, 0.53f},
         {64, 128, 3, 2.49f, 0.32f, 0.188f, 0.21f, 1.27f, 1.14f, 0.52f}, {64, 64, 4, 2.29f, 0.30f, 0.138f, 0.13f, 0.94f, 0.89f, 0.47f},
         {}, {}, {}, {32, 64, 1, 2.88f, 0.30f, 0.071f, 0.05f, 0.57f, 1.91f, 0.80f}, {32, 32, 1, 2.38f, 0.34f, 0.053f, 0.13f, 1.48f, 1.49f, 0.68f}}};
-// Token-scaled layers whose rows end within a line: all of their tiles store whole rows, and there are three more of them.  Fitted to launches by
-// themselves (graph replays, three sets of operands in turn), 720 sizes of 1 to 33289 tokens, rows of 64 to 4032 bytes, 64 to 5120
-// channels, with and without GELU: 2.0 % more than the best of the nine plans in the mean on 180 other sizes too, where the constants and tiles
-// of the layers above take 4.0 %, and 9 % from 2000 tokens on (33289 x 960 -> 4096: 247 us, now 157 in 256 x 256 tiles).
+// Token-scaled layers whose rows end within a line: all of their tiles store whole rows, and there are three more of them.
+// Fitted to launches by themselves (graph replays, three sets of operands in turn), 720 sizes of 1 to 33289 tokens, rows of 64
+// to 4032 bytes, 64 to 5120 channels, with and without GELU: 2.0 % more than the best of the nine plans in the mean on 180
+// other sizes too, where the constants and tiles of the layers above take 4.0 %, and 9 % from 2000 tokens on (33289 x 960 ->
+// 4096: 247 us, now 157 in 256 x 256 tiles).
 constexpr TileCost kTokenTileCosts[kLinearPlans] = {{}, {128, 256, 2, 0.46f, 4.62f, 0.301f, 2.14f, 0.69f, 0.81f, 0.56f, 1.14f},
     {128, 128, 2, 2.16f, 1.54f, 0.186f, 0.86f, 0.71f, 0.86f, 0.55f, 0.96f}, {64, 128, 3, 2.87f, 0.72f, 0.097f, 0.42f, 0.71f, 0.82f, 0.39f, 1.68f},
     {64, 64, 4, 3.15f, 0.33f, 0.086f, 0.16f, 0.70f, 0.81f, 0.65f, 0.82f}, {}, {}, {},

@@ -17,17 +17,17 @@ __device__ inline u16x2 max_abs(u16x2 m, uint32_t pair)
     return __builtin_elementwise_max(m, bits_as<u16x2>(pair & 0x7fff7fffu));
 }
 
-// What a row's values are multiplied by, 127 / amax in two parts: the second is what the first is off by, so a product with both is the
-// quotient rounded once.  A quotient half way between two integers therefore comes out as such (a product with one rounded
-// factor misses now and then, and amax / 2 is a common value: 63.5), and any other is further from half way than a rounding
-// moves it: 127 x / amax has operands of 11 bits.
+// What a row's values are multiplied by, 127 / amax in two parts: the second is what the first is off by, so a product with
+// both is the quotient rounded once.  A quotient half way between two integers therefore comes out as such (a product with one
+// rounded factor misses now and then, and amax / 2 is a common value: 63.5), and any other is further from half way than a
+// rounding moves it: 127 x / amax has operands of 11 bits.
 struct RowScale
 {
     float high, low;
 };
 
-// From the bits of amax.  Rows of zeros have factors of 0, and so have rows with an infinity or a NaN.  The scale, amax / 127, is rounded
-// correctly: a product with 1 / 127, corrected by its exact remainder.
+// From the bits of amax.  Rows of zeros have factors of 0, and so have rows with an infinity or a NaN.  The scale, amax / 127,
+// is rounded correctly: a product with 1 / 127, corrected by its exact remainder.
 __device__ inline RowScale row_scale(uint32_t bits, float& scale)
 {
     float const amax = (float) bits_as<f16>((uint16_t) bits);
@@ -40,8 +40,8 @@ __device__ inline RowScale row_scale(uint32_t bits, float& scale)
     return finite && bits ? RowScale{high, fmaf(-high, amax, 127.f) * inverse} : RowScale{0.f, 0.f};
 }
 
-// Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the lowest byte.  What is not a number (an infinity or a NaN times
-// the factors of its row, 0) has zeros there.
+// Adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the lowest byte.  What is not a number (an infinity or
+// a NaN times the factors of its row, 0) has zeros there.
 __device__ inline uint32_t quantized_bits(f16 x, RowScale const& r)
 {
     float const low = fmaf((float) x, r.low, 0.f); // as a multiply-add it takes the binary16 as it is
@@ -82,10 +82,11 @@ __device__ inline u16x2 max_abs(u16x2 m, u32x4 const& v)
     return m;
 }
 
-// GELU for FP16 results: gelu(y) = max(y, 0) - |y| Phi(-|y|), with log2(Phi(-a)) as a polynomial of degree 5 whose error counts by what it
-// does to the result: 8.5e-5 of it where that is a normal binary16 (a sixth of the half step that rounding costs), 5.2e-9 below (a sixth
-// too).  Degree 7 gives 4e-6 for two more multiply-adds, which are 6 of 170 us at 33289 tokens x 1024 -> 4096: the vector ALU and the
-// matrix cores take turns there.  The leading coefficient is negative, so the term vanishes for larger a; a NaN stays one (through a).
+// GELU for FP16 results: gelu(y) = max(y, 0) - |y| Phi(-|y|), with log2(Phi(-a)) as a polynomial of degree 5 whose error counts
+// by what it does to the result: 8.5e-5 of it where that is a normal binary16 (a sixth to a third of the half step that rounding
+// costs), 5.2e-9 below (a sixth).  Degree 7 gives 4e-6 for two more multiply-adds, which are 6 of 170 us at 33289 tokens x 1024 ->
+// 4096: the vector ALU and the matrix cores take turns there.  The leading coefficient is negative, so the term vanishes for
+// larger a; a NaN stays one (through a).
 __device__ inline float gelu_f16(float y)
 {
     float const a = fabsf(y);
@@ -97,9 +98,9 @@ __device__ inline float gelu_f16(float y)
     return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaxf(y, 0.f));
 }
 
-// The result of a token-scaled layer for four consecutive channels of a token: y = acc * tokenScale[t] * channelScale[n] + bias[n], or gelu(y).
-// Converted in pairs: one by one the compiler now and then makes the multiply-add and the conversion one instruction, and a token's bits would
-// depend on the kernel.
+// The result of a token-scaled layer for four consecutive channels of a token: y = acc * tokenScale[t] * channelScale[n] +
+// bias[n], or gelu(y). Converted in pairs: one by one the compiler now and then makes the multiply-add and the conversion one
+// instruction, and a token's bits would depend on the kernel.
 template <bool GELU, typename Acc4>
 __device__ __forceinline__ u32x2 token_results(Acc4 const& acc, float const ts, f32x4 const& al, f32x4 const& be)
 {

@@ -1,13 +1,16 @@
 """Norms of queries and keys for each head with their rotation, against the definition in binary64.
 
-Tolerances.  Everything but the angle is binary32.  A mean of squares of up to 256 values: a lane adds up to 16 of them (two roundings each with
-the square), lanes meet in 6 steps, so it is within 24 steps of 2^-24; the division, the addition of eps, the root and the reciprocal
-add four more, the root halves what came before them, and the products with the scale and the weight are two: a normed value is within
-20 * 2^-24 of itself.  A LayerNorm's mean is within 24 * 2^-24 of the largest |x| and is subtracted with one more rounding: 25 * 2^-24 max|x| scale |w| more, and the
-variance takes that twice over (relative to the deviation, which is no less than max|x| / 4 in these inputs): 60 * 2^-24 of the value instead of 20; the bias adds one rounding.
-The angle is reduced to half a turn in binary64 (two products of 2^-53 of the turns) and rounded to binary32 (2^-25 of half a turn, 1e-7 = 1.6 * 2^-24); the library's
-sine and cosine are within 4 steps of 2^-24 of 1.  Two products and a sum: three roundings.  Together a rotated value is within
-(20 or 60 + 1.6 + 4 + 3) * 2^-24 (|a| + |b|), where a and b are the normed pair.  FP16 results round once more: 2^-11 of the value or 2^-25."""
+Tolerances. Everything but the angle is binary32. A mean of squares of up to 256 values: a lane adds up to 16 of them
+(two roundings each with the square), lanes meet in 6 steps, so it is within 24 steps of 2^-24; the division, the
+addition of eps, the root and the reciprocal add four more, the root halves what came before them, and the products
+with the scale and the weight are two: a normed value is within 20 * 2^-24 of itself. A LayerNorm's mean is within 24
+* 2^-24 of the largest |x| and is subtracted with one more rounding: 25 * 2^-24 max|x| scale |w| more, and the
+variance takes that twice over (relative to the deviation, which is no less than max|x| / 4 in these inputs): 60 *
+2^-24 of the value instead of 20; the bias adds one rounding. The angle is reduced to half a turn in binary64 (two
+products of 2^-53 of the turns) and rounded to binary32 (2^-25 of half a turn, 1e-7 = 1.6 * 2^-24); the library's sine
+and cosine are within 4 steps of 2^-24 of 1. Two products and a sum: three roundings. Together a rotated value is
+within (20 or 60 + 1.6 + 4 + 3) * 2^-24 (|a| + |b|), where a and b are the normed pair. FP16 results round once more:
+2^-11 of the value or 2^-25."""
 import ctypes as C
 
 import numpy as np

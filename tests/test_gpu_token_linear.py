@@ -1,9 +1,11 @@
 """Quantisation with a scale for each token and the INT8 linear layers on it, against the definitions in binary64.
 
-Tolerances.  The quantised values are exact, and so is the scale (one binary32 division).  A layer's result is formed in binary32: the
-accumulator's conversion, its products with the two scales and the addition of the bias round at most four times, each to 2^-24 of the
-product p or of the sum (which is no more than |p| + |bias|); GELU's slope is at most 1.13, and its polynomial is within 8.5e-5 of the
-value where that is a normal binary16 and 5.2e-9 below (test_gelu_polynomial evaluates it).  One rounding to binary16 follows: half a step, 2^-11 of the value or 2^-25, whichever is more."""
+Tolerances. The quantised values are exact, and so is the scale (one binary32 division). A layer's result is formed in
+binary32: the accumulator's conversion, its products with the two scales and the addition of the bias round at most
+four times, each to 2^-24 of the product p or of the sum (which is no more than |p| + |bias|); GELU's slope is at most
+1.13, and its polynomial is within 8.5e-5 of the value where that is a normal binary16 and 5.2e-9 below
+(test_gelu_polynomial evaluates it). One rounding to binary16 follows: half a step, 2^-11 of the value or 2^-25,
+whichever is more."""
 import ctypes as C
 
 import numpy as np
@@ -202,9 +204,11 @@ def test_quantiser_beyond_32_bits(api):
 
 # ---- the layers --------------------------------------------------------------------------------------------------
 
-SHAPES = [(1, 64, 32), (1, 1024, 1024), (2, 768, 2304), (3, 4096, 1024), (4, 128, 4096), (5, 192, 96), (7, 1088, 544), (8, 1024, 4096),
-          (9, 512, 512), (16, 4096, 1024), (17, 64, 4128), (31, 128, 64), (33, 320, 160), (40, 4096, 1024), (64, 768, 768), (100, 1024, 288),
-          (129, 192, 32), (257, 1024, 1024), (777, 768, 2304), (1000, 4096, 1024), (2049, 384, 1536), (4099, 1024, 4096), (5003, 960, 4096), (2600, 832, 2304)]
+SHAPES = [(1, 64, 32), (1, 1024, 1024), (2, 768, 2304), (3, 4096, 1024), (4, 128, 4096), (5, 192, 96),
+          (7, 1088, 544), (8, 1024, 4096), (9, 512, 512), (16, 4096, 1024), (17, 64, 4128), (31, 128, 64),
+          (33, 320, 160), (40, 4096, 1024), (64, 768, 768), (100, 1024, 288), (129, 192, 32), (257, 1024, 1024),
+          (777, 768, 2304), (1000, 4096, 1024), (2049, 384, 1536), (4099, 1024, 4096), (5003, 960, 4096),
+          (2600, 832, 2304)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)

@@ -1,7 +1,8 @@
-"""One encoder layer without calibrated activations and with rotary positions, put together as a caller would: the QKV projection on FP16
-tokens, norms and rotation of queries and keys in place in the packed tensor, fused attention, projection, SkipLayerNorm, and the feed-forward
-layers, the first from tokens that are quantised once.  Every stage is checked against the binary64 definition on what
-the stage before it left on the GPU; the attention and the norms with the tolerances of their own tests, the rest with theirs."""
+"""One encoder layer without calibrated activations and with rotary positions, put together as a caller would: the QKV
+projection on FP16 tokens, norms and rotation of queries and keys in place in the packed tensor, fused attention,
+projection, SkipLayerNorm, and the feed-forward layers, the first from tokens that are quantised once. Every stage is
+checked against the binary64 definition on what the stage before it left on the GPU; the attention and the norms with
+the tolerances of their own tests, the rest with theirs."""
 import ctypes as C
 
 import numpy as np

@@ -1,5 +1,5 @@
-"""What the token-scaled INT8 layers and the norm-and-rotation pass refuse, and that they do so before anything is launched:
-no GPU is needed here, and no address that is given is ever read."""
+"""What the token-scaled INT8 layers and the norm-and-rotation pass refuse, and that they do so before anything is
+launched: no GPU is needed here, and no address that is given is ever read."""
 import ctypes as C
 import os
 import re
