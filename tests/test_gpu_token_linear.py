@@ -283,6 +283,27 @@ def test_every_plan_gives_the_same_bits(api, T, K, N, gelu):
             api.test_reset_tuning(switch)
 
 
+def test_choices_of_other_layers_are_kept_apart(api):
+    """Plans are remembered by sizes, and token-scaled layers have some that the other INT8 layers lack: the two in turn at the same sizes."""
+    T, K, N = 5003, 960, 1056
+    layer = Layer(api, T, K, N, bias=False)
+    want, tol = layer.want()
+    q, scales = quantised(layer.x)
+    dq, ones, zeros = dev(q), dev(np.full(N, 2.0 ** -13, np.float32)), dev(np.zeros(N, np.float32))
+    first = None
+    for _ in range(2):
+        out, out8 = layer.out(), dev_empty((T, N), np.int8, fill=99)
+        layer.token(out)
+        p = capi.Int8LinearParams(a=ptr(dq), w=ptr(layer.dw), alpha=ptr(ones), beta=ptr(zeros), out=ptr(out8), T=T, K=K, N=N)
+        api.check(api.int8_linear(stream(), C.byref(p)))
+        sync()
+        assert_within(host(out)[:T], want, tol)
+        acc = q.astype(np.float64) @ layer.w.astype(np.float64).T
+        assert np.array_equal(host(out8), np.clip(np.rint(acc * 2.0 ** -13), -128, 127))
+        assert first is None or np.array_equal(first, bits(out))
+        first = bits(out)
+
+
 @pytest.mark.parametrize("T,K,N", [(6, 1024, 1024), (70, 256, 96), (700, 1024, 1024)])
 @pytest.mark.parametrize("gelu", [False, True])
 def test_tokens_that_are_not_finite_stay_by_themselves(api, T, K, N, gelu):

@@ -88,6 +88,7 @@ def test_dynamic_linear_refuses(api, change, word):
     (dict(frequencies=A + 1), "aligned"), (dict(positions=A + 2), "aligned"), (dict(axes=0), "axes=0"), (dict(axes=5), "axes=5"),
     (dict(axes=2, sections=(16, 17)), "33 pairs"), (dict(axes=2, sections=(-1, 33)), "sections[0]"),
     (dict(axes=3, sections=(16, 33, 0)), "sections[1]"), (dict(axes=3, sections=(8, 12, 12), axes_cycled=1), "sections[1]"),
+    (dict(q_out_token_stride=128), "in place"), (dict(k_out_head_stride=32, k_heads=2), "in place"),
     (dict(T=1 << 16, q_heads=512, k_heads=512), "2^26"), (dict(q_heads=(1 << 31) - 1, k_heads=(1 << 31) - 1), "2^26")])
 def test_norm_rotary_refuses(api, change, word):
     sections = change.pop("sections", ())
