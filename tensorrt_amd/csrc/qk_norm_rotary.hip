@@ -104,6 +104,9 @@ __device__ __forceinline__ float element(C const& c, int e)
     }
 }
 
+// Non-temporal: what ordinary stores leave in the L2 is written back at the kernel's end, while nothing else runs.  4963 tokens, 12 heads 7.9 ->
+// 6.9 us, images 26.4 -> 22.9, a clip 51.5 -> 44.7, into tensors of their own; in place, with the attention behind it, the same to 1 % (32
+// sequences 19.6 and 19.7 us, 128 126 and 125).  Written through the L2 (sc1), chunks that do not fill lines take longer: images 38.8.
 template <int V, typename T>
 __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
 {
@@ -123,7 +126,7 @@ __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
             x[e] = two[0];
             x[e + 1] = two[1];
         }
-        *reinterpret_cast<ChunkT<T, V>*>(p) = x;
+        __builtin_nontemporal_store(x, reinterpret_cast<ChunkT<T, V>*>(p));
     }
 }
 
