@@ -104,10 +104,12 @@ __device__ __forceinline__ float element(C const& c, int e)
     }
 }
 
-// Non-temporal: what ordinary stores leave in the L2 is written back at the kernel's end, while nothing else runs.  4963 tokens, 12 heads 7.9 ->
-// 6.9 us, images 26.4 -> 22.9, a clip 51.5 -> 44.7, into tensors of their own; in place, with the attention behind it, the same to 1 % (32
-// sequences 19.6 and 19.7 us, 128 126 and 125).  Written through the L2 (sc1), chunks that do not fill lines take longer: images 38.8.
-template <int V, typename T>
+// Non-temporal where a group of G lanes writes 64 bytes or more at a time: what ordinary stores leave in the L2 is written back at the kernel's
+// end, while nothing else runs.  Into tensors of their own, 4963 tokens of 12 heads of 64 7.9 -> 6.9 us, images 26.4 -> 22.9, a clip 51.5 -> 44.7,
+// 20280 tokens of 16 heads of 128 67 -> 59; in place, with the attention behind it, the same to 1 % (32 sequences 19.6 and 19.7 us, 128 126 and
+// 125).  Pieces of 32 bytes would go to the memory one by one: 33289 tokens, heads of 32, 34 -> 39.  Written through the L2 (sc1), chunks that
+// do not fill lines take longer: images 38.8.
+template <int V, int G, typename T>
 __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
 {
     if constexpr (V == 1)
@@ -126,7 +128,14 @@ __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
             x[e] = two[0];
             x[e + 1] = two[1];
         }
-        __builtin_nontemporal_store(x, reinterpret_cast<ChunkT<T, V>*>(p));
+        if constexpr (G * V * sizeof(T) >= 64)
+        {
+            __builtin_nontemporal_store(x, reinterpret_cast<ChunkT<T, V>*>(p));
+        }
+        else
+        {
+            *reinterpret_cast<ChunkT<T, V>*>(p) = x;
+        }
     }
 }
 
@@ -136,33 +145,36 @@ constexpr int lane_values(int V)
     return V == 8 ? 16 : 8;
 }
 
-// A slot of a head: two chunks of V values.  Pairs of distant values are the same places of chunks rotary_dim / 2
-// apart, adjacent ones lie in two chunks one behind the other, as does what is not rotated.
+// A slot of a head: two chunks of V values, in such places that neighbouring lanes' first ones, and their second ones, lie side by side.  Pairs of
+// distant values are the same places of chunks rotary_dim / 2 apart; adjacent pairs are in one chunk (V = 1: in two one behind the other); what
+// is not rotated is cut in halves.
 struct Slot
 {
-    int at[2]; // where the chunks are; at[1] < 0: there is no second one
-    int pair;  // its first pair; V of them (those from `half` on are not rotated)
+    int at[2];   // where the chunks are; at[1] < 0: there is no second one
+    int pair[2]; // their first pairs (distant values: of both in pair[0]); those from `half` on are not rotated
 };
 
 template <int V, bool ADJACENT>
 __device__ inline Slot slot_of(RotaryArgs const& p, int slot)
 {
-    int first, second, pair;
-    int const pairSlots = p.half / V;
-    if (!ADJACENT && slot < pairSlots)
+    int first, second, pair, pair2 = p.half;
+    if constexpr (ADJACENT)
     {
-        first = slot * V;
-        second = first + p.half;
-        pair = first;
+        int const slots = (p.d + 2 * V - 1) / (2 * V);
+        first = slot >= slots ? p.d : V == 1 ? 2 * slot : V * slot;
+        second = V == 1 ? first + 1 : first + V * slots;
+        pair = V == 1 ? slot : first / 2;
+        pair2 = V == 1 ? p.half : second / 2;
     }
     else
     {
-        int const base = ADJACENT ? 0 : 2 * p.half, n = ADJACENT ? slot : slot - pairSlots;
-        first = base + 2 * V * n;
-        second = first + V;
-        pair = ADJACENT ? V * n : p.half;
+        int const pairSlots = p.half / V, n = slot - pairSlots, rest = (p.d - 2 * p.half + 2 * V - 1) / (2 * V);
+        first = n < 0 ? slot * V : 2 * p.half + n * V;
+        second = n < 0 ? first + p.half : n < rest ? first + rest * V : p.d;
+        first = n < rest ? first : p.d;
+        pair = n < 0 ? first : p.half;
     }
-    return {{first < p.d ? first : -1, second < p.d ? second : -1}, pair};
+    return {{first < p.d ? first : -1, second < p.d ? second : -1}, {pair, pair2}};
 }
 
 // A workgroup takes 256 / G rows (a row: a head of a token), G lanes each.  Rows are numbered token by token, so its
@@ -300,26 +312,49 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
         float const scale = rsqrtf(fmaf(total(square), p.inverseD, p.eps));
         each([&](float& v, int n, int c, int e) { v = fmaf(v * scale, element<V>(weight[n][c], e), element<V>(bias[n][c], e)); });
     }
+    float const* const turns = lds + (t - t0) * 2 * p.pitch;
+    auto const turn = [](float& a, float& b, float c, float s) {
+        float const ra = a * c - b * s, rb = b * c + a * s;
+        a = ra;
+        b = rb;
+    };
 #pragma unroll
     for (int k = 0; k < NS; ++k)
     {
-        int const pair = slots[k].pair;
-        if (pair < p.half)
+        if constexpr (ADJACENT && V > 1)
         {
-            // chunks of V pairs begin at multiples of V; what lies behind the last pair of one (adjacent pairs) is not used
-            float const* const from = lds + (t - t0) * 2 * p.pitch + pair;
-            ChunkT<float, V> const cosines = *reinterpret_cast<ChunkT<float, V> const*>(from);
-            ChunkT<float, V> const sines = *reinterpret_cast<ChunkT<float, V> const*>(from + p.pitch);
 #pragma unroll
-            for (int e = 0; e < V; ++e)
+            for (int h = 0; h < 2; ++h)
             {
-                float& a = ADJACENT ? x[k][2 * e / V][2 * e % V] : x[k][0][e];
-                float& b = ADJACENT ? x[k][(2 * e + 1) / V][(2 * e + 1) % V] : x[k][1][e];
-                float const c = element<V>(cosines, e), s = element<V>(sines, e);
-                float const ra = a * c - b * s, rb = b * c + a * s;
-                bool const turned = !ADJACENT || pair + e < p.half;
-                a = turned ? ra : a;
-                b = turned ? rb : b;
+                int const pair = slots[k].pair[h];
+                if (pair < p.half)
+                {
+                    // chunks begin at multiples of V / 2 pairs; what lies behind the last pair is not used
+                    ChunkT<float, V / 2> const c = *reinterpret_cast<ChunkT<float, V / 2> const*>(turns + pair);
+                    ChunkT<float, V / 2> const s = *reinterpret_cast<ChunkT<float, V / 2> const*>(turns + p.pitch + pair);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e)
+                    {
+                        if (pair + e < p.half)
+                        {
+                            turn(x[k][h][2 * e], x[k][h][2 * e + 1], element<V / 2>(c, e), element<V / 2>(s, e));
+                        }
+                    }
+                }
+            }
+        }
+        else
+        {
+            int const pair = slots[k].pair[0];
+            if (pair < p.half)
+            {
+                ChunkT<float, V> const c = *reinterpret_cast<ChunkT<float, V> const*>(turns + pair);
+                ChunkT<float, V> const s = *reinterpret_cast<ChunkT<float, V> const*>(turns + p.pitch + pair);
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                {
+                    turn(x[k][0][e], x[k][1][e], element<V>(c, e), element<V>(s, e));
+                }
             }
         }
     }
@@ -336,7 +371,7 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
         {
             if (slots[k].at[c] >= 0)
             {
-                store_values<V>(out + slots[k].at[c], x[k][c]);
+                store_values<V, G>(out + slots[k].at[c], x[k][c]);
             }
         }
     }
