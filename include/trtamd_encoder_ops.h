@@ -18,7 +18,8 @@ extern "C"
 {
 #endif
 
-/* What happens to the INT32 accumulator acc[t][n] = sum_k a[t][k] * w[n][k] (exact). */
+/* What happens to the INT32 accumulator acc[t][n] = sum_k a[t][k] * w[n][k] (exact, modulo 2^32: rows of 131072 values or
+ * more can pass its range, and whether theirs do is the caller's to know). */
 enum
 {
     /* y = fmaf(float(acc), alpha[n], beta[n]);  out8 = sat8(rne(y)).  alpha = s_a * s_w[n] / s_out and
@@ -102,7 +103,7 @@ typedef struct trtamd_int8_token_linear_params
     float const* channel_scale; /* [N] */
     float const* bias;          /* [N], or NULL for none */
     trtamd_half_t* out;         /* [T][N] */
-    int32_t T, K, N;            /* K % 64 == 0, N % 32 == 0 */
+    int32_t T, K, N;            /* K % 64 == 0, N % 32 == 0; K < 131072, so that no sum passes INT32 */
     int32_t epilogue;           /* TRTAMD_LINEAR_AFFINE or TRTAMD_LINEAR_GELU */
 } trtamd_int8_token_linear_params;
 
@@ -121,7 +122,7 @@ typedef struct trtamd_int8_dynamic_linear_params
     trtamd_half_t* out;         /* [T][N] */
     void* workspace;
     size_t workspace_bytes;     /* trtamd_int8_dynamic_linear_workspace_size(T, K, N) or more */
-    int32_t T, K, N;            /* K % 64 == 0, N % 32 == 0 */
+    int32_t T, K, N;            /* K % 64 == 0, N % 32 == 0; K < 131072, so that no sum passes INT32 */
     int32_t epilogue;           /* TRTAMD_LINEAR_AFFINE or TRTAMD_LINEAR_GELU */
 } trtamd_int8_dynamic_linear_params;
 

@@ -43,6 +43,7 @@ namespace trtamd
 namespace
 {
 
+constexpr int kTokenRow = 1 << 17;             // values of a token-scaled layer's row: 2^17 products of -128 and -128 are 2^31
 constexpr int64_t kStreamedBytes = 64 << 20; // a quarter of the last-level cache: see store_rows
 constexpr int kBigTile = 256; // channels and tokens of the large workgroup tile
 
@@ -2697,6 +2698,10 @@ int check_token(char const* what, trtamd_int8_token_linear_params const* p)
     if (p->epilogue != TRTAMD_LINEAR_AFFINE && p->epilogue != TRTAMD_LINEAR_GELU)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: unknown epilogue %d", what, p->epilogue);
+    }
+    if (p->K >= kTokenRow)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: rows of %d values or more, whose sums can pass INT32", what, kTokenRow);
     }
     if (p->T == 0)
     {

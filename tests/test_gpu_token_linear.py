@@ -433,3 +433,40 @@ def test_captured_and_replayed(api, T, K, N):
         want, tol = layer.want()
         assert_within(host(out)[:T], want, tol)
     del graph
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 12352, 96), (33, 16384, 64), (300, 20480, 288), (70, 33344, 160), (2, 131008, 32)])
+def test_long_rows(api, T, K, N):
+    layer = Layer(api, T, K, N)
+    want, tol = layer.want()
+    one, two = layer.out(), layer.out()
+    layer.token(one)
+    layer.dynamic(two, layer.workspace())
+    sync()
+    assert_within(host(one)[:T], want, tol)
+    assert np.array_equal(bits(one), bits(two))
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_the_largest_sums(api, T):
+    """Rows of the greatest length whose values and weights are all at the ends of their range: sums up to 2146435072 of the 2147483647
+    that INT32 holds."""
+    K, N = 131008, 64
+    x = np.full((T, K), 5, np.float16)
+    x[1::2] = -5
+    layer = Layer(api, T, K, N, x=x)
+    layer.w = np.full((N, K), 127, np.int8)
+    layer.w[1::2] = -128
+    layer.channel = np.full(N, 1e-6, np.float32)
+    layer.dw, layer.dc = dev(layer.w), dev(layer.channel)
+    out = layer.out()
+    layer.dynamic(out, layer.workspace())
+    sync()
+    assert_within(host(out)[:T], *layer.want())
+    q, scales = np.full((T, K), -128, np.int8), np.full(T, 0.0125, np.float32)
+    q[1::2] = 127
+    dq, ds, one = dev(q), dev(scales), layer.out()
+    p = params(capi.Int8TokenLinearParams, T, K, N, False, layer.dw, layer.dc, layer.db, one, a=ptr(dq), token_scale=ptr(ds))
+    api.check(api.int8_token_linear(stream(), C.byref(p)))
+    sync()
+    assert_within(host(one)[:T], *reference(q, scales, layer.w, layer.channel, layer.bias, False))

@@ -148,3 +148,12 @@ def test_gelu_polynomial():
     far = 10.0 ** np.arange(1, 9)
     poly = np.polyval([float(v) for v in c], far)
     assert (poly < -70).all() and (np.diff(poly) < 0).all()
+
+
+@pytest.mark.parametrize("T", [0, 1])
+@pytest.mark.parametrize("K", [131072, 133184, 262144, (1 << 31) - 64])
+def test_rows_whose_sums_could_pass_int32_are_refused(api, T, K):
+    """131072 products of -128 and -128 are 2^31; 131008, the next shorter row, has sums of 2146435072 at most."""
+    refused(api, api.int8_token_linear(None, token(T=T, K=K, N=32)), "131072", "int8_token_linear")
+    ref = dynamic(T=T, K=K, N=32, a_stride=K, workspace_bytes=1 << 40)
+    refused(api, api.int8_dynamic_linear(None, ref), "131072", "int8_dynamic_linear")
