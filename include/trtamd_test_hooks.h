@@ -10,6 +10,7 @@
 #define TRTAMD_TEST_HOOKS_H
 
 #include "trtamd_bert_kernels.h"
+#include "trtamd_encoder_ops.h"
 
 #ifdef __cplusplus
 extern "C"
@@ -43,6 +44,10 @@ TRTAMD_API int64_t trtamd_test_linear_estimates(void);
  * LDS at once) or with 128 (2); bits 4-7: workgroups per (sequence, head); bit 8: the longest sequences first; from bit 17 on:
  * how many times two rounds of 256 workgroups, the second of them backwards.  -1: parameters that have no kernel. */
 TRTAMD_API int64_t trtamd_test_fmha_route(int32_t data_type, trtamd_fmha_params const* params);
+
+/* The kernel that trtamd_qk_norm_rotary launches for these parameters: bits 0-7 the values of a load, bits 8-15 the lanes of a
+ * head, bit 16 stores past the caches.  -1: parameters that are refused, or without a launch. */
+TRTAMD_API int trtamd_test_qk_norm_rotary_route(int32_t data_type, trtamd_qk_norm_rotary_params const* params);
 
 #ifdef __cplusplus
 }

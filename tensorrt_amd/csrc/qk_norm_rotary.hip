@@ -10,6 +10,9 @@
 #include "device_utils.hpp"
 #include "host_utils.hpp"
 #include "trtamd_encoder_ops.h"
+#include "trtamd_test_hooks.h"
+
+#include <algorithm>
 
 namespace trtamd
 {
@@ -104,12 +107,8 @@ __device__ __forceinline__ float element(C const& c, int e)
     }
 }
 
-// Non-temporal where a group of G lanes writes 64 bytes or more at a time: what ordinary stores leave in the L2 is written back at the kernel's
-// end, while nothing else runs.  Into tensors of their own, 4963 tokens of 12 heads of 64 7.9 -> 6.9 us, images 26.4 -> 22.9, a clip 51.5 -> 44.7,
-// 20280 tokens of 16 heads of 128 67 -> 59; in place, with the attention behind it, the same to 1 % (32 sequences 19.6 and 19.7 us, 128 126 and
-// 125).  Pieces of 32 bytes would go to the memory one by one: 33289 tokens, heads of 32, 34 -> 39.  Written through the L2 (sc1), chunks that
-// do not fill lines take longer: images 38.8.
-template <int V, int G, typename T>
+// Past the caches or not: see past_caches.
+template <int V, bool PAST, typename T>
 __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
 {
     if constexpr (V == 1)
@@ -128,7 +127,7 @@ __device__ __forceinline__ void store_values(T* p, float const (&v)[V])
             x[e] = two[0];
             x[e + 1] = two[1];
         }
-        if constexpr (G * V * sizeof(T) >= 64)
+        if constexpr (PAST)
         {
             __builtin_nontemporal_store(x, reinterpret_cast<ChunkT<T, V>*>(p));
         }
@@ -180,7 +179,7 @@ __device__ inline Slot slot_of(RotaryArgs const& p, int slot)
 // A workgroup takes 256 / G rows (a row: a head of a token), G lanes each.  Rows are numbered token by token, so its
 // rows are heads of few tokens: their cosines and sines are worked out once, a thread each, while the rows are on their way, and
 // shared through LDS.
-template <typename T, int V, int G, bool ADJACENT, int NORM>
+template <typename T, int V, int G, bool ADJACENT, int NORM, bool PAST>
 __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
 {
     constexpr int kRows = 256 / G, NS = lane_values(V) / (2 * V);
@@ -371,69 +370,16 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_kernel(RotaryArgs const p)
         {
             if (slots[k].at[c] >= 0)
             {
-                store_values<V, G>(out + slots[k].at[c], x[k][c]);
+                store_values<V, PAST>(out + slots[k].at[c], x[k][c]);
             }
         }
     }
 }
 
-// One of the kernels for the norms.
-template <typename T, int V, int G, bool ADJACENT>
-auto kernel_of(int norm)
+// The slots of a head (pairs of chunks of V values).
+int slots_of(RotaryArgs const& a, int V)
 {
-    return norm == TRTAMD_QK_NORM_NONE ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_NONE>
-        : norm == TRTAMD_QK_NORM_RMS  ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_RMS>
-                                      : qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_LAYER>;
-}
-
-template <typename T, int V, int G>
-int launch_group(hipStream_t stream, RotaryArgs a)
-{
-    constexpr int kRows = 256 / G;
-    dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, kRows));
-    a.pitch = ceil_div(a.half, V < 4 ? 4 : V) * (V < 4 ? 4 : V);
-    // the rows of a workgroup are heads of no more tokens than this
-    unsigned const lds = (unsigned) (2 * a.pitch * (ceil_div(kRows - 1, a.heads) + 1)) * sizeof(float);
-    auto const kernel = a.adjacent ? kernel_of<T, V, G, true>(a.norm) : kernel_of<T, V, G, false>(a.norm);
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a);
-    return check_launch("qk_norm_rotary_kernel");
-}
-
-// The lanes of a head: its slots (pairs of chunks), NS a lane.
-int lanes_of(RotaryArgs const& a, int V)
-{
-    int const slots = a.adjacent ? ceil_div(a.d, 2 * V) : a.half / V + ceil_div(a.d - 2 * a.half, 2 * V);
-    return ceil_div(slots, lane_values(V) / (2 * V));
-}
-
-template <typename T, int V>
-int launch_width(hipStream_t stream, RotaryArgs const& a)
-{
-    int const lanes = lanes_of(a, V);
-    if constexpr (V >= 4)
-    {
-        if (lanes <= 2)
-        {
-            return launch_group<T, V, 2>(stream, a);
-        }
-        if (lanes <= 4)
-        {
-            return launch_group<T, V, 4>(stream, a);
-        }
-    }
-    if (lanes <= 8)
-    {
-        return launch_group<T, V, 8>(stream, a);
-    }
-    static_assert(TRTAMD_ROTARY_MAX_HEAD <= 32 * lane_values(1) && TRTAMD_ROTARY_MAX_HEAD <= 16 * lane_values(8), "lanes enough");
-    if constexpr (V == 8)
-    {
-        return launch_group<T, V, 16>(stream, a);
-    }
-    else
-    {
-        return lanes <= 16 ? launch_group<T, V, 16>(stream, a) : launch_group<T, V, 32>(stream, a);
-    }
+    return a.adjacent ? ceil_div(a.d, 2 * V) : a.half / V + ceil_div(a.d - 2 * a.half, 2 * V);
 }
 
 // Whether chunks of V values start at multiples of their size everywhere.
@@ -455,17 +401,128 @@ bool fits(RotaryArgs const& a, int V)
     return ok;
 }
 
+// The kernel of a call: values a load, lanes a head, stores past the caches.
+struct Route
+{
+    int values, lanes;
+    bool pastCaches;
+};
+
+// The least of what a store instruction writes of a head side by side, in values: the rotated chunks and the others are in places of
+// their own, and so are first and second chunks.
+int shortest_row(RotaryArgs const& a, int V, int lanes)
+{
+    int const pairSlots = a.adjacent ? 0 : a.half / V, slots = slots_of(a, V);
+    bool const odd = (a.adjacent ? a.d : a.d - 2 * a.half) % (2 * V) != 0; // the last slot has one chunk
+    int shortest = a.d;
+    for (int from = 0; from < slots; from += lanes)
+    {
+        int const end = std::min(from + lanes, slots), pairs = std::max(std::min(end, pairSlots) - from, 0), first = end - from - pairs;
+        int const second = first - (odd && end == slots ? 1 : 0);
+        for (int const chunks : {pairs, first, second})
+        {
+            shortest = chunks > 0 ? std::min(shortest, chunks * V) : shortest;
+        }
+    }
+    return shortest;
+}
+
+// Where each row of values that a store instruction writes side by side is longer than 64 bytes, or of 64 and the outputs no more
+// than half of the L2s: what ordinary stores leave there is written back at the kernel's end, while nothing else runs.  us by
+// itself, past the caches / ordinary, FP16, halves, heads of Q and of K: 4963 tokens of 12 x 64 7.3 / 7.8, but of 16 x 64 9.2 / 8.6
+// (20 MB), 33289 of 16 x 64 55 / 53; images (16 x 80) 23.7 / 25.7, a clip (12 x 128) 45 / 49, 33289 of 16 x 128 95 / 100.  Shorter
+// rows reach the memory one by one: 33289 of 16 x 32 45 / 32, of 16 x 64 with 32 rotated 66 / 56, of 16 x 96 with 48 96 / 91 (of 16 x
+// 72 with 36 and 16 x 80 with 40 121 / 122 and 87 / 89).  With the attention behind it (in place, 128 keys) the two are the same to 1
+// %; what reads the outputs faster than that finds less of them in the last-level cache: with a copy of them behind it, 4963 of 16 x
+// 128 take 37 / 32, images 56 / 47, 4963 of 16 x 80 with 40 rotated 34 / 29.
+template <typename T>
+bool past_caches(RotaryArgs const& a, int V, int lanes)
+{
+    int const row = shortest_row(a, V, lanes) * (int) sizeof(T);
+    return row > 64 || (row == 64 && (int64_t) a.T * a.heads * a.d * (int64_t) sizeof(T) <= (int64_t) 16 << 20);
+}
+
+template <typename T>
+Route route_of(RotaryArgs const& a)
+{
+    int V = 16 / (int) sizeof(T);
+    while (V > 1 && !fits<T>(a, V))
+    {
+        V /= 2;
+    }
+    int const need = ceil_div(slots_of(a, V), lane_values(V) / (2 * V));
+    int lanes = V >= 4 ? 2 : 8;
+    while (lanes < need)
+    {
+        lanes *= 2;
+    }
+    return {V, lanes, V > 1 && past_caches<T>(a, V, lanes)};
+}
+
+// One of the kernels for the norms.
+template <typename T, int V, int G, bool ADJACENT, bool PAST>
+auto kernel_of(int norm)
+{
+    return norm == TRTAMD_QK_NORM_NONE ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_NONE, PAST>
+        : norm == TRTAMD_QK_NORM_RMS  ? qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_RMS, PAST>
+                                      : qk_norm_rotary_kernel<T, V, G, ADJACENT, TRTAMD_QK_NORM_LAYER, PAST>;
+}
+
+template <typename T, int V, int G>
+int launch_group(hipStream_t stream, RotaryArgs a, [[maybe_unused]] bool past)
+{
+    constexpr int kRows = 256 / G;
+    dim3 const grid((unsigned) ceil_div<int64_t>((int64_t) a.T * a.heads, kRows));
+    a.pitch = ceil_div(a.half, V < 4 ? 4 : V) * (V < 4 ? 4 : V);
+    // the rows of a workgroup are heads of no more tokens than this
+    unsigned const lds = (unsigned) (2 * a.pitch * (ceil_div(kRows - 1, a.heads) + 1)) * sizeof(float);
+    auto kernel = a.adjacent ? kernel_of<T, V, G, true, false>(a.norm) : kernel_of<T, V, G, false, false>(a.norm);
+    if constexpr (V > 1 && G * V * sizeof(T) >= 64) // no row is longer than a head's lanes
+    {
+        if (past)
+        {
+            kernel = a.adjacent ? kernel_of<T, V, G, true, true>(a.norm) : kernel_of<T, V, G, false, true>(a.norm);
+        }
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a);
+    return check_launch("qk_norm_rotary_kernel");
+}
+
+template <typename T, int V>
+int launch_width(hipStream_t stream, RotaryArgs const& a, Route const& r)
+{
+    static_assert(TRTAMD_ROTARY_MAX_HEAD <= 32 * lane_values(1) && TRTAMD_ROTARY_MAX_HEAD <= 16 * lane_values(8), "lanes enough");
+    if constexpr (V >= 4)
+    {
+        if (r.lanes <= 4)
+        {
+            return r.lanes == 2 ? launch_group<T, V, 2>(stream, a, r.pastCaches) : launch_group<T, V, 4>(stream, a, r.pastCaches);
+        }
+    }
+    if constexpr (V < 8)
+    {
+        if (r.lanes == 32)
+        {
+            return launch_group<T, V, 32>(stream, a, r.pastCaches);
+        }
+    }
+    return r.lanes == 8 ? launch_group<T, V, 8>(stream, a, r.pastCaches) : launch_group<T, V, 16>(stream, a, r.pastCaches);
+}
+
 template <typename T>
 int launch_type(hipStream_t stream, RotaryArgs const& a)
 {
+    Route const r = route_of<T>(a);
     if constexpr (sizeof(T) == 2)
     {
-        if (fits<T>(a, 8))
+        if (r.values == 8)
         {
-            return launch_width<T, 8>(stream, a);
+            return launch_width<T, 8>(stream, a, r);
         }
     }
-    return fits<T>(a, 4) ? launch_width<T, 4>(stream, a) : fits<T>(a, 2) ? launch_width<T, 2>(stream, a) : launch_width<T, 1>(stream, a);
+    return r.values == 4 ? launch_width<T, 4>(stream, a, r)
+        : r.values == 2  ? launch_width<T, 2>(stream, a, r)
+                         : launch_width<T, 1>(stream, a, r);
 }
 
 int bad(char const* what)
@@ -573,18 +630,8 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
     return TRTAMD_STATUS_SUCCESS;
 }
 
-} // namespace
-} // namespace trtamd
-
-using namespace trtamd;
-
-extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, trtamd_qk_norm_rotary_params const* p)
+RotaryArgs args_of(trtamd_qk_norm_rotary_params const* p)
 {
-    int const st = check(data_type, p);
-    if (st != TRTAMD_STATUS_SUCCESS || p->T == 0 || p->q_heads + p->k_heads == 0)
-    {
-        return st;
-    }
     RotaryArgs a{};
     bool const norms = p->norm != TRTAMD_QK_NORM_NONE, layer = p->norm == TRTAMD_QK_NORM_LAYER;
     a.side[0] = {p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride,
@@ -610,5 +657,32 @@ extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, 
     }
     a.headsDiv = fast_div((uint32_t) a.heads);
     a.halfDiv = fast_div((uint32_t) (a.half > 0 ? a.half : 1));
+    return a;
+}
+
+} // namespace
+} // namespace trtamd
+
+using namespace trtamd;
+
+extern "C" int trtamd_qk_norm_rotary(trtamd_stream_t stream, int32_t data_type, trtamd_qk_norm_rotary_params const* p)
+{
+    int const st = check(data_type, p);
+    if (st != TRTAMD_STATUS_SUCCESS || p->T == 0 || p->q_heads + p->k_heads == 0)
+    {
+        return st;
+    }
+    RotaryArgs const a = args_of(p);
     return data_type == 1 ? launch_type<f16>(as_stream(stream), a) : launch_type<float>(as_stream(stream), a);
+}
+
+extern "C" int trtamd_test_qk_norm_rotary_route(int32_t data_type, trtamd_qk_norm_rotary_params const* p)
+{
+    if (check(data_type, p) != TRTAMD_STATUS_SUCCESS || p->T == 0 || p->q_heads + p->k_heads == 0)
+    {
+        return -1;
+    }
+    RotaryArgs const a = args_of(p);
+    Route const r = data_type == 1 ? route_of<f16>(a) : route_of<float>(a);
+    return r.values | r.lanes << 8 | (int) r.pastCaches << 16;
 }
