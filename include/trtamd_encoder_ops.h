@@ -92,8 +92,8 @@ TRTAMD_API int trtamd_quantize_fp16_per_token(trtamd_stream_t stream, int32_t T,
     int64_t in_stride, int8_t* out, float* scales);
 
 /* out[t][n] = binary16(f(acc * token_scale[t] * channel_scale[n] + bias[n])), acc = sum_k a[t][k] * w[n][k] (exact), f =
- * identity (TRTAMD_LINEAR_AFFINE) or erf-GELU (TRTAMD_LINEAR_GELU, to 8.5e-5 of its value; of infinities, which only scales or offsets
- * near the end of binary32 give, NaN).  Scales, sums and f are binary32, with one rounding at the end; a token's results do not depend on
+ * identity (TRTAMD_LINEAR_AFFINE) or erf-GELU (TRTAMD_LINEAR_GELU, to 8.5e-5 of its value; of infinities, which products past the end of
+ * binary32 give, infinity and 0).  Scales, sums and f are binary32, with one rounding at the end; a token's results do not depend on
  * what other tokens are in the call. */
 typedef struct trtamd_int8_token_linear_params
 {

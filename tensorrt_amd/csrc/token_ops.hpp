@@ -86,10 +86,10 @@ __device__ inline u16x2 max_abs(u16x2 m, u32x4 const& v)
 // by what it does to the result: 8.5e-5 of it where that is a normal binary16 (a sixth to a third of the half step that rounding
 // costs), 5.2e-9 below (a sixth).  Degree 7 gives 4e-6 for two more multiply-adds, which are 6 of 170 us at 33289 tokens x 1024 ->
 // 4096: the vector ALU and the matrix cores take turns there.  The leading coefficient is negative, so the term vanishes for
-// larger a; a NaN stays one (through a).
+// larger a, also of infinities (an infinity times nothing would be a NaN); a NaN stays one, through the IEEE minimum.
 __device__ inline float gelu_f16(float y)
 {
-    float const a = fabsf(y);
+    float const a = __builtin_elementwise_minimum(fabsf(y), 0x1p126f);
     float p = fmaf(a, -3.205105604e-04f, 5.827311892e-03f);
     p = fmaf(p, a, -4.823749512e-02f);
     p = fmaf(p, a, -4.641202092e-01f);

@@ -470,3 +470,23 @@ def test_the_largest_sums(api, T):
     api.check(api.int8_token_linear(stream(), C.byref(p)))
     sync()
     assert_within(host(one)[:T], *reference(q, scales, layer.w, layer.channel, layer.bias, False))
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 1024, 64), (20, 128, 64), (4, 4160, 64), (300, 256, 288), (1500, 192, 320), (2600, 1024, 1024)])
+def test_gelu_beyond_binary32(api, T, K, N):
+    """Products past the end of binary32, either way: infinity and zero, as for every large result; the other channels as ever."""
+    layer = Layer(api, T, K, N, gelu=True, bias=False)
+    layer.channel[::2] = 3e38
+    layer.dc = dev(layer.channel)
+    one, two = layer.out(), layer.out()
+    layer.token(one)
+    layer.dynamic(two, layer.workspace())
+    sync()
+    assert np.array_equal(bits(one), bits(two))
+    q, scales = quantised(layer.x)
+    acc = q.astype(np.float64) @ layer.w.astype(np.float64).T
+    got, up, down = host(one)[:T], acc[:, ::2] > 1000, acc[:, ::2] < -1000  # scales of 0.005 and more: beyond 1.5e39
+    assert up.any() and down.any() and (scales > 0.005).all()
+    assert (got[:, ::2][up] == np.inf).all() and (got[:, ::2][down] == 0).all()
+    want, tol = layer.want()
+    assert_within(got[:, 1::2], want[:, 1::2], tol[:, 1::2])
