@@ -92,9 +92,10 @@ TRTAMD_API int trtamd_quantize_fp16_per_token(trtamd_stream_t stream, int32_t T,
     int64_t in_stride, int8_t* out, float* scales);
 
 /* out[t][n] = binary16(f(acc * token_scale[t] * channel_scale[n] + bias[n])), acc = sum_k a[t][k] * w[n][k] (exact), f =
- * identity (TRTAMD_LINEAR_AFFINE) or erf-GELU (TRTAMD_LINEAR_GELU, to 8.5e-5 of its value; of infinities, which products past the end of
- * binary32 give, infinity and 0).  Scales, sums and f are binary32, with one rounding at the end; a token's results do not depend on
- * what other tokens are in the call. */
+ * identity (TRTAMD_LINEAR_AFFINE) or erf-GELU (TRTAMD_LINEAR_GELU), which before the rounding to binary16 is within 8.5e-5 of its
+ * value where that is a normal binary16, 2^-14 or more, and within 5.2e-9 where it is less; of infinities, which products past the
+ * end of binary32 give, it is infinity and 0.  Scales, sums and f are binary32, with one rounding at the end; a token's results do
+ * not depend on what other tokens are in the call. */
 typedef struct trtamd_int8_token_linear_params
 {
     int8_t const* a;            /* [T][K] */
