@@ -157,8 +157,8 @@ enum
  * q and k are read at q + t * q_token_stride + head * q_head_stride (elements), each head's d values in a row, and written
  * to q_out and k_out in the same way: the packed layouts of the attention plugins ([token][head][q|k|v][d] has token strides
  * of 3 N d and head strides of 3 d) as well as tensors of their own, with fewer heads of k than of q or none.  q_out = q with the
- * same strides works in place; other overlaps of what is written with anything else in the call are not allowed.  T * (q_heads + k_heads)
- * < 2^26. */
+ * same strides works in place, if no two heads overlap (heads that are only read may: a stride of 0 is one head for all); other
+ * overlaps of what is written with anything else in the call are not allowed.  T * (q_heads + k_heads) < 2^26. */
 typedef struct trtamd_qk_norm_rotary_params
 {
     void const* q;

@@ -13,6 +13,7 @@
 #include "trtamd_test_hooks.h"
 
 #include <algorithm>
+#include <utility>
 
 namespace trtamd
 {
@@ -530,6 +531,39 @@ int bad(char const* what)
     return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: %s", what);
 }
 
+// Whether any two of n x m rows of d values, at i * a + j * b, overlap.
+bool rows_overlap(int64_t n, int64_t a, int64_t m, int64_t b, int64_t d)
+{
+    typedef __int128 Wide; // strides are any 64 bits
+    auto const size = [](Wide v) { return v < 0 ? -v : v; };
+    if (size(a) > size(b))
+    {
+        std::swap(a, b);
+        std::swap(n, m);
+    }
+    if (size(a) >= d && size(b) >= (n - 1) * size(a) + d)
+    {
+        return false; // all rows of one kind lie between two of the other
+    }
+    if (n > m)
+    {
+        std::swap(a, b);
+        std::swap(n, m);
+    }
+    for (int64_t i = 0; i < n; ++i) // the distance of two rows is i * a + j * b, least where j is next to -i * a / b
+    {
+        Wide const off = (Wide) i * a, near = b == 0 ? i == 0 : -off / b;
+        for (Wide j = near - 1; j <= near + 1; ++j)
+        {
+            if (size(j) < m && (i != 0 || j != 0) && size(off + j * b) < d)
+            {
+                return true;
+            }
+        }
+    }
+    return false;
+}
+
 int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
 {
     if (type != 0 && type != 1)
@@ -562,6 +596,7 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
     {
         return bad("neither a norm nor a rotation");
     }
+    bool const many = (int64_t) p->T * ((int64_t) p->q_heads + p->k_heads) >= (int64_t) 1 << 26; // a launch has 2^32 threads
     size_t const size = type == 1 ? 2 : 4;
     for (int i = 0; i < 2; ++i)
     {
@@ -583,6 +618,12 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
         if (data[0] == data[1] && !(sameToken && sameHead))
         {
             return bad("in place the strides have to be the same");
+        }
+        if (data[0] == data[1] && !many
+            && rows_overlap(p->T, q ? p->q_token_stride : p->k_token_stride, q ? p->q_heads : p->k_heads,
+                q ? p->q_head_stride : p->k_head_stride, p->d))
+        {
+            return bad("in place no two heads may overlap");
         }
         for (int j = 0; j < 2; ++j)
         {
@@ -623,9 +664,9 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
             return set_error(TRTAMD_STATUS_BAD_PARAM, "qk_norm_rotary: sections of %lld pairs, rotary_dim has %d", (long long) sum, pairs);
         }
     }
-    if ((int64_t) p->T * ((int64_t) p->q_heads + p->k_heads) >= (int64_t) 1 << 26)
+    if (many)
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: 2^26 heads of tokens or more"); // a launch has 2^32 threads
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "qk_norm_rotary: 2^26 heads of tokens or more");
     }
     return TRTAMD_STATUS_SUCCESS;
 }

@@ -59,3 +59,31 @@ def test_longer_rows_go_past_the_caches(T, dtype, d, rotary, adjacent):
 
 def test_without_a_launch():
     assert route(FP16, 0, 4, 64, 64) == route(FP16, 8, 4, 64, 66) == route(2, 8, 4, 64, 64) == -1
+
+
+def in_place(T, heads, d, token_stride, head_stride, dtype=FP16):
+    """Q alone, in place."""
+    p = capi.QkNormRotaryParams(q=A, q_out=A, q_token_stride=token_stride, q_head_stride=head_stride, q_out_token_stride=token_stride,
+                                q_out_head_stride=head_stride, T=T, q_heads=heads, d=d, norm=1, q_weight=A, rotary_dim=d, frequencies=A,
+                                positions=A, axes=1)
+    return capi.api().test_qk_norm_rotary_route(dtype, C.byref(p)), capi.api().last_error_str()
+
+
+@pytest.mark.parametrize("T,heads,d,token_stride,head_stride", [
+    (4, 2, 64, 64, 0), (4, 1, 64, 0, 64), (4, 1, 64, 32, 0), (1, 3, 64, 999, 63), (4, 4, 64, 64, 64), (3, 5, 64, 320, 160 - 1),
+    (9, 2, 64, 64, 8 * 64), (3, 3, 64, -64, 128), (2, 2, 64, 1 << 62, (1 << 62) + 32), (4, 2, 64, -64, 0), (1000, 3, 64, 100, 50)])
+def test_heads_that_overlap_are_refused_in_place(T, heads, d, token_stride, head_stride):
+    """One would be read after another has been written over it."""
+    status, text = in_place(T, heads, d, token_stride, head_stride)
+    assert status == -1 and "overlap" in text
+
+
+@pytest.mark.parametrize("T,heads,d,token_stride,head_stride", [
+    (4, 2, 64, 128, 64), (4, 2, 64, 384, 192), (4, 2, 64, 64, 256), (4, 1, 64, 64, 0), (1, 4, 64, 0, 64), (1, 1, 64, 0, 0), (3, 2, 64, 128, 192),
+    (8, 2, 64, 64, 8 * 64), (4, 2, 64, -128, 64), (4, 2, 64, -128, -64), (2, 2, 64, 1 << 62, (1 << 62) + 64), (5, 5, 64, 5 * 64, 64)])
+def test_heads_side_by_side_are_taken_in_place(T, heads, d, token_stride, head_stride):
+    assert in_place(T, heads, d, token_stride, head_stride)[0] > 0
+
+
+def test_heads_that_overlap_may_be_read():
+    assert route(FP16, 8, 4, 64, 64, k_head_stride=0)[0] == route(FP16, 8, 4, 64, 64, q_token_stride=0, q_head_stride=0)[0] == 8
