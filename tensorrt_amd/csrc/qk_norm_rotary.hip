@@ -606,9 +606,9 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
             continue;
         }
         void const* const data[2] = {q ? p->q : p->k, q ? p->q_out : p->k_out};
+        int const used = p->norm == TRTAMD_QK_NORM_NONE ? 0 : p->norm == TRTAMD_QK_NORM_RMS ? 1 : 2;
         float const* const vectors[2] = {q ? p->q_weight : p->k_weight, q ? p->q_bias : p->k_bias};
-        if (data[0] == nullptr || data[1] == nullptr || (norms && vectors[0] == nullptr)
-            || (p->norm == TRTAMD_QK_NORM_LAYER && vectors[1] == nullptr))
+        if (data[0] == nullptr || data[1] == nullptr || (used > 0 && vectors[0] == nullptr) || (used > 1 && vectors[1] == nullptr))
         {
             return bad("null pointer");
         }
@@ -627,7 +627,7 @@ int check(int32_t type, trtamd_qk_norm_rotary_params const* p)
         }
         for (int j = 0; j < 2; ++j)
         {
-            if (reinterpret_cast<uintptr_t>(data[j]) % size != 0 || reinterpret_cast<uintptr_t>(vectors[j]) % 4 != 0)
+            if (reinterpret_cast<uintptr_t>(data[j]) % size != 0 || (j < used && reinterpret_cast<uintptr_t>(vectors[j]) % 4 != 0))
             {
                 return bad("pointers must be aligned to their values");
             }

@@ -87,3 +87,11 @@ def test_heads_side_by_side_are_taken_in_place(T, heads, d, token_stride, head_s
 
 def test_heads_that_overlap_may_be_read():
     assert route(FP16, 8, 4, 64, 64, k_head_stride=0)[0] == route(FP16, 8, 4, 64, 64, q_token_stride=0, q_head_stride=0)[0] == 8
+
+
+def test_pointers_that_are_not_used_may_be_anything():
+    odd = A + 1
+    assert route(FP16, 8, 4, 64, 64, norm=0, q_weight=odd, k_weight=odd, q_bias=odd, k_bias=odd)[0] == 8
+    assert route(FP16, 8, 4, 64, 64, norm=1, q_bias=odd, k_bias=odd)[0] == 8
+    assert route(FP16, 8, 4, 64, 0, norm=1, frequencies=odd, positions=odd)[0] == 8
+    assert route(FP16, 8, 4, 64, 64, norm=2, q_bias=odd) == route(FP16, 8, 4, 64, 64, norm=1, k_weight=odd) == -1
