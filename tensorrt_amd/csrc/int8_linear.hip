@@ -2840,19 +2840,38 @@ int int8_token_linear_check(char const* what, trtamd_int8_token_linear_params co
 
 } // namespace trtamd
 
-extern "C" int trtamd_test_linear_plan(int32_t interleaved, int32_t T, int32_t row_bytes, int32_t N, int32_t gelu)
+namespace trtamd
 {
-    using namespace trtamd;
-    if (T <= 0 || row_bytes <= 0 || N <= 0 || row_bytes % 64 != 0 || N % 32 != 0)
+namespace
+{
+
+int plan_of(bool interleaved, int32_t T, int32_t rowBytes, int32_t N, bool gelu, float const* tokenScale)
+{
+    if (T <= 0 || rowBytes <= 0 || N <= 0 || rowBytes % 64 != 0 || N % 32 != 0)
     {
         return -1;
     }
     LinearArgs a{};
     a.T = T;
-    a.K = row_bytes;
+    a.K = rowBytes;
     a.N = N;
+    a.tokenScale = tokenScale;
     int64_t const smallTiles = place_large_tiles(a);
-    return interleaved ? plan_behind_large_tiles<true>(a, smallTiles, gelu != 0) : plan_behind_large_tiles<false>(a, smallTiles, gelu != 0);
+    return interleaved ? plan_behind_large_tiles<true>(a, smallTiles, gelu) : plan_behind_large_tiles<false>(a, smallTiles, gelu);
+}
+
+} // namespace
+} // namespace trtamd
+
+extern "C" int trtamd_test_linear_plan(int32_t interleaved, int32_t T, int32_t row_bytes, int32_t N, int32_t gelu)
+{
+    return trtamd::plan_of(interleaved != 0, T, row_bytes, N, gelu != 0, nullptr);
+}
+
+extern "C" int trtamd_test_token_linear_plan(int32_t T, int32_t K, int32_t N, int32_t gelu)
+{
+    float const some = 0.f; // its address says which layer it is
+    return trtamd::plan_of(false, T, K, N, gelu != 0, &some);
 }
 
 extern "C" int64_t trtamd_test_linear_estimates(void)
