@@ -1311,7 +1311,8 @@ constexpr bool scales_late(int ringBytes)
 //   fragments read ahead                                      38.7 / 15.8 / 46.5 / 43.0
 //   loads spread out, order kept                              36.0 / 14.8 / 45.1 / 39.3
 //   rows stored whole, through the L2 (see the end)           32.6 / 12.5 / 41.2 / 35.5
-template <bool IL, bool IL_OUT, int EPI, int WM, int WN, int MT, int NT, int RING, int KS = 2>
+// REGISTERS: what a lane has.
+template <bool IL, bool IL_OUT, int EPI, int WM, int WN, int MT, int NT, int RING, int KS = 2, int REGISTERS = 256>
 __device__ __forceinline__ void linear_tile_dma(
     LinearArgs const& p, int const n0, int const t0, uint8_t* __restrict__ lds)
 {
@@ -1555,10 +1556,15 @@ __device__ __forceinline__ void linear_tile_dma(
         uint8_t* const own = lds + (kOneSlot ? slot * STAGE : 0) + wave * (32 * kRow); // nobody needs any slot any more
         int const nw = n0 + wm * MT * 32;
         BlockScales sc[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-        {
+        auto const scales_of = [&](int i) {
             sc[i] = load_block_scales<EPI>(sScale + (wm * MT + i) * 32, sScale + kBigTile + (wm * MT + i) * 32);
+        };
+        // read once for all tokens, where a lane can hold them beside its sums
+        constexpr bool kHeld = MT * NT * 16 + MT * 32 + 32 <= REGISTERS;
+#pragma unroll
+        for (int i = 0; kHeld && i < MT; ++i)
+        {
+            scales_of(i);
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -1566,6 +1572,10 @@ __device__ __forceinline__ void linear_tile_dma(
 #pragma unroll
             for (int i = 0; i < MT; ++i)
             {
+                if constexpr (!kHeld)
+                {
+                    scales_of(i);
+                }
                 u32x4 first, second;
                 pack_half_block<EPI>(acc[i][j], sc[i], ts[j], first, second);
                 u32x4* dst = reinterpret_cast<u32x4*>(own + (lane & 31) * kRow + i * 64 + (lane >> 5) * 32);
@@ -1724,7 +1734,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_SIMD) void linear_tile_kernel(uint
     uint32_t const tile = xcd_remap(blockIdx.x, (uint32_t) p.mainTiles);
     uint32_t const pan = tile / p.perPanelDiv, rem = tile - pan * p.perPanelDiv.d;
     uint32_t const tokenTile = rem / p.panelDiv, inPanel = rem - tokenTile * p.panelDiv.d;
-    linear_tile_dma<IL, IL_OUT, EPI, WM, WN, MT, NT, RING, KS>(
+    linear_tile_dma<IL, IL_OUT, EPI, WM, WN, MT, NT, RING, KS, 512 / PER_SIMD>(
         p, (int) (pan * p.panelDiv.d + inPanel) * (WM * MT * 32), (int) tokenTile * (WN * NT * 32), lds);
 }
 
