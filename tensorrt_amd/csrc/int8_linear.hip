@@ -2159,8 +2159,12 @@ constexpr TileCost kTileCosts[3][kLinearPlans] = {
 // Fitted to launches by themselves (graph replays, three sets of operands in turn), 720 sizes of 1 to 33289 tokens, rows of 64
 // to 4032 bytes, 64 to 5120 channels, with and without GELU: 2.0 % more than the best of the nine plans in the mean on 180
 // other sizes too, where the constants and tiles of the layers above take 4.0 %, and 9 % from 2000 tokens on (33289 x 960 ->
-// 4096: 247 us, now 157 in 256 x 256 tiles).
-constexpr TileCost kTokenTileCosts[kLinearPlans] = {{}, {128, 256, 2, 0.46f, 4.62f, 0.301f, 2.14f, 0.69f, 0.81f, 0.56f, 1.14f},
+// 4096: 247 us, now 157 in 256 x 256 tiles).  Those of 128 x 256 were fitted again without spills, on 4000 sizes: on 790 others
+// that have 24 such tiles or more 1.4 % more than the best instead of 2.0 %, none longer by more than 2 % (33289 x 960 -> 4096 with GELU
+// 192 us, now 173).  Affine layers of one or three stages are left to the other tiles: 30413 x 192 -> 1888 59 us in 128 x 256
+// tiles, 31 in 128 x 128.
+constexpr int kTokenWideRow = 256;
+constexpr TileCost kTokenTileCosts[kLinearPlans] = {{}, {128, 256, 2, 4.50f, 1.94f, 0.390f, 0.67f, 0.98f, 1.20f, 0.88f, 0.31f, 0.02f},
     {128, 128, 2, 2.16f, 1.54f, 0.186f, 0.86f, 0.71f, 0.86f, 0.55f, 0.96f}, {64, 128, 3, 2.87f, 0.72f, 0.097f, 0.42f, 0.71f, 0.82f, 0.39f, 1.68f},
     {64, 64, 4, 3.15f, 0.33f, 0.086f, 0.16f, 0.70f, 0.81f, 0.65f, 0.82f}, {}, {}, {},
     {32, 64, 1, 2.82f, 0.82f, 0.035f, 0.09f, 0.01f, 1.35f, 0.68f, 2.03f, 0.10f}, {32, 32, 1, 3.09f, 0.53f, 0.018f, 0.08f, 2.01f, 1.32f, 0.51f, 2.90f, 0.15f},
@@ -2386,7 +2390,7 @@ int cheapest_plan(LinearArgs const& a, int64_t smallTiles, bool gelu, int plan)
     float best = std::numeric_limits<float>::max();
     for (int q = kLargeTiles; q < kLinearPlans; ++q)
     {
-        if (!exists(q))
+        if (!exists(q) || (q == kTile128x256 && a.tokenScale && !gelu && a.K < kTokenWideRow))
         {
             continue;
         }
