@@ -38,6 +38,8 @@ TRTAMD_API int trtamd_test_reset_tuning(char const* name);
 TRTAMD_API int trtamd_test_linear_plan(int32_t interleaved, int32_t T, int32_t row_bytes, int32_t N, int32_t gelu);
 /* The same of a token-scaled layer (trtamd_int8_token_linear). */
 TRTAMD_API int trtamd_test_token_linear_plan(int32_t T, int32_t K, int32_t N, int32_t gelu);
+/* Whether its result goes past the last-level cache. */
+TRTAMD_API int trtamd_test_token_linear_streams(int32_t T, int32_t K, int32_t N);
 /* How often the calling thread has worked such a number out, rather than remembered it. */
 TRTAMD_API int64_t trtamd_test_linear_estimates(void);
 

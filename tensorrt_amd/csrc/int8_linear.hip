@@ -44,7 +44,8 @@ namespace
 {
 
 constexpr int kTokenRow = 1 << 17;             // values of a token-scaled layer's row: 2^17 products of -128 and -128 are 2^31
-constexpr int64_t kStreamedBytes = 64 << 20; // a quarter of the last-level cache: see store_rows
+constexpr int64_t kStreamedBytes = 64 << 20;   // a quarter of the last-level cache, and
+constexpr int64_t kTouchedBytes = 140 << 20;  // a little more than half of it: see store_rows
 constexpr int kBigTile = 256; // channels and tokens of the large workgroup tile
 
 enum Epilogue
@@ -179,9 +180,11 @@ __device__ __forceinline__ void store_out(void* p, V const& v)
 // cache too.  Results of a size that it cannot hold beside what else a layer touches only push each other out of it: 33289
 // tokens x 1024 -> 4096 (273 MB) 186 us through it and 165 past it, x 1024 -> 1024 (68 MB) 49 and 42.  What reads them next
 // gives most of that back, and for smaller ones more (the layer and the quantiser that reads it, 4963 x 768 -> 2304, 23 MB:
-// 19.8 through, 20.4 past).  Whole layers (projection, feed-forward layers, their quantisers and norms), results above 64 MiB
-// past the cache: 33289 tokens of 1024 (4096) values 539 -> 528 us, of 768 (2304) 308 -> 302, of 512 (2048) 211 -> 207; 16384
-// of 1024 259 -> 260, 9000 of them 154 -> 156, 20000 of 512 129 -> 132.  Inline assembly as in store_through_l2.
+// 19.8 through, 20.4 past).  Whole layers (projection, feed-forward layers, their quantisers and norms), first feed-forward
+// layer through / past, by what that one and its quantiser touch (FP16 tokens, 8-bit tokens, result): 108 MiB (10000 tokens of 1024, 4096)
+// 158.7 / 160.5 us, 118 173.7 / 175.0, 129 183.3 / 184.4 (24000 of 512, 2048 144.8 / 145.9), 140 199.8 / 199.9, 150 215.6 / 214.0, 161
+// 227.8 / 225.5, 176 248.6 / 240.2, 198 (30000 of 768, 2304) 265.0 / 257.4; 33289 of 1024, 4096 (358 MiB) 539 / 528.  Projections of 98 and 117
+// MiB of tokens and result are the same either way in a layer.  Inline assembly as in store_through_l2.
 __device__ __forceinline__ void store_rows(void* base, uint32_t laneOffset, u32x4 const& v, bool streaming)
 {
     uint64_t const b = reinterpret_cast<uint64_t>(base);
@@ -2680,6 +2683,13 @@ int check_fp16(trtamd_fp16_linear_params const* p)
     return TRTAMD_STATUS_SUCCESS;
 }
 
+// Whether a token-scaled layer's result goes past the last-level cache: see store_rows.
+bool streams(int64_t T, int64_t K, int64_t N)
+{
+    int64_t const result = T * N * (int64_t) sizeof(trtamd_half_t), tokens = T * K * (1 + (int64_t) sizeof(trtamd_half_t));
+    return result > kStreamedBytes && tokens + result > kTouchedBytes;
+}
+
 LinearArgs args_of(trtamd_int8_token_linear_params const& p)
 {
     LinearArgs a{};
@@ -2688,7 +2698,7 @@ LinearArgs args_of(trtamd_int8_token_linear_params const& p)
     a.alpha = p.channel_scale;
     a.beta = p.bias;
     a.tokenScale = p.token_scale;
-    a.streaming = (int64_t) p.T * p.N * (int64_t) sizeof(trtamd_half_t) > kStreamedBytes;
+    a.streaming = streams(p.T, p.K, p.N);
     a.out = p.out;
     a.T = p.T;
     a.K = p.K;
@@ -2880,6 +2890,11 @@ int plan_of(bool interleaved, int32_t T, int32_t rowBytes, int32_t N, bool gelu,
 extern "C" int trtamd_test_linear_plan(int32_t interleaved, int32_t T, int32_t row_bytes, int32_t N, int32_t gelu)
 {
     return trtamd::plan_of(interleaved != 0, T, row_bytes, N, gelu != 0, nullptr);
+}
+
+extern "C" int trtamd_test_token_linear_streams(int32_t T, int32_t K, int32_t N)
+{
+    return trtamd::streams(T, K, N);
 }
 
 extern "C" int trtamd_test_token_linear_plan(int32_t T, int32_t K, int32_t N, int32_t gelu)

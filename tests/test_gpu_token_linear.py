@@ -490,3 +490,26 @@ def test_gelu_beyond_binary32(api, T, K, N):
     assert (got[:, ::2][up] == np.inf).all() and (got[:, ::2][down] == 0).all()
     want, tol = layer.want()
     assert_within(got[:, 1::2], want[:, 1::2], tol[:, 1::2])
+
+
+@pytest.mark.parametrize("T,K,N", [(33333, 64, 2208), (33000, 128, 2304), (17001, 192, 4512), (40001, 256, 1952), (19000, 64, 4160)])
+@pytest.mark.parametrize("gelu", [False, True])
+def test_results_past_the_last_level_cache(api, T, K, N, gelu):
+    """The bits of the same tokens in calls whose results stay in the caches, and the definition on some of them."""
+    import torch
+    assert api.test_token_linear_streams(T, K, N) and not api.test_token_linear_streams(4000, K, N)
+    layer = Layer(api, T, K, N, gelu)
+    out, ws = layer.out(), layer.workspace()
+    layer.dynamic(out, ws)
+    for t in range(0, T, 4000):
+        n = min(4000, T - t)
+        part, space = dev_empty((n, N), np.float16, fill=-7), dev_empty((api.int8_dynamic_linear_workspace_size(n, K, N),), np.uint8)
+        p = params(capi.Int8DynamicLinearParams, n, K, N, gelu, layer.dw, layer.dc, layer.db, part, a=ptr(layer.dx[t:]), a_stride=K,
+                   workspace=ptr(space), workspace_bytes=space.numel())
+        api.check(api.int8_dynamic_linear(stream(), C.byref(p)))
+        assert torch.equal(part.view(torch.int16), out[t:t + n].view(torch.int16)), t
+    sync()
+    assert (host(out[T]) == -7).all()
+    some = np.r_[0:40, T - 300:T]
+    want, tol = reference(*quantised(layer.x[some]), layer.w, layer.channel, layer.bias, gelu)
+    assert_within(host(out[:T])[some], want, tol)
