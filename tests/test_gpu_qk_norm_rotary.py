@@ -348,3 +348,12 @@ def test_the_turned_inner_product_depends_on_the_distance_only(api):
         # 64 products of values off by 8.6 steps of |a| + |b| each
         bound = 2 * 8.6 * STEP * 4 * (np.abs(p.q[0]).max() * np.abs(p.k[0]).sum(-1)).max() * 2
         assert np.abs(near - far).max() <= bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 2, 255, 1000])
+@pytest.mark.parametrize("hq,hk,d,rotary,norm", [(1, 0, 64, 64, "rms"), (0, 1, 64, 64, "layer"), (1, 0, 256, 256, "rms"), (1, 0, 7, 2, "layer"),
+                                                 (0, 1, 32, 0, "rms"), (1, 0, 2, 2, "none")])
+def test_one_head_in_all(api, dtype, T, hq, hk, d, rotary, norm):
+    """Each row of a workgroup is a token of its own, with angles of its own."""
+    run(api, dtype=dtype, T=T, hq=hq, hk=hk, d=d, rotary=rotary, norm=norm)

@@ -513,3 +513,41 @@ def test_results_past_the_last_level_cache(api, T, K, N, gelu):
     some = np.r_[0:40, T - 300:T]
     want, tol = reference(*quantised(layer.x[some]), layer.w, layer.channel, layer.bias, gelu)
     assert_within(host(out[:T])[some], want, tol)
+
+
+def test_two_threads_at_once(api):
+    """Calls of two threads, each with layers and a stream of its own: plans are remembered by each thread for itself."""
+    import threading
+
+    import torch
+    work = [[Layer(api, T, K, N, gelu, seed=s) for T, K, N, gelu in sizes]
+            for s, sizes in enumerate([[(600, 960, 1056, False), (5003, 960, 1056, False), (1, 1024, 512, True)],
+                                       [(600, 960, 1056, True), (3, 4096, 224, False), (2049, 384, 1536, True)]])]
+    want = []
+    for layers in work:
+        for layer in layers:
+            want.append(layer.out())
+            layer.dynamic(want[-1], layer.workspace())
+    outs = [[layer.out() for layer in layers] for layers in work]
+    spaces = [[layer.workspace() for layer in layers] for layers in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    sync()
+    failed = []
+
+    def calls(i):
+        try:
+            for _ in range(20):
+                for layer, out, ws in zip(work[i], outs[i], spaces[i]):
+                    layer.dynamic(out, ws, streams[i].cuda_stream)
+        except Exception as e:  # an assertion of a thread is not seen by itself
+            failed.append(e)
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    sync()
+    assert not failed
+    for got, ref in zip(outs[0] + outs[1], want):
+        assert np.array_equal(bits(got), bits(ref))
