@@ -3,7 +3,7 @@
 //   y = x | x / sqrt(mean(x^2) + eps) w | (x - mean) / sqrt(var + eps) w + b        over the d values of a head
 //   (a, b) -> (a cos(p f) - b sin(p f), b cos(p f) + a sin(p f))                    for its rotary_dim / 2 pairs
 //
-// HBM streaming: each value is read and written once.  33289 tokens, 16 and 16 heads of 64 in the packed layout, FP16: 55 us, 4.9 TB/s
+// HBM streaming: each value is read and written once.  33289 tokens, 16 and 16 heads of 64 in the packed layout, FP16: 54 us, 5.0 TB/s
 // (a copy of 1 GiB reaches 5.2); heads of 128 5.7, in FP32 5.9 TB/s.  A group of a few lanes per head, each with 16 bytes a load, keeps the norm's sums
 // within a row of 16 lanes and every load whole; with the angles worked out by every group for itself it took 88 us (their
 // binary64 and the sine are 130 instructions a pair), with loads one behind the other 63.
