@@ -188,6 +188,139 @@ TRTAMD_API int trtamd_qk_norm_rotary(
     trtamd_stream_t stream, int32_t data_type, trtamd_qk_norm_rotary_params const* params);
 
 /* ------------------------------------------------------------------------------------------
+ * A cache of keys and values in 8 bits, in pages, for sequences that grow: written as the projection leaves them (with
+ * trtamd_qk_norm_rotary before it where the layer has that), attended to, and read back.  No counterpart in the reference's plugins,
+ * whose attention has all of a sequence in one call.
+ *
+ * Token t of sequence b is token t % page_tokens of page page_table[b * max_pages + t / page_tokens]; the keys of head h of page p
+ * are k[p][h][token][d], its values v[p][h][d][token] (a value's tokens side by side, as the second product wants them), one byte
+ * each, INT8 or E4M3 (a sign, 4 bits of exponent, 3 of mantissa, no infinities), and what they stand for is the byte's value times
+ * k_scale[p][h] or v_scale[p][h].
+ *
+ * A call has cu_seqlens[b + 1] - cu_seqlens[b] tokens of sequence b, rows cu_seqlens[b] on of its tensors, which are the LAST ones
+ * of the lengths[b] that the sequence has.  Lengths, rows and pages are read on the GPU, so a captured call follows them: B, T,
+ * max_tokens and max_pages are what may not be passed.  What does not fit is left out and harms nothing: rows at or behind T,
+ * a sequence's rows from the max_tokens-th on (neither read nor written), tokens before a sequence's first one or behind its
+ * max_pages pages, and pages whose number is not in 0 .. pages - 1 (not written; read as zeros; not attended to, so that
+ * pages that a window has left behind can go back to the pool with -1 in their place).
+ *
+ * No page may be written for two sequences, or two rows, of a call; reading them may be shared.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct trtamd_kv_cache
+{
+    void* k;                   /* [pages][kv_heads][page_tokens][d] */
+    void* v;                   /* [pages][kv_heads][d][page_tokens] */
+    float* k_scale;            /* [pages][kv_heads] */
+    float* v_scale;            /* [pages][kv_heads] */
+    int32_t const* page_table; /* [B][max_pages] */
+    int32_t const* lengths;    /* [B]: tokens of each sequence, those of the call included */
+    int32_t const* cu_seqlens; /* [B + 1]: rows of each sequence in the call's tensors */
+    int32_t data_type;         /* of k and v: 2 = INT8, 6 = FP8 E4M3 (nvinfer1::DataType values) */
+    int32_t pages;             /* in the pool */
+    int32_t page_tokens;       /* 16, 32, 64 or 128 */
+    int32_t kv_heads;
+    int32_t d;                 /* a multiple of 16, at most 256 */
+    int32_t B;                 /* sequences, at most 65535 */
+    int32_t max_pages;         /* entries of a sequence in page_table */
+    int32_t max_tokens;        /* rows of a sequence in the call, or more */
+    int32_t T;                 /* rows of the call's tensors */
+} trtamd_kv_cache;
+
+/* Quantises the call's rows into the cache.  top = 127 (INT8) or 448 (E4M3); for each page and head that gets new tokens, for keys and
+ * values by themselves, a = the largest absolute value among the new ones:
+ *   where the new tokens begin the page, or what it held had the scale 0: scale = a / top;
+ *   otherwise the scale s stays while a <= s * top, and else becomes s * 2^n with the smallest n that makes it so, and what the page
+ *   held becomes round_half_even(byte * 2^-n).
+ *   byte = round_half_even(x * (1 / scale)), within -top .. top; 0 where the scale is 0.
+ * All of it in binary32, each operation rounded correctly.  Doubling keeps what a page goes through as it fills bounded: whatever
+ * the order, an INT8 token is within one step of its last scale (half a step where the scale never grew), and in E4M3 only what
+ * falls below its normal numbers is rounded again.  New values that hold an infinity or a NaN leave the scale NaN and zeros in their
+ * place, so that whatever is computed from this page and head is NaN, and nothing else is; a scale of NaN stays until the page is
+ * begun again.  Other pages, heads and tokens are left as they were.  k and v: row t, head h at k + t * k_token_stride + h * k_head_stride, multiples of 8
+ * elements, d values in a row. */
+typedef struct trtamd_kv_cache_write_params
+{
+    trtamd_kv_cache cache;
+    trtamd_half_t const* k;
+    trtamd_half_t const* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} trtamd_kv_cache_write_params;
+
+TRTAMD_API int trtamd_kv_cache_write(trtamd_stream_t stream, trtamd_kv_cache_write_params const* params);
+
+/* The call's rows from the cache, binary16(byte * scale): the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence. */
+typedef struct trtamd_kv_cache_read_params
+{
+    trtamd_kv_cache cache;
+    trtamd_half_t* k;
+    trtamd_half_t* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} trtamd_kv_cache_read_params;
+
+TRTAMD_API int trtamd_kv_cache_read(trtamd_stream_t stream, trtamd_kv_cache_read_params const* params);
+
+/* Attention of the call's rows over their sequences in the cache, causal: row i of a sequence, its token p = begin + i, sees the
+ * tokens j <= p, with a window only those with j > p - window, and the first `sinks` tokens whatever the window is.
+ *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j),  k_j and v_j what the cache's bytes stand for.
+ * Products of the bytes' values are exact, sums, maxima and exponentials binary32; the weights of the second product are rounded
+ * to binary16 once, half to even.  A row that sees nothing is zeros.  Query head h reads head h / (q_heads / kv_heads) of the cache.
+ * A result can differ in its last bits between calls of other sizes or estimates, not between calls of the same.
+ * q: row t, head h at q + t * q_token_stride + h * q_head_stride, multiples of 8 elements, d values in a row; out alike.  What is
+ * written overlaps nothing that is read, but out may be q with the same strides. */
+typedef struct trtamd_kv_cache_attention_params
+{
+    trtamd_kv_cache cache;
+    trtamd_half_t const* q;
+    trtamd_half_t* out;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int32_t q_heads;        /* a multiple of kv_heads */
+    float scale;            /* of the scores; finite and not negative */
+    int32_t window;         /* tokens that a row sees, itself the last of them; 0: all */
+    int32_t sinks;          /* 0 or more */
+    int32_t max_length;     /* about the longest of the lengths, by which work is shared out (longer ones are served as well); 0:
+                               as long as max_pages allows */
+    void* workspace;        /* 16-byte aligned; calls that may overlap need one each */
+    size_t workspace_bytes; /* trtamd_kv_cache_attention_workspace_size(params) or more */
+} trtamd_kv_cache_attention_params;
+
+/* Of the parameters' sizes alone: no pointer is looked at.  0: none is needed, or the sizes are refused. */
+TRTAMD_API size_t trtamd_kv_cache_attention_workspace_size(trtamd_kv_cache_attention_params const* params);
+TRTAMD_API int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache_attention_params const* params);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention in windows, over packed sequences in FP16: row i of a sequence sees the rows i - left .. i + right and the first `sinks`
+ * rows, of them none behind i + right; left or right -1: all on that side (right = 0: causal).
+ *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j)
+ * Sums, maxima and exponentials are binary32, the weights of the second product rounded to binary16 once, half to even.  Rows that
+ * are not seen do not take part whatever they hold, infinities and NaNs included (a NaN or an infinity anywhere near makes the
+ * rows around it slow).  A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
+ * max_tokens-th on, are left out: neither read nor written.  Row t, head h of q at q + t * q_token_stride + h * q_head_stride, d
+ * values in a row, multiples of 8 elements; k, v and out alike: the attention plugins' packing ([token][head][q|k|v][d]) as well
+ * as tensors of their own.  What is written overlaps nothing that is read.  No counterpart in the reference's plugins.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct trtamd_window_attention_params
+{
+    trtamd_half_t const* q;
+    trtamd_half_t const* k;
+    trtamd_half_t const* v;
+    trtamd_half_t* out;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int32_t const* cu_seqlens; /* [B + 1] */
+    int32_t B;                 /* sequences, at most 65535 */
+    int32_t T;                 /* rows of the tensors */
+    int32_t max_tokens;        /* of a sequence, or more */
+    int32_t q_heads;           /* a multiple of kv_heads */
+    int32_t kv_heads;
+    int32_t d;                 /* a multiple of 8, at most 256 */
+    float scale;               /* finite and not negative */
+    int32_t left, right;       /* -1 or more */
+    int32_t sinks;             /* 0 or more */
+} trtamd_window_attention_params;
+
+TRTAMD_API int trtamd_window_attention(trtamd_stream_t stream, trtamd_window_attention_params const* params);
+
+/* ------------------------------------------------------------------------------------------
  * Reformats either side of the interleaved plugins.  TensorRT inserts these itself when a plugin asks
  * for TensorFormat::kCHW32 (include/NvInferRuntime.h:1471; the INT8 interleaved plugins do:
  * plugin/bertQKVToContextPlugin/qkvToContextInt8InterleavedPlugin.cpp:124-127,

@@ -81,6 +81,47 @@ class QkNormRotaryParams(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """struct trtamd_kv_cache (include/trtamd_encoder_ops.h), as are the four that follow."""
+    _fields_ = [
+        ("k", c_p), ("v", c_p), ("k_scale", c_p), ("v_scale", c_p),
+        ("page_table", c_p), ("lengths", c_p), ("cu_seqlens", c_p),
+        ("data_type", i32), ("pages", i32), ("page_tokens", i32), ("kv_heads", i32), ("d", i32),
+        ("B", i32), ("max_pages", i32), ("max_tokens", i32), ("T", i32),
+    ]
+
+
+class KvCacheWriteParams(C.Structure):
+    _fields_ = [
+        ("cache", KvCache), ("k", c_p), ("v", c_p),
+        ("k_token_stride", i64), ("k_head_stride", i64), ("v_token_stride", i64), ("v_head_stride", i64),
+    ]
+
+
+class KvCacheReadParams(C.Structure):
+    _fields_ = KvCacheWriteParams._fields_
+
+
+class KvCacheAttentionParams(C.Structure):
+    _fields_ = [
+        ("cache", KvCache), ("q", c_p), ("out", c_p),
+        ("q_token_stride", i64), ("q_head_stride", i64), ("out_token_stride", i64), ("out_head_stride", i64),
+        ("q_heads", i32), ("scale", f32), ("window", i32), ("sinks", i32), ("max_length", i32),
+        ("workspace", c_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class WindowAttentionParams(C.Structure):
+    _fields_ = [
+        ("q", c_p), ("k", c_p), ("v", c_p), ("out", c_p),
+        ("q_token_stride", i64), ("q_head_stride", i64), ("k_token_stride", i64), ("k_head_stride", i64),
+        ("v_token_stride", i64), ("v_head_stride", i64), ("out_token_stride", i64), ("out_head_stride", i64),
+        ("cu_seqlens", c_p), ("B", i32), ("T", i32), ("max_tokens", i32),
+        ("q_heads", i32), ("kv_heads", i32), ("d", i32), ("scale", f32), ("left", i32), ("right", i32), ("sinks", i32),
+    ]
+
+
+KV_CACHE_INT8, KV_CACHE_FP8 = 2, 6
 QK_NORM_NONE, QK_NORM_RMS, QK_NORM_LAYER = 0, 1, 2
 LINEAR_AFFINE, LINEAR_GELU, LINEAR_RAW_INT32, LINEAR_AFFINE_FP16 = 0, 1, 2, 3
 UNFUSED_ROUTE_ONE_LAUNCH, UNFUSED_ROUTE_THREE_LAUNCHES, UNFUSED_ROUTE_BY_SHAPE = 0, 1, 99
@@ -186,6 +227,11 @@ _SIGS = {
     "trtamd_int8_dynamic_linear_workspace_size": (C.c_size_t, [i32, i32, i32]),
     "trtamd_int8_dynamic_linear": (C.c_int, [c_p, C.POINTER(Int8DynamicLinearParams)]),
     "trtamd_qk_norm_rotary": (C.c_int, [c_p, i32, C.POINTER(QkNormRotaryParams)]),
+    "trtamd_kv_cache_write": (C.c_int, [c_p, C.POINTER(KvCacheWriteParams)]),
+    "trtamd_kv_cache_read": (C.c_int, [c_p, C.POINTER(KvCacheReadParams)]),
+    "trtamd_kv_cache_attention_workspace_size": (C.c_size_t, [C.POINTER(KvCacheAttentionParams)]),
+    "trtamd_kv_cache_attention": (C.c_int, [c_p, C.POINTER(KvCacheAttentionParams)]),
+    "trtamd_window_attention": (C.c_int, [c_p, C.POINTER(WindowAttentionParams)]),
     "trtamd_encoder_create": (c_p, [C.POINTER(EncoderConfig)]),
     "trtamd_encoder_destroy": (None, [c_p]),
     "trtamd_encoder_set_embedding": (C.c_int, [c_p, C.POINTER(EncoderEmbedding)]),
@@ -211,7 +257,9 @@ TEST_HOOK_SYMBOLS = ["trtamd_fused_mha_run_debug", "trtamd_test_set_tuning", "tr
 ENCODER_OPS_SYMBOLS = ["trtamd_int8_linear", "trtamd_fp16_linear", "trtamd_int8_linear_to_interleaved", "trtamd_int8_interleaved_to_linear",
                        "trtamd_quantize_fp16_to_interleaved", "trtamd_dequantize_interleaved_to_fp16",
                        "trtamd_quantize_fp16_per_token", "trtamd_int8_token_linear",
-                       "trtamd_int8_dynamic_linear_workspace_size", "trtamd_int8_dynamic_linear", "trtamd_qk_norm_rotary"]
+                       "trtamd_int8_dynamic_linear_workspace_size", "trtamd_int8_dynamic_linear", "trtamd_qk_norm_rotary",
+                       "trtamd_kv_cache_write", "trtamd_kv_cache_read", "trtamd_kv_cache_attention_workspace_size",
+                       "trtamd_kv_cache_attention", "trtamd_window_attention"]
 # Entry points declared in include/trtamd_encoder_runtime.h.
 ENCODER_RUNTIME_SYMBOLS = ["trtamd_encoder_create", "trtamd_encoder_destroy", "trtamd_encoder_set_embedding",
                            "trtamd_encoder_set_layer", "trtamd_encoder_workspace_size", "trtamd_encoder_enqueue",

@@ -1,0 +1,134 @@
+// What the attention kernels over a cache and in windows share: 32 rows of queries a wavefront, keys in chunks of 64 of which each
+// half of the wavefront owns 16 consecutive ones twice, and a softmax kept up from chunk to chunk.
+//
+// S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_f16. Row 8 b + 4 a + c of a block of 32 keys is key 16 a + 4 b + c, so that
+// a lane of half a = lane / 32 gets the scores of keys 16 a .. 16 a + 15 of its query lane % 32, in order, and eight of them side by
+// side are the second product's operand as they are: nothing moves between lanes but a row's maximum.
+#pragma once
+
+#include "device_utils.hpp"
+
+namespace trtamd
+{
+
+constexpr int kChunkKeys = 64;
+constexpr float kNothingSeen = 3.402823466e+38f; // minus the maximum of no scores, finite
+
+// The key of a block of 32 that LDS row m of the block holds, and the row that holds key k.
+__device__ inline int key_of_row(int m)
+{
+    return 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3);
+}
+
+__device__ inline int row_of_key(int k)
+{
+    return 8 * ((k >> 2) & 3) + 4 * (k >> 4) + (k & 3);
+}
+
+// Which keys a row sees: those below sinks and from lo on, all below hi.
+struct Seen
+{
+    int lo, hi, sinks;
+    __device__ bool operator()(int key) const
+    {
+        return key < hi && (key >= lo || key < sinks);
+    }
+};
+
+// The chunks that any of some rows sees: `sinkChunks` from 0 on, then those from `first` on.
+struct Chunks
+{
+    int sinkChunks, first, total;
+    __device__ int key0(int i) const
+    {
+        return (i < sinkChunks ? i : first + i - sinkChunks) * kChunkKeys;
+    }
+};
+
+// lo: the lowest of the rows' lo, hi: the highest of their hi.
+__device__ inline Chunks chunks_of(int lo, int hi, int sinks)
+{
+    Chunks c;
+    int const sink = max(min(min(sinks, lo), hi), 0);
+    c.sinkChunks = (sink + kChunkKeys - 1) / kChunkKeys;
+    c.first = max(c.sinkChunks, lo / kChunkKeys);
+    int const last = hi > lo ? (int) (((int64_t) hi + kChunkKeys - 1) / kChunkKeys) : 0;
+    c.total = c.sinkChunks + max(last - c.first, 0);
+    return c;
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// 16-byte chunk `chunk` of LDS row `row` lies at this place of the row: eight rows side by side then fill all banks.
+__device__ inline int swizzled(int row, int chunk)
+{
+    return chunk ^ (row & 7);
+}
+
+// A wavefront's 32 rows: DV blocks of 32 of the head's values.
+template <int DV>
+struct RowSums
+{
+    f32x16 out[DV]; // O^T: elements 32 d + 8 (v / 4) + 4 h + v % 4 of query lane % 32
+    float negMax;   // minus the maximum that the weights are relative to, in powers of 2
+    float sum;      // of this lane's keys
+
+    __device__ void clear()
+    {
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+        {
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+            {
+                out[d][v] = 0.f;
+            }
+        }
+        negMax = kNothingSeen;
+        sum = 0.f;
+    }
+
+    // Brings the sums so far to a new maximum where it passes the old one by more than 2^8, which weights in binary16 hold; mx: of
+    // this chunk's scores, of both halves.
+    __device__ void move(float mx)
+    {
+        float const negNew = fminf(-mx, kNothingSeen);
+        if (__ballot(negNew < negMax - 8.f) != 0)
+        {
+            float const to = fminf(negNew, negMax);
+            float const f = __builtin_amdgcn_exp2f(to - negMax);
+#pragma unroll
+            for (int d = 0; d < DV; ++d)
+            {
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                {
+                    out[d][v] *= f;
+                }
+            }
+            sum *= f;
+            negMax = to;
+        }
+    }
+};
+
+__device__ inline float max_of(float a, float b)
+{
+    return fmaxf(a, b);
+}
+
+// Eight weights as the second product's operand, rounded half to even, in pairs (one instruction).
+__device__ inline f16x8 weights_f16(float const (&p)[8])
+{
+    f16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+    {
+        f16x2 const pair = __builtin_convertvector(f32x2{p[j], p[j + 1]}, f16x2);
+        r[j] = pair[0];
+        r[j + 1] = pair[1];
+    }
+    return r;
+}
+
+} // namespace trtamd
