@@ -8,6 +8,8 @@
 
 #include "device_utils.hpp"
 
+#include <type_traits>
+
 namespace trtamd
 {
 
@@ -115,6 +117,55 @@ struct RowSums
 __device__ inline float max_of(float a, float b)
 {
     return fmaxf(a, b);
+}
+
+// Steps of 16 values that a head is rounded up to, one of the numbers that kernels are built for.
+inline int head_steps(int d)
+{
+    int const s = (d + 15) / 16;
+    return s <= 2 ? 2 : s <= 4 ? 4 : s <= 6 ? s : s <= 8 ? 8 : 16;
+}
+
+// Values of a head in LDS, rows of 128 bytes or a multiple.
+constexpr int padded_head(int steps)
+{
+    return steps <= 4 ? 64 : steps <= 8 ? 128 : 256;
+}
+
+// Calls f with the number of steps as a constant.
+template <typename F>
+int by_head(int d, F&& f)
+{
+    switch (head_steps(d))
+    {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 5: return f(std::integral_constant<int, 5>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    default: return f(std::integral_constant<int, 16>{});
+    }
+}
+
+// Scores of keys that a row does not see become -infinity; keys key0 + 16 half + v % 16 + 32 (v / 16) in s[v / 16][v % 16].
+__device__ inline void hide(f32x16 (&s)[2], Seen const& seen, int key0)
+{
+    // behind the sinks one unsigned comparison has both ends
+    uint32_t const from = (uint32_t) (key0 - seen.lo), width = (uint32_t) max(seen.hi - seen.lo, 0);
+    if (key0 >= seen.sinks)
+    {
+#pragma unroll
+        for (int v = 0; v < 32; ++v)
+        {
+            s[v >> 4][v & 15] = from + (uint32_t) (32 * (v >> 4) + (v & 15)) < width ? s[v >> 4][v & 15] : -__builtin_inff();
+        }
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < 32; ++v)
+    {
+        s[v >> 4][v & 15] = seen(key0 + 32 * (v >> 4) + (v & 15)) ? s[v >> 4][v & 15] : -__builtin_inff();
+    }
 }
 
 // Eight weights as the second product's operand, rounded half to even, in pairs (one instruction).

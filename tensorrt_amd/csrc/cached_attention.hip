@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace trtamd
 {
@@ -103,13 +104,14 @@ __device__ inline u32x4 bytes_below(int n)
 // values. 16 keys lie in one page, so a lane has one page for the keys and one for the values and the factors of a chunk.
 // The wavefronts meet in LDS at the end, workgroups that share a row's keys in memory.
 // ------------------------------------------------------------------------------------------
-template <int DC /* 64 of the head's values */, bool FP8>
-__global__ __launch_bounds__(kThreads) void cached_few_kernel(CacheArgs const c, AttentionArgs const a)
+template <int KS /* 16 of the head's values */, bool FP8>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_few_kernel(
+    CacheArgs const c, AttentionArgs const a)
 {
-    constexpr int NT = 4 * DC;
+    constexpr int NT = KS, DC = (KS + 3) / 4;
     __shared__ f32x4 meet[2][NT][kWaveSize];
     __shared__ float stats[kWaves][2][kFewRows];
-    int const split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    int const h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
     CacheRows const r = cache_rows(c, b);
     int const group = a.group.d;
     if (r.n == 0 || (int64_t) r.n * group > a.fewLimit)
@@ -183,14 +185,11 @@ __global__ __launch_bounds__(kThreads) void cached_few_kernel(CacheArgs const c,
         size_t const scaleAt = (size_t) page * c.heads + h;
         kScale = c.kScale[scaleAt];
         vScale = c.vScale[scaleAt];
-        uint8_t const* const from = c.v + page_offset(c, page, h) + (uint32_t) m * P + (key & (P - 1));
+        uint8_t const* const from = c.v + page_offset(c, page, h) + m * P + (key & (P - 1));
 #pragma unroll
         for (int t = 0; t < NT; ++t)
         {
-            if (16 * t < c.d)
-            {
-                vr[t] = *reinterpret_cast<u32x4 const*>(from + 16 * t * P);
-            }
+            vr[t] = *reinterpret_cast<u32x4 const*>(from + (16 * t < c.d ? 16 * t * P : 0)); // elements behind the head's end are not written
         }
     };
 
@@ -242,10 +241,31 @@ __global__ __launch_bounds__(kThreads) void cached_few_kernel(CacheArgs const c,
 #pragma unroll
             for (int e = 0; e < 4; ++e)
             {
-                float const v = fmaf(s[t][e], f.score, f.log2Value);
-                s[t][e] = whole || (4 * t + e < there && seen(key0 + 16 * g + 4 * t + e)) ? v : -__builtin_inff();
-                mx = fmaxf(mx, s[t][e]);
+                s[t][e] = fmaf(s[t][e], f.score, f.log2Value);
             }
+        }
+        if (!whole)
+        {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+            {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    s[t][e] = 4 * t + e < there && seen(key0 + 16 * g + 4 * t + e) ? s[t][e] : -__builtin_inff();
+                }
+            }
+            u32x4 const keep = bytes_below(there);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+            {
+                vr[t] &= keep; // what was never written may be anything, and 0 times it not 0
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+        {
+            mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
         }
         mx = reduce_step<32>(reduce_step<16>(mx, max_of), max_of);
         float const negNew = fminf(-mx, kNothingSeen);
@@ -273,19 +293,11 @@ __global__ __launch_bounds__(kThreads) void cached_few_kernel(CacheArgs const c,
             }
             p[j] = weights_f16(w);
         }
-        u32x4 const keep = bytes_below(there);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
         {
-            if (16 * t < c.d)
-            {
-                if (!whole)
-                {
-                    vr[t] &= keep; // what was never written may be anything, and 0 times it not 0
-                }
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][0], vr[t][1]), p[0], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][2], vr[t][3]), p[1], o[t], 0, 0, 0);
-            }
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][0], vr[t][1]), p[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][2], vr[t][3]), p[1], o[t], 0, 0, 0);
         }
         if (more)
         {
@@ -396,19 +408,21 @@ struct ManyLds
     static constexpr int kTotal = 2 * (kSlot + kFactors);
 };
 
-template <int DP /* the head's values in LDS */, bool FP8>
-__global__ __launch_bounds__(kThreads) void cached_many_kernel(CacheArgs const c, AttentionArgs const a, FastDiv const splits)
+template <int KS /* 16 of the head's values */, bool FP8>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 8 ? 2 : 1))) void cached_many_kernel(
+    CacheArgs const c, AttentionArgs const a, FastDiv const heads)
 {
+    constexpr int DP = padded_head(KS);
     using Lds = ManyLds<DP>;
     constexpr int kPieces = DP / 16;                     // of 16 bytes in a key
     constexpr int NL = kChunkKeys * kPieces / kThreads;  // loads a thread of keys, and of values
-    constexpr int DV = DP / 32;
+    constexpr int DV = (KS + 1) / 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    int const h = blockIdx.y, b = blockIdx.z;
+    // tiles of a head are a multiple of the heads apart, so that where those divide by 8 they share an XCD's L2
+    int const fromEnd = (int) (blockIdx.x / heads), h = (int) (blockIdx.x - fromEnd * heads.d), b = blockIdx.y, split = blockIdx.z;
     CacheRows const r = cache_rows(c, b);
     int const group = a.group.d;
     int64_t const rows64 = (int64_t) r.n * group;
-    int const fromEnd = (int) (blockIdx.x / splits), split = (int) (blockIdx.x - fromEnd * splits.d);
     int64_t const tiles = (rows64 + kTileRows - 1) / kTileRows;
     if (rows64 <= a.fewLimit || fromEnd >= tiles)
     {
@@ -435,11 +449,11 @@ __global__ __launch_bounds__(kThreads) void cached_many_kernel(CacheArgs const c
     Seen const least = seen_by(r, (int) ((uint32_t) min(wRow, rowEnd - 1) / a.group), a);
     Seen const most = seen_by(r, (int) ((uint32_t) min(wRow + 31, rowEnd - 1) / a.group), a);
 
-    f16x8 q[DP / 16]; // row lq, elements 16 s + 8 half .. + 7
+    f16x8 q[KS]; // row lq, elements 16 s + 8 half .. + 7
     {
         uint8_t const* const from = a.q + 2 * ((int64_t) (r.row0 + token) * a.qToken + (int64_t) head * a.qHead);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        for (int s = 0; s < KS; ++s)
         {
             q[s] = f16x8{};
             if (16 * s < c.d)
@@ -559,31 +573,47 @@ __global__ __launch_bounds__(kThreads) void cached_many_kernel(CacheArgs const c
                     s[0][v] = s[1][v] = 0.f;
                 }
 #pragma unroll
-                for (int e = 0; e < DP / 16; ++e)
+                for (int e = 0; e < KS; ++e)
                 {
-                    if (16 * e < c.d)
-                    {
 #pragma unroll
-                        for (int t = 0; t < 2; ++t)
-                        {
-                            int const kRow = 32 * t + lq;
-                            f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRow * DP * 2 + 16 * swizzled(kRow, 2 * e + half));
-                            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
-                        }
+                    for (int t = 0; t < 2; ++t)
+                    {
+                        int const kRow = 32 * t + lq;
+                        f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRow * DP * 2 + 16 * swizzled(kRow, 2 * e + half));
+                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
                     }
                 }
                 bool const whole = sees_all(least, most, key0) && __ballot(there[0] < 16 || there[1] < 16) == 0;
-                float mx = -__builtin_inff();
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
                 {
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
                     {
-                        float const y = fmaf(s[t][v], f[t][0], f[t][1]);
-                        s[t][v] = whole || (v < there[t] && seen(key0 + 32 * t + 16 * half + v)) ? y : -__builtin_inff();
-                        mx = fmaxf(mx, s[t][v]);
+                        s[t][v] = fmaf(s[t][v], f[t][0], f[t][1]);
                     }
+                }
+                if (!whole)
+                {
+                    hide(s, seen, key0 + 16 * half);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                    {
+                        if (__ballot(there[t] < 16) != 0)
+                        {
+#pragma unroll
+                            for (int v = 0; v < 16; ++v)
+                            {
+                                s[t][v] = v < there[t] ? s[t][v] : -__builtin_inff();
+                            }
+                        }
+                    }
+                }
+                float mx = -__builtin_inff();
+#pragma unroll
+                for (int v = 0; v < 32; ++v)
+                {
+                    mx = fmaxf(mx, s[v >> 4][v & 15]);
                 }
                 sums.move(reduce_step<32>(mx, max_of));
 #pragma unroll
@@ -603,13 +633,10 @@ __global__ __launch_bounds__(kThreads) void cached_many_kernel(CacheArgs const c
 #pragma unroll
                         for (int d = 0; d < DV; ++d)
                         {
-                            if (32 * d < c.d)
-                            {
-                                int const vRow = 32 * d + lq;
-                                f16x8 const v = *reinterpret_cast<f16x8 const*>(
-                                    values + vRow * kChunkKeys * 2 + 16 * swizzled(vRow, 4 * t + 2 * half + w));
-                                sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, sums.out[d], 0, 0, 0);
-                            }
+                            int const vRow = 32 * d + lq;
+                            f16x8 const v = *reinterpret_cast<f16x8 const*>(
+                                values + vRow * kChunkKeys * 2 + 16 * swizzled(vRow, 4 * t + 2 * half + w));
+                            sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, sums.out[d], 0, 0, 0);
                         }
                     }
                 }
@@ -659,28 +686,34 @@ __global__ __launch_bounds__(kThreads) void cached_many_kernel(CacheArgs const c
 }
 
 // ------------------------------------------------------------------------------------------
-// The parts of a row's keys: a wavefront a row. Rows whose keys one workgroup had are written already.
+// The parts of a row's keys: a workgroup a row, L lanes on a part's values, 256 / L parts at a time. Rows whose keys one workgroup
+// had are written already.
 // ------------------------------------------------------------------------------------------
+template <int L>
 __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs const c, AttentionArgs const a, FastDiv const heads)
 {
+    constexpr int kGroups = kThreads / L;
+    __shared__ f32x4 meet[kGroups][L];
+    __shared__ float totals[kGroups];
     int const b = blockIdx.y, lane = threadIdx.x & 63;
     CacheRows const r = cache_rows(c, b);
     int const group = a.group.d;
     int64_t const rows = (int64_t) r.n * group;
-    int64_t const unit = (int64_t) blockIdx.x * kWaves + (threadIdx.x >> 6); // token, query head
+    int const unit = blockIdx.x; // token, query head
     if (unit >= (int64_t) r.n * a.qHeads)
     {
         return;
     }
-    int const token = (int) ((uint32_t) unit / heads), head = (int) (unit - (int64_t) token * heads.d);
+    int const token = (int) ((uint32_t) unit / heads), head = unit - token * (int) heads.d;
     bool const few = rows <= a.fewLimit;
     int const span = few ? a.fewSpan : a.manySpan;
     int i0 = 0, i1 = r.n - 1;
     if (!few)
     {
-        int const row0 = (token * group + head % group) / kTileRows * kTileRows;
-        i0 = row0 / group;
-        i1 = (int) (min((int64_t) row0 + kTileRows, rows) - 1) / group;
+        int const own = head - (int) ((uint32_t) head / a.group) * group;
+        int const row0 = (token * group + own) / kTileRows * kTileRows;
+        i0 = (int) ((uint32_t) row0 / a.group);
+        i1 = (int) ((uint32_t) (min((int64_t) row0 + kTileRows, rows) - 1) / a.group);
     }
     int const used = (chunks_of_tokens(r, i0, i1, a).total + span - 1) / span;
     if (used <= 1)
@@ -695,24 +728,41 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs const c
         least = fminf(least, a.stats[2 * (slot + s)]);
     }
     least = group_allreduce<kWaveSize>(least, [](float x, float y) { return fminf(x, y); });
+    int const part = threadIdx.x / L, e = 4 * (threadIdx.x & (L - 1));
     float total = 0.f;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < used; ++s)
+    if (e < c.d)
     {
-        f32x2 const st = *reinterpret_cast<f32x2 const*>(a.stats + 2 * (slot + s));
-        float const by = __builtin_amdgcn_exp2f(least - st[0]);
-        total = fmaf(st[1], by, total);
-        if (4 * lane < c.d)
+#pragma unroll 4
+        for (int s = part; s < used; s += kGroups)
         {
-            y += *reinterpret_cast<f32x4 const*>(a.partial + (slot + s) * c.d + 4 * lane) * by;
+            f32x2 const st = *reinterpret_cast<f32x2 const*>(a.stats + 2 * (slot + s));
+            float const by = __builtin_amdgcn_exp2f(least - st[0]);
+            total = fmaf(st[1], by, total);
+            y += *reinterpret_cast<f32x4 const*>(a.partial + (slot + s) * c.d + e) * by;
         }
     }
-    float const inverse = total == 0.f ? 0.f : 1.f / total;
-    if (4 * lane < c.d)
+    meet[part][threadIdx.x & (L - 1)] = y;
+    if (e == 0)
     {
-        *reinterpret_cast<f16x4*>(a.out + 2 * (outRow * a.outToken + (int64_t) head * a.outHead + 4 * lane))
-            = f16x4{(f16) (y[0] * inverse), (f16) (y[1] * inverse), (f16) (y[2] * inverse), (f16) (y[3] * inverse)};
+        totals[part] = total;
     }
+    __syncthreads();
+    if (threadIdx.x >= L || e >= c.d)
+    {
+        return;
+    }
+    total = totals[0];
+    y = meet[0][threadIdx.x];
+#pragma unroll
+    for (int p = 1; p < kGroups; ++p)
+    {
+        total += totals[p];
+        y += meet[p][threadIdx.x];
+    }
+    float const inverse = total == 0.f ? 0.f : 1.f / total;
+    *reinterpret_cast<f16x4*>(a.out + 2 * (outRow * a.outToken + (int64_t) head * a.outHead + e))
+        = f16x4{(f16) (y[0] * inverse), (f16) (y[1] * inverse), (f16) (y[2] * inverse), (f16) (y[3] * inverse)};
 }
 
 // ------------------------------------------------------------------------------------------
@@ -731,13 +781,12 @@ struct Plan
     }
 };
 
-// Chunks a part takes, so that `units` units of `chunks` chunks each make about `target` workgroups, and how many parts that are.
-void share_out(int64_t units, int64_t chunks, int64_t target, int64_t least, int64_t most, int& span, int& splits)
+// Chunks of `most` that a part takes, and how many parts that are at most.
+void share_out(int64_t chunksAPart, int64_t most, int& span, int& splits)
 {
-    int64_t const parts = std::max<int64_t>(1, std::min(ceil_div(target, std::max<int64_t>(units, 1)), ceil_div(chunks, least)));
-    int64_t const s = std::max(ceil_div(chunks, parts), ceil_div(most, (int64_t) 65535));
+    int64_t const s = std::max(chunksAPart, ceil_div(most, (int64_t) 65535)); // a launch's third extent
     span = (int) s;
-    splits = (int) ceil_div(most, s); // of the longest that may come
+    splits = (int) ceil_div(most, s);
 }
 
 Plan plan_of(trtamd_kv_cache_attention_params const& p)
@@ -758,9 +807,15 @@ Plan plan_of(trtamd_kv_cache_attention_params const& p)
     };
     int64_t const most = ceil_div(seen(capacity), (int64_t) kChunkKeys) + 2;
     int64_t const chunks = ceil_div(seen(p.max_length > 0 ? std::min<int64_t>(p.max_length, capacity) : capacity), (int64_t) kChunkKeys) + (p.window ? 1 : 0);
-    int64_t const cus = num_cus();
-    share_out((int64_t) c.B * c.kv_heads, chunks, 4 * cus, 4, most, plan.fewSpan, plan.fewSplits);
-    share_out(std::max<int64_t>(ceil_div((int64_t) c.T * group, (int64_t) kTileRows), 1) * c.kv_heads, chunks, 2 * cus, 8, most, plan.manySpan, plan.manySplits);
+    int64_t const cus = num_cus(), head = head_steps(c.d);
+    // Few rows: one generation of workgroups, and where there are several sequences, whose lengths differ, parts of no more than 16
+    // chunks. Four chunks are one a wavefront.
+    int64_t const resident = cus * (head <= 4 ? 3 : head <= 8 ? 2 : 1);
+    int64_t const even = ceil_div((int64_t) c.B * c.kv_heads * chunks, resident);
+    share_out(std::max<int64_t>(c.B > 1 ? std::min<int64_t>(even, 16) : even, 4), most, plan.fewSpan, plan.fewSplits);
+    // More rows: whole where there are tiles enough for two a CU.
+    int64_t const tiles = ceil_div((int64_t) c.T * group, (int64_t) kTileRows) * c.kv_heads;
+    share_out(tiles >= 2 * cus ? most : std::max<int64_t>(ceil_div(tiles * chunks, 2 * cus), 8), most, plan.manySpan, plan.manySplits);
     return plan;
 }
 
@@ -788,9 +843,9 @@ int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: window=%d sinks=%d max_length=%d", what, p.window, p.sinks, p.max_length);
     }
-    if ((int64_t) p.cache.T * p.q_heads >= (int64_t) 1 << 31)
+    if ((int64_t) p.cache.T * p.q_heads >= (int64_t) 1 << 30) // a launch has 2^32 threads
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: T * q_heads of 2^31 or more", what);
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: T * q_heads of 2^30 or more", what);
     }
     return TRTAMD_STATUS_SUCCESS;
 }
@@ -800,20 +855,20 @@ bool nothing(trtamd_kv_cache const& c)
     return c.B == 0 || c.T == 0 || c.max_tokens == 0;
 }
 
-template <int DP, bool FP8>
-int launch_many(hipStream_t stream, dim3 grid, CacheArgs const& c, AttentionArgs const& a, FastDiv const& splits)
+template <int KS, bool FP8>
+int launch_many(hipStream_t stream, dim3 grid, CacheArgs const& c, AttentionArgs const& a, FastDiv const& heads)
 {
-    constexpr int kBytes = ManyLds<DP>::kTotal;
+    constexpr int kBytes = ManyLds<padded_head(KS)>::kTotal;
     if constexpr (kBytes > 65536)
     {
-        static hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(cached_many_kernel<DP, FP8>),
+        static hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(cached_many_kernel<KS, FP8>),
             hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
         if (e != hipSuccess)
         {
             return set_error(TRTAMD_STATUS_FAILURE, "kv_cache_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
         }
     }
-    hipLaunchKernelGGL((cached_many_kernel<DP, FP8>), grid, dim3(kThreads), kBytes, stream, c, a, splits);
+    hipLaunchKernelGGL((cached_many_kernel<KS, FP8>), grid, dim3(kThreads), kBytes, stream, c, a, heads);
     return check_launch("cached_many_kernel");
 }
 
@@ -825,14 +880,11 @@ int launch(hipStream_t stream, trtamd_kv_cache_attention_params const& p, Plan c
     int const group = p.q_heads / k.kv_heads;
     if (plan.few)
     {
-        dim3 const grid((unsigned) plan.fewSplits, (unsigned) k.kv_heads, (unsigned) k.B);
-        auto const run = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, c, a);
+        dim3 const grid((unsigned) k.kv_heads, (unsigned) k.B, (unsigned) plan.fewSplits);
+        int const st = by_head(k.d, [&](auto steps) {
+            hipLaunchKernelGGL((cached_few_kernel<decltype(steps)::value, FP8>), grid, dim3(kThreads), 0, stream, c, a);
             return check_launch("cached_few_kernel");
-        };
-        int const st = k.d <= 64 ? run(cached_few_kernel<1, FP8>)
-            : k.d <= 128         ? run(cached_few_kernel<2, FP8>)
-                                 : run(cached_few_kernel<4, FP8>);
+        });
         if (st)
         {
             return st;
@@ -841,15 +893,9 @@ int launch(hipStream_t stream, trtamd_kv_cache_attention_params const& p, Plan c
     if (plan.many)
     {
         int64_t const tiles = ceil_div((int64_t) std::min(k.max_tokens, k.T) * group, (int64_t) kTileRows);
-        if (tiles * plan.manySplits >= 1 << 24)
-        {
-            return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "kv_cache_attention: %lld tiles of rows in %d parts", (long long) tiles, plan.manySplits);
-        }
-        dim3 const grid((unsigned) (tiles * plan.manySplits), (unsigned) k.kv_heads, (unsigned) k.B);
-        FastDiv const splits = fast_div((uint32_t) plan.manySplits);
-        int const st = k.d <= 64 ? launch_many<64, FP8>(stream, grid, c, a, splits)
-            : k.d <= 128         ? launch_many<128, FP8>(stream, grid, c, a, splits)
-                                 : launch_many<256, FP8>(stream, grid, c, a, splits);
+        dim3 const grid((unsigned) (tiles * k.kv_heads), (unsigned) k.B, (unsigned) plan.manySplits);
+        FastDiv const heads = fast_div((uint32_t) k.kv_heads);
+        int const st = by_head(k.d, [&](auto steps) { return launch_many<decltype(steps)::value, FP8>(stream, grid, c, a, heads); });
         if (st)
         {
             return st;
@@ -859,8 +905,10 @@ int launch(hipStream_t stream, trtamd_kv_cache_attention_params const& p, Plan c
     {
         // where only sequences of few rows are shared between workgroups, theirs alone
         int64_t const tokens = plan.many && plan.manySplits > 1 ? std::min(k.max_tokens, k.T) : std::min(std::min(k.max_tokens, k.T), kFewRows / group);
-        dim3 const grid((unsigned) ceil_div(tokens * p.q_heads, (int64_t) kWaves), (unsigned) k.B);
-        hipLaunchKernelGGL(cached_join_kernel, grid, dim3(kThreads), 0, stream, c, a, fast_div((uint32_t) p.q_heads));
+        dim3 const grid((unsigned) (tokens * p.q_heads), (unsigned) k.B);
+        FastDiv const heads = fast_div((uint32_t) p.q_heads);
+        auto const run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, c, a, heads); };
+        k.d <= 64 ? run(cached_join_kernel<16>) : k.d <= 128 ? run(cached_join_kernel<32>) : run(cached_join_kernel<64>);
         return check_launch("cached_join_kernel");
     }
     return TRTAMD_STATUS_SUCCESS;

@@ -385,6 +385,10 @@ int cache_check(char const* what, trtamd_kv_cache const& c)
     {
         return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d kv_heads=%d (at most 65535 and 32767)", what, c.B, c.kv_heads);
     }
+    if ((int64_t) c.pages * c.kv_heads >= (int64_t) 1 << 31)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: pages * kv_heads of 2^31 or more", what);
+    }
     for (void const* p : {(void const*) c.k, (void const*) c.v, (void const*) c.k_scale, (void const*) c.v_scale,
              (void const*) c.page_table, (void const*) c.lengths, (void const*) c.cu_seqlens})
     {

@@ -54,10 +54,10 @@ __device__ inline uint32_t page_bytes(CacheArgs const& c)
     return (uint32_t) c.d << c.shift;
 }
 
-// Where head h of a page begins.
-__device__ inline size_t page_offset(CacheArgs const& c, int page, int h)
+// Where head h of a page begins; pages * heads is less than 2^32.
+__device__ inline uint64_t page_offset(CacheArgs const& c, int page, int h)
 {
-    return ((size_t) (uint32_t) page * c.heads + h) * page_bytes(c);
+    return (uint64_t) ((uint32_t) page * (uint32_t) c.heads + (uint32_t) h) * page_bytes(c);
 }
 
 // ---- bytes to binary16, exactly: every INT8 and every E4M3 value is one -----------------------------------------------

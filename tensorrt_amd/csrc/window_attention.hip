@@ -41,6 +41,7 @@ struct WindowArgs
     int32_t T, maxTokens, d;
     int32_t left, right, sinks; // beyond any length where there is no limit
     float scale;                // in powers of 2
+    bool near;                  // whole chunks lie within 32-bit offsets, and heads fill their rows in LDS
     FastDiv group, kvHeads;
 };
 
@@ -103,11 +104,13 @@ __device__ void one_row(WindowArgs const& a, int first, int token, int head, int
     }
 }
 
-template <int DP /* the head's values in LDS */>
-__global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs const a)
+template <int KS /* 16 of the head's values */>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void window_attention_kernel(
+    WindowArgs const a)
 {
+    constexpr int DP = padded_head(KS);
     using Lds = WindowLds<DP>;
-    constexpr int kRow = Lds::kRow, DV = DP / 32;
+    constexpr int kRow = Lds::kRow, DV = (KS + 1) / 2;
     constexpr int kChunks = DP / 8;              // of 16 bytes in a row
     constexpr int kRowsPerLoad = 64 / kChunks;   // of a wavefront's load into LDS
     constexpr int NL = kChunkKeys / kRowsPerLoad / kWaves;
@@ -137,11 +140,11 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
     int const token = (int) ((uint32_t) row / a.group), head = h * group + row - token * group;
     Seen const seen = seen_by(row), least = seen_by(min(wRow, rowEnd - 1)), most = seen_by(min(wRow + 31, rowEnd - 1));
 
-    f16x8 q[DP / 16]; // row lq, elements 16 s + 8 half .. + 7
+    f16x8 q[KS]; // row lq, elements 16 s + 8 half .. + 7
     {
         uint8_t const* const from = a.q.p + (int64_t) (first + token) * a.q.token + (int64_t) head * a.q.head;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        for (int s = 0; s < KS; ++s)
         {
             q[s] = f16x8{};
             if (16 * s + 8 * half < a.d)
@@ -153,9 +156,31 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
 
     uint32_t const ldsBase = (uint32_t) (size_t) (lds_u8*) lds;
     int const rowInLoad = lane / kChunks, place = lane & (kChunks - 1);
+    // where this lane's pieces of a whole chunk lie from its first row on
+    uint32_t kAt[NL], vAt[NL];
+#pragma unroll
+    for (int l = 0; l < NL; ++l)
+    {
+        int const r = (l * kWaves + wave) * kRowsPerLoad + rowInLoad, chunk = swizzled(r, place);
+        kAt[l] = (uint32_t) ((r & 32) + key_of_row(r & 31)) * (uint32_t) a.k.token + 16u * (uint32_t) chunk;
+        vAt[l] = (uint32_t) r * (uint32_t) a.v.token + 16u * (uint32_t) chunk;
+    }
+    uint8_t const* const kUnit = a.k.p + (int64_t) first * a.k.token + (int64_t) h * a.k.head;
+    uint8_t const* const vUnit = a.v.p + (int64_t) first * a.v.token + (int64_t) h * a.v.head;
     auto request = [&](int i, int slot) {
         int const key0 = chunks.key0(i);
         uint32_t const to = ldsBase + (uint32_t) (2 * slot * Lds::kMatrix);
+        if (a.near && key0 + kChunkKeys <= n)
+        {
+#pragma unroll
+            for (int l = 0; l < NL; ++l)
+            {
+                uint32_t const at = to + (uint32_t) ((l * kWaves + wave) * kRowsPerLoad * kRow);
+                load_to_lds16_sbase(kUnit + (int64_t) key0 * a.k.token, kAt[l], at);
+                load_to_lds16_sbase(vUnit + (int64_t) key0 * a.v.token, vAt[l], at + (uint32_t) Lds::kMatrix);
+            }
+            return;
+        }
 #pragma unroll
         for (int l = 0; l < NL; ++l)
         {
@@ -163,9 +188,9 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
             int const chunk = swizzled(r, place); // its own inverse
             bool const inHead = 8 * chunk < a.d;
             int const kKey = min(key0 + (r & 32) + key_of_row(r & 31), n - 1), vKey = key0 + r;
-            uint8_t const* const k = a.k.p + (int64_t) (first + kKey) * a.k.token + (int64_t) h * a.k.head + 16 * chunk;
+            uint8_t const* const k = kUnit + (int64_t) kKey * a.k.token + 16 * chunk;
             // 0, the weight of a key behind the sequence, times an infinite value would not be 0
-            uint8_t const* const v = a.v.p + (int64_t) (first + vKey) * a.v.token + (int64_t) h * a.v.head + 16 * chunk;
+            uint8_t const* const v = vUnit + (int64_t) vKey * a.v.token + 16 * chunk;
             uint8_t const* const zeros = reinterpret_cast<uint8_t const*>(kZeros);
             load_to_lds16(inHead ? k : zeros, to + (uint32_t) (r0 * kRow));
             load_to_lds16(inHead && vKey < n ? v : zeros, to + (uint32_t) (Lds::kMatrix + r0 * kRow));
@@ -202,27 +227,19 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
             s[0][v] = s[1][v] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < DP / 16; ++e)
+        for (int e = 0; e < KS; ++e)
         {
-            if (16 * e < a.d)
-            {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                {
-                    int const kRowAt = 32 * t + lq;
-                    f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRowAt * kRow + 16 * swizzled(kRowAt, 2 * e + half));
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
-                }
+            for (int t = 0; t < 2; ++t)
+            {
+                int const kRowAt = 32 * t + lq;
+                f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRowAt * kRow + 16 * swizzled(kRowAt, 2 * e + half));
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
             }
         }
         if (!(key0 + kChunkKeys <= least.hi && (key0 >= most.lo || key0 + kChunkKeys <= a.sinks)))
         {
-#pragma unroll
-            for (int v = 0; v < 32; ++v)
-            {
-                int const key = key0 + 32 * (v >> 4) + 16 * half + (v & 15);
-                s[v >> 4][v & 15] = seen(key) ? s[v >> 4][v & 15] : -__builtin_inff();
-            }
+            hide(s, seen, key0 + 16 * half);
         }
         float mx = -__builtin_inff();
 #pragma unroll
@@ -248,16 +265,13 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
 #pragma unroll
                 for (int d = 0; d < DV; ++d)
                 {
-                    if (32 * d < a.d)
-                    {
-                        int const r = 32 * t + 16 * half + 8 * w + tr;
-                        i16x4 const lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_i16x4*) (values + r * kRow + 16 * swizzled(r, 4 * d + trChunk) + trByte));
-                        i16x4 const hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_i16x4*) (values + (r + 4) * kRow + 16 * swizzled(r + 4, 4 * d + trChunk) + trByte));
-                        i16x8 const both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                        sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bits_as<f16x8>(both), weights, sums.out[d], 0, 0, 0);
-                    }
+                    int const r = 32 * t + 16 * half + 8 * w + tr;
+                    i16x4 const lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_i16x4*) (values + r * kRow + 16 * swizzled(r, 4 * d + trChunk) + trByte));
+                    i16x4 const hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_i16x4*) (values + (r + 4) * kRow + 16 * swizzled(r + 4, 4 * d + trChunk) + trByte));
+                    i16x8 const both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bits_as<f16x8>(both), weights, sums.out[d], 0, 0, 0);
                 }
             }
         }
@@ -309,20 +323,20 @@ __global__ __launch_bounds__(kThreads) void window_attention_kernel(WindowArgs c
     }
 }
 
-template <int DP>
+template <int KS>
 int launch(hipStream_t stream, dim3 grid, WindowArgs const& a)
 {
-    constexpr int kBytes = WindowLds<DP>::kTotal;
+    constexpr int kBytes = WindowLds<padded_head(KS)>::kTotal;
     if constexpr (kBytes > 65536)
     {
         static hipError_t const e = hipFuncSetAttribute(
-            reinterpret_cast<void const*>(window_attention_kernel<DP>), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+            reinterpret_cast<void const*>(window_attention_kernel<KS>), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
         if (e != hipSuccess)
         {
             return set_error(TRTAMD_STATUS_FAILURE, "window_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
         }
     }
-    hipLaunchKernelGGL(window_attention_kernel<DP>, grid, dim3(kThreads), kBytes, stream, a);
+    hipLaunchKernelGGL(window_attention_kernel<KS>, grid, dim3(kThreads), kBytes, stream, a);
     return check_launch("window_attention_kernel");
 }
 
@@ -419,6 +433,7 @@ extern "C" int trtamd_window_attention(trtamd_stream_t stream, trtamd_window_att
     a.group = fast_div((uint32_t) group);
     a.kvHeads = fast_div((uint32_t) p.kv_heads);
     int64_t const tiles = ceil_div((int64_t) std::min(p.max_tokens, p.T) * group, (int64_t) kTileRows);
+    a.near = p.d == padded_head(head_steps(p.d)) && std::max(a.k.token, a.v.token) < (int64_t) 1 << 25;
     dim3 const grid((unsigned) (tiles * p.kv_heads), 1, (unsigned) p.B);
-    return p.d <= 64 ? launch<64>(as_stream(stream), grid, a) : p.d <= 128 ? launch<128>(as_stream(stream), grid, a) : launch<256>(as_stream(stream), grid, a);
+    return by_head(p.d, [&](auto steps) { return launch<decltype(steps)::value>(as_stream(stream), grid, a); });
 }

@@ -59,7 +59,7 @@ def test_cache_refused_everywhere(api, change, word):
 
 @pytest.mark.parametrize("change,word", [
     (dict(rows_k=0), "null"), (dict(rows_v=0), "null"), (dict(rows_k=A + 2), "aligned"), (dict(rows_v=A + 8), "aligned"),
-    (dict(rows_k_token_stride=100), "strides"), (dict(rows_v_head_stride=-8), "strides"), (dict(kv_heads=32768), "32767")])
+    (dict(rows_k_token_stride=100), "strides"), (dict(rows_v_head_stride=-8), "strides"), (dict(kv_heads=32768), "32767"), (dict(pages=1 << 30), "2^31")])
 def test_copies_refuse(api, change, word):
     refused(api, api.kv_cache_write(None, copied(capi.KvCacheWriteParams, **change)), word)
     refused(api, api.kv_cache_read(None, copied(capi.KvCacheReadParams, **change)), word)
@@ -70,7 +70,7 @@ def test_copies_refuse(api, change, word):
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(window=-1), "window=-1"), (dict(sinks=-1), "sinks=-1"),
     (dict(max_length=-1), "max_length=-1"), (dict(q=0), "null"), (dict(out=0), "null"), (dict(q=A + 8), "aligned"),
     (dict(out=A + 2), "aligned"), (dict(q_token_stride=250), "strides"), (dict(out_head_stride=-64), "strides"),
-    (dict(T=1 << 30, q_heads=4), "2^31"),
+    (dict(T=1 << 28, q_heads=4), "2^30"),
     (dict(max_pages=1 << 12, max_length=0, workspace=0), "workspace"), (dict(max_pages=1 << 12, max_length=0, workspace=A + 8), "workspace"),
     (dict(max_pages=1 << 12, max_length=0, workspace_bytes=64), "workspace")])
 def test_attention_refuses(api, change, word):
