@@ -61,10 +61,19 @@ __device__ inline Chunks chunks_of(int lo, int hi, int sinks)
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
-// 16-byte chunk `chunk` of LDS row `row` lies at this place of the row: eight rows side by side then fill all banks.
+// Where the 16-byte chunk `chunk` of LDS row `row` lies in its row, ROW bytes long, a power of 2 from 128 on. The 64 banks are 256 bytes: 16
+// lanes that read the same chunk of 16 rows side by side then have them all (an operand's 16 bytes a lane).
+template <int ROW>
 __device__ inline int swizzled(int row, int chunk)
 {
-    return chunk ^ (row & 7);
+    return ROW == 128 ? chunk ^ ((row >> 1) & 7) : chunk ^ (row & 15);
+}
+
+// The same for transposing reads, whose 32 lanes read 64 bytes of four rows side by side.
+template <int ROW>
+__device__ inline int swizzled_turned(int row, int chunk)
+{
+    return ROW == 128 ? chunk ^ (2 * row & 4) : chunk ^ (4 * row & 12);
 }
 
 // A wavefront's 32 rows: DV blocks of 32 of the head's values.

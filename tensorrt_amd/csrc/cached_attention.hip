@@ -23,7 +23,7 @@ namespace trtamd
 namespace
 {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWaveSize;
+constexpr int kThreads = 256;
 constexpr int kFewRows = 16;
 constexpr int kTileRows = 128; // of cached_many_kernel
 
@@ -32,13 +32,16 @@ struct AttentionArgs
     uint8_t const* q; // FP16
     uint8_t* out;
     int64_t qToken, qHead, outToken, outHead; // elements
-    float* partial;   // [row][slot][d], the sums that parts of a row's keys have, and behind them [row][slot][2]
-    float* stats;
+    float* partial;   // [row][slot][d], the sums that parts of a row's keys have in cached_many_kernel
+    float* stats;     // [row][slot][2]: minus the maximum, sum of the weights
+    float* fewPartial; // [stretch][2][16][d]
+    float* fewStats;  // [stretch][2][16][2]
+    int32_t* fewHeads; // [B][key heads][2]: the first of a head's sums in fewPartial, and how many
     FastDiv group;    // query heads of a key head
     int32_t qHeads;
     int32_t window, sinks;
     int32_t slots;    // of a row in partial
-    int32_t fewSpan, manySpan; // chunks of 64 keys that a workgroup takes
+    int32_t manySpan; // chunks of 64 keys that a workgroup takes
     int32_t fewLimit; // sequences of up to so many rows are cached_few_kernel's
     float scale;      // in powers of 2
 };
@@ -101,41 +104,66 @@ __device__ inline u32x4 bytes_below(int n)
 // Up to 16 rows of a key head: v_mfma_f32_16x16x32_f16, S^T = K Q^T and O^T = V^T P^T again. Each wavefront takes chunks of 64 keys
 // on its own, from global memory to the operands' registers: lane (g, m) loads 16 bytes of the key 16 (m / 4) + 4 t + m % 4 for tile
 // t, so that its scores are those of the keys 16 g .. 16 g + 15 of row m, and 16 bytes of the same keys of element 16 i + m of the
-// values. 16 keys lie in one page, so a lane has one page for the keys and one for the values and the factors of a chunk.
-// The wavefronts meet in LDS at the end, workgroups that share a row's keys in memory.
+// values. 16 keys lie in one page, so a lane has one page for the keys and one for the values and the factors of a chunk. The next
+// chunk's keys are requested as soon as this one's are used, its values likewise: 16 KB a wavefront (heads of 128) are always on
+// their way.
 // ------------------------------------------------------------------------------------------
-template <int KS /* 16 of the head's values */, bool FP8>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_few_kernel(
-    CacheArgs const c, AttentionArgs const a)
-{
-    constexpr int NT = KS, DC = (KS + 3) / 4;
-    __shared__ f32x4 meet[2][NT][kWaveSize];
-    __shared__ float stats[kWaves][2][kFewRows];
-    int const h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
-    CacheRows const r = cache_rows(c, b);
-    int const group = a.group.d;
-    if (r.n == 0 || (int64_t) r.n * group > a.fewLimit)
-    {
-        return;
-    }
-    int const rows = r.n * group;
-    Chunks const chunks = chunks_of_tokens(r, 0, r.n - 1, a);
-    int const used = max((chunks.total + a.fewSpan - 1) / a.fewSpan, 1);
-    if (split >= used)
-    {
-        return;
-    }
-    int const cEnd = min(chunks.total, (split + 1) * a.fewSpan);
-    int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int const m = lane & 15, g = lane >> 4;
-    int const row = min(m, rows - 1);
-    int const token = (int) ((uint32_t) row / a.group), head = h * group + row - token * group;
-    Seen const seen = seen_by(r, token, a), least = seen_by(r, 0, a), most = seen_by(r, r.n - 1, a);
-    int const P = 1 << c.shift;
 
-    f16x8 q[DC][2];
+// A sequence and key head, the same for a wavefront.
+struct FewUnit
+{
+    CacheRows r;
+    Chunks chunks;
+    int b, h, rows;
+    // a row that sees nothing has a chunk all the same, which writes its zeros
+    __device__ int count() const
     {
-        uint8_t const* const from = a.q + 2 * ((int64_t) (r.row0 + token) * a.qToken + (int64_t) head * a.qHead);
+        return max(chunks.total, 1);
+    }
+};
+
+// Sequences that are not here (more rows, or none) have no rows.
+__device__ inline FewUnit few_unit(CacheArgs const& c, AttentionArgs const& a, int b, int h)
+{
+    FewUnit u;
+    u.b = b;
+    u.h = h;
+    u.r = cache_rows(c, b);
+    int64_t const rows = (int64_t) u.r.n * a.group.d;
+    u.rows = rows <= kFewRows ? (int) rows : 0;
+    u.chunks = chunks_of_tokens(u.r, 0, u.r.n - 1, a);
+    return u;
+}
+
+// Pages of a chunk: those of the lane's keys and of its values.
+struct FewPages
+{
+    int k, v;
+};
+
+template <int KS /* 16 of the head's values */, bool FP8>
+struct FewWave
+{
+    static constexpr int DC = (KS + 3) / 4;
+    f16x8 q[DC][2];
+    u32x4 kr[4][DC], vr[KS];
+    float kScale, vScale;
+    f32x4 o[KS];
+    float negMax, sum;
+    int m, g, token, head;
+    Seen seen, least, most;
+
+    __device__ void begin(CacheArgs const& c, AttentionArgs const& a, FewUnit const& u)
+    {
+        int const lane = threadIdx.x & 63, row = min(lane & 15, u.rows - 1), group = a.group.d;
+        m = lane & 15;
+        g = lane >> 4;
+        token = (int) ((uint32_t) row / a.group);
+        head = u.h * group + row - token * group;
+        seen = seen_by(u.r, token, a);
+        least = seen_by(u.r, 0, a);
+        most = seen_by(u.r, u.r.n - 1, a);
+        uint8_t const* const from = a.q + 2 * ((int64_t) (u.r.row0 + token) * a.qToken + (int64_t) head * a.qHead);
 #pragma unroll
         for (int k = 0; k < DC; ++k)
         {
@@ -150,24 +178,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                 }
             }
         }
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+        {
+            o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        negMax = kNothingSeen;
+        sum = 0.f;
     }
 
-    // pages of a chunk: those of the lane's keys and of its values
-    struct Pages
+    __device__ static FewPages pages_of(CacheArgs const& c, FewUnit const& u, int i)
     {
-        int k, v;
-    };
-    int32_t const* const table = c.table + (int64_t) b * c.maxPages;
-    auto pages_of = [&](int i) {
-        int const key0 = chunks.key0(i);
-        return Pages{table[min((key0 + 16 * (m >> 2)) >> c.shift, c.maxPages - 1)], table[min((key0 + 16 * g) >> c.shift, c.maxPages - 1)]};
-    };
-    u32x4 kr[4][DC], vr[NT];
-    float kScale, vScale;
-    auto load_keys = [&](int i, Pages const& p) {
-        int const key = chunks.key0(i) + 16 * (m >> 2) + (m & 3);
+        int const lane = threadIdx.x & 63, key0 = u.chunks.key0(i);
+        int32_t const* const table = c.table + (int64_t) u.b * c.maxPages;
+        return {table[min((key0 + 4 * (lane & 12)) >> c.shift, c.maxPages - 1)], table[min((key0 + 16 * (lane >> 4)) >> c.shift, c.maxPages - 1)]};
+    }
+
+    __device__ void load_keys(CacheArgs const& c, FewUnit const& u, int i, FewPages const& p)
+    {
+        int const lane = threadIdx.x & 63, key = u.chunks.key0(i) + 4 * (lane & 12) + (lane & 3), P = 1 << c.shift;
         int const page = (uint32_t) p.k < (uint32_t) c.pages ? p.k : 0;
-        uint8_t const* const from = c.k + page_offset(c, page, h) + (uint32_t) (key & (P - 1)) * c.d;
+        uint8_t const* const from = c.k + page_offset(c, page, u.h) + (uint32_t) (key & (P - 1)) * c.d;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
         {
@@ -175,43 +206,31 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
             for (int k = 0; k < DC; ++k)
             {
                 // lanes behind the head's end read its last values, times a query of zeros
-                kr[t][k] = *reinterpret_cast<u32x4 const*>(from + 4 * t * c.d + min(64 * k + 16 * g, c.d - 16));
+                kr[t][k] = *reinterpret_cast<u32x4 const*>(from + 4 * t * c.d + min(64 * k + 16 * (lane >> 4), c.d - 16));
             }
         }
-    };
-    auto load_values = [&](int i, Pages const& p) {
-        int const key = chunks.key0(i) + 16 * g;
+    }
+
+    __device__ void load_values(CacheArgs const& c, FewUnit const& u, int i, FewPages const& p)
+    {
+        int const lane = threadIdx.x & 63, key = u.chunks.key0(i) + 16 * (lane >> 4), P = 1 << c.shift;
         int const page = (uint32_t) p.v < (uint32_t) c.pages ? p.v : 0;
-        size_t const scaleAt = (size_t) page * c.heads + h;
+        size_t const scaleAt = (size_t) page * c.heads + u.h;
         kScale = c.kScale[scaleAt];
         vScale = c.vScale[scaleAt];
-        uint8_t const* const from = c.v + page_offset(c, page, h) + m * P + (key & (P - 1));
+        uint8_t const* const from = c.v + page_offset(c, page, u.h) + (lane & 15) * P + (key & (P - 1));
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < KS; ++t)
         {
             vr[t] = *reinterpret_cast<u32x4 const*>(from + (16 * t < c.d ? 16 * t * P : 0)); // elements behind the head's end are not written
         }
-    };
+    }
 
-    f32x4 o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
+    // The chunk that was loaded; the next one's keys and values are requested by `keys` and `values`.
+    template <typename Keys, typename Values>
+    __device__ __forceinline__ void step(CacheArgs const& c, AttentionArgs const& a, FewUnit const& u, int i, FewPages const& p, Keys&& keys, Values&& values)
     {
-        o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    float negMax = kNothingSeen, sum = 0.f;
-    int i = split * a.fewSpan + wave;
-    Pages now{}, next{};
-    if (i < cEnd)
-    {
-        now = pages_of(i);
-        next = pages_of(min(i + kWaves, cEnd - 1));
-        load_keys(i, now);
-        load_values(i, now);
-    }
-    for (; i < cEnd; i += kWaves)
-    {
-        int const key0 = chunks.key0(i);
+        int const key0 = u.chunks.key0(i);
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -224,17 +243,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                 s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(kr[t][k][2], kr[t][k][3]), q[k][1], s[t], 0, 0, 0);
             }
         }
-        bool const more = i + kWaves < cEnd;
-        Pages const after = pages_of(min(i + 2 * kWaves, cEnd - 1));
-        if (more)
-        {
-            load_keys(i + kWaves, next);
-        }
         PageFactors const f = page_factors(kScale, vScale, a.scale);
+        keys();
         // keys of this lane that are there at all
-        int const there = (uint32_t) now.v < (uint32_t) c.pages ? min(max(r.len - key0 - 16 * g, 0), 16) : 0;
+        int const there = (uint32_t) p.v < (uint32_t) c.pages ? min(max(u.r.len - key0 - 16 * g, 0), 16) : 0;
         bool const whole = sees_all(least, most, key0) && __ballot(there < 16) == 0;
-        float mx = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 4; ++t)
         {
@@ -257,11 +270,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
             }
             u32x4 const keep = bytes_below(there);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < KS; ++t)
             {
                 vr[t] &= keep; // what was never written may be anything, and 0 times it not 0
             }
         }
+        float mx = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 4; ++t)
         {
@@ -273,125 +287,495 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
         {
             float const to = fminf(negNew, negMax), by = __builtin_amdgcn_exp2f(to - negMax);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < KS; ++t)
             {
                 o[t] *= by;
             }
             sum *= by;
             negMax = to;
         }
-        f16x8 p[2];
+        f16x8 w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
         {
-            float w[8];
+            float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                w[e] = __builtin_amdgcn_exp2f(s[2 * j + (e >> 2)][e & 3] + negMax);
-                sum = fmaf(w[e], f.inverse, sum);
+                x[e] = __builtin_amdgcn_exp2f(s[2 * j + (e >> 2)][e & 3] + negMax);
+                sum = fmaf(x[e], f.inverse, sum);
             }
-            p[j] = weights_f16(w);
+            w[j] = weights_f16(x);
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < KS; ++t)
         {
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][0], vr[t][1]), p[0], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][2], vr[t][3]), p[1], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][0], vr[t][1]), w[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_values8<FP8>(vr[t][2], vr[t][3]), w[1], o[t], 0, 0, 0);
         }
-        if (more)
+        values();
+    }
+
+    // Over the lanes that share a row.
+    __device__ float total() const
+    {
+        return reduce_step<32>(reduce_step<16>(sum, sum_of), sum_of);
+    }
+
+};
+
+// The sums of a workgroup's W wavefronts meet in LDS, as they are; then each thread adds some elements up over the wavefronts and gives
+// them to store(tile, sums, minus the maximum, sum of the weights).
+template <int KS, bool FP8, int W>
+struct FewMeeting
+{
+    static constexpr int kTiles = KS < 32 / W ? KS : 32 / W; // at a time: 32 KB
+    f32x4 sums[W][kTiles][kWaveSize];
+    float stats[W][2][kFewRows];
+
+    template <typename Store>
+    __device__ __forceinline__ void operator()(FewWave<KS, FP8> const& w, int wave, Store&& store)
+    {
+        int const lane = threadIdx.x & 63, m = w.m;
+        float const own = w.total();
+        if (lane < kFewRows)
         {
-            load_values(i + kWaves, next);
+            stats[wave][0][m] = w.negMax;
+            stats[wave][1][m] = own;
         }
+        float least = kNothingSeen, total = 0.f, by[W];
+#pragma unroll
+        for (int t0 = 0; t0 < KS; t0 += kTiles)
+        {
+            if (t0 > 0)
+            {
+                __syncthreads();
+            }
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+            {
+                if (t0 + t < KS)
+                {
+                    sums[wave][t][lane] = w.o[t0 + t];
+                }
+            }
+            __syncthreads();
+            if (t0 == 0)
+            {
+#pragma unroll
+                for (int x = 0; x < W; ++x)
+                {
+                    by[x] = stats[x][0][m];
+                    least = fminf(least, by[x]);
+                }
+#pragma unroll
+                for (int x = 0; x < W; ++x)
+                {
+                    by[x] = __builtin_amdgcn_exp2f(least - by[x]);
+                    total = fmaf(stats[x][1][m], by[x], total);
+                }
+            }
+            for (int t = wave; t < kTiles && t0 + t < KS; t += W)
+            {
+                f32x4 y = sums[0][t][lane] * by[0];
+#pragma unroll
+                for (int x = 1; x < W; ++x)
+                {
+                    y += sums[x][t][lane] * by[x];
+                }
+                store(t0 + t, y, least, total);
+            }
+        }
+    }
+};
+
+// Elements 16 t + 4 g .. + 3 of the lane's row, if there is such a row.
+template <int KS, bool FP8>
+__device__ inline void write_few(CacheArgs const& c, AttentionArgs const& a, FewUnit const& u, FewWave<KS, FP8> const& w, int t, f32x4 const& y, float total)
+{
+    float const inverse = total == 0.f ? 0.f : 1.f / total; // a row that sees nothing is zeros; a NaN stays one
+    if (16 * t < c.d && w.m < u.rows)
+    {
+        uint8_t* const to = a.out + 2 * ((int64_t) (u.r.row0 + w.token) * a.outToken + (int64_t) w.head * a.outHead);
+        *reinterpret_cast<f16x4*>(to + 2 * (16 * t + 4 * w.g))
+            = f16x4{(f16) (y[0] * inverse), (f16) (y[1] * inverse), (f16) (y[2] * inverse), (f16) (y[3] * inverse)};
+    }
+}
+
+// One workgroup a sequence and key head, its W wavefronts' sums meeting in LDS.
+template <int KS, bool FP8, int W>
+__global__ __launch_bounds__(W* kWaveSize) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_few_kernel(
+    CacheArgs const c, AttentionArgs const a)
+{
+    __shared__ FewMeeting<KS, FP8, W> meet;
+    FewUnit const u = few_unit(c, a, blockIdx.y, blockIdx.x);
+    if (u.rows == 0)
+    {
+        return;
+    }
+    int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    FewWave<KS, FP8> w;
+    int i = wave, end = u.count();
+    FewPages now{}, next{};
+    if (i < end)
+    {
+        now = w.pages_of(c, u, i);
+        next = w.pages_of(c, u, min(i + W, end - 1));
+    }
+    w.begin(c, a, u);
+    if (i < end)
+    {
+        w.load_keys(c, u, i, now);
+        w.load_values(c, u, i, now);
+    }
+    for (; i < end; i += W)
+    {
+        bool const more = i + W < end;
+        FewPages after{};
+        w.step(
+            c, a, u, i, now,
+            [&] {
+                if (more)
+                {
+                    after = w.pages_of(c, u, min(i + 2 * W, end - 1));
+                    w.load_keys(c, u, i + W, next);
+                }
+            },
+            [&] {
+                if (more)
+                {
+                    w.load_values(c, u, i + W, next);
+                }
+            });
         now = next;
         next = after;
     }
+    meet(w, wave, [&](int t, f32x4 const& y, float, float total) { write_few(c, a, u, w, t, y, total); });
+}
 
-    // ---- the wavefronts' sums
-    sum = reduce_step<32>(reduce_step<16>(sum, sum_of), sum_of);
-    if (g == 0)
+// All chunks of all sequences and key heads in a row, in equal stretches, one a workgroup, whose wavefronts take every fourth chunk:
+// sequences of any lengths keep the chip evenly busy to the end, and a wavefront's requests never pause, also from one head to the
+// next. A stretch that has all of a head's chunks writes its rows; of the others there is at most one at its beginning and one at its
+// end, whose sums go to memory, and the stretch in which a head begins says which those are. Where heads are few (ALIGNED) every stretch
+// is of one head: the meeting of the wavefronts and the next head's queries would be paid for twice by some.
+constexpr int kStretchWaves = 4;
+constexpr int kHeadCost = 4; // chunks that a head counts more, for its queries and the wavefronts' meeting: so many places come before its first
+
+// The sum over the lanes up to this one.
+__device__ inline int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false); // from 1, 2, 4 and 8 lanes below, in rows of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false); // the last lane of a row into the next
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false); // lane 31 into the upper half
+    return v;
+}
+
+struct Stretch
+{
+    FewUnit u; // that it begins with, at chunk `first`
+    int first;
+    int start;  // the place of u: chunk i of it is at start + kHeadCost + i of all
+    int end;    // of the stretch's places
+    int share;  // places of a stretch
+    bool none;
+};
+
+template <bool ALIGNED>
+__device__ inline int unit_places(FewUnit const& u)
+{
+    return u.rows ? u.count() + (ALIGNED ? 0 : kHeadCost) : 0;
+}
+
+// u of lane l.
+__device__ inline FewUnit unit_of_lane(FewUnit const& u, int b, int l)
+{
+    auto const from = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+    FewUnit v;
+    v.r = CacheRows{from(u.r.row0), from(u.r.n), from(u.r.begin), from(u.r.len)};
+    v.chunks = Chunks{from(u.chunks.sinkChunks), from(u.chunks.first), from(u.chunks.total)};
+    v.b = b;
+    v.h = 0;
+    v.rows = from(u.rows);
+    return v;
+}
+
+template <bool ALIGNED>
+__device__ inline Stretch stretch_of_workgroup(CacheArgs const& c, AttentionArgs const& a, int B)
+{
+    int const lane = threadIdx.x & 63, wgs = (int) gridDim.x, wg = (int) blockIdx.x;
+    auto const unit_at = [&](int b) {
+        FewUnit u{};
+        if (b < B)
+        {
+            u = few_unit(c, a, b, 0);
+        }
+        return u;
+    };
+    FewUnit u = unit_at(lane);
+    int n = unit_places<ALIGNED>(u);
+    for (int b0 = kWaveSize; b0 < B; b0 += kWaveSize)
     {
-        stats[wave][0][m] = negMax;
-        stats[wave][1][m] = sum;
+        n += unit_places<ALIGNED>(unit_at(b0 + lane));
+    }
+    int const total = wave_sum_i32(n) * c.heads;
+    Stretch s{};
+    s.none = true;
+    // a chunk a wavefront at least; ALIGNED: so that the stretches' number with one more for each head is no more than the workgroups'
+    s.share = max((total + wgs - 1) / (ALIGNED ? max(wgs - B * c.heads, 1) : wgs), kStretchWaves);
+    int const target = ALIGNED ? wg : wg * s.share; // stretches, or chunks, before this one
+    if (!ALIGNED && target >= total)
+    {
+        return s;
+    }
+    int before = 0;
+    for (int b0 = 0;;)
+    {
+        int const of = unit_places<ALIGNED>(u), here = (ALIGNED ? (of + s.share - 1) / s.share : of) * c.heads, scanned = wave_scan(here);
+        uint64_t const behind = __ballot(before + scanned > target);
+        if (behind != 0)
+        {
+            int const l = __builtin_ctzll(behind);
+            before += __builtin_amdgcn_readlane(scanned, l) - __builtin_amdgcn_readlane(here, l);
+            s.u = unit_of_lane(u, b0 + l, l);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(scanned, 63);
+        b0 += kWaveSize;
+        if (b0 >= B)
+        {
+            return s; // none is left for this workgroup
+        }
+        u = unit_at(b0 + lane);
+    }
+    int const places = unit_places<ALIGNED>(s.u), each = ALIGNED ? (places + s.share - 1) / s.share : places;
+    s.u.h = (target - before) / each;
+    int const at = target - before - s.u.h * each;
+    s.none = false;
+    if (ALIGNED)
+    {
+        s.first = at * s.share;
+        s.start = -kHeadCost;
+        s.end = s.first + s.share;
+    }
+    else
+    {
+        s.first = max(at - kHeadCost, 0);
+        s.start = target - at;
+        s.end = min(target + s.share, total);
+    }
+    return s;
+}
+
+template <int KS, bool FP8, bool ALIGNED>
+__global__ __launch_bounds__(kStretchWaves* kWaveSize) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_stretch_kernel(
+    CacheArgs const c, AttentionArgs const a, int const B)
+{
+    constexpr int W = kStretchWaves;
+    __shared__ FewMeeting<KS, FP8, W> meet;
+    Stretch start = stretch_of_workgroup<ALIGNED>(c, a, B);
+    // the same in every lane, which the compiler does not see behind the search
+    int const head_of_start = start.u.h;
+    start.u = unit_of_lane(start.u, __builtin_amdgcn_readfirstlane(start.u.b), 0);
+    start.u.h = __builtin_amdgcn_readfirstlane(head_of_start);
+    start.first = __builtin_amdgcn_readfirstlane(start.first);
+    start.start = __builtin_amdgcn_readfirstlane(start.start);
+    start.share = __builtin_amdgcn_readfirstlane(start.share);
+    int const stop = __builtin_amdgcn_readfirstlane(start.end);
+    if (start.none)
+    {
+        return;
+    }
+    int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // A chunk of the stretch, or none.
+    struct Cursor
+    {
+        FewUnit u;
+        int i, start;
+        bool valid;
+    };
+    // By a number of chunks; only heads that have a place in the stretch are looked at.
+    auto const next_head = [&](Cursor& x) {
+        x.start += x.u.count() + kHeadCost;
+        if (x.u.h + 1 < c.heads)
+        {
+            ++x.u.h;
+            return;
+        }
+        do
+        {
+            x.u = few_unit(c, a, x.u.b + 1, 0);
+        } while (x.u.rows == 0 && x.u.b + 1 < B);
+    };
+    auto const advance = [&](Cursor& x, int by) {
+        x.i += by;
+        while (x.i >= x.u.count())
+        {
+            bool const another = !ALIGNED && x.start + x.u.count() + 2 * kHeadCost < stop; // its first chunk's place
+            x.i -= x.u.count();
+            if (another)
+            {
+                next_head(x);
+            }
+            if (!another || x.u.rows == 0)
+            {
+                x.valid = false;
+                return;
+            }
+        }
+        x.valid = x.start + kHeadCost + x.i < stop;
+    };
+    Cursor head = {start.u, start.first, start.start, true}; // the head that the wavefronts are at
+    Cursor now = head;
+    advance(now, wave);
+    Cursor next = now;
+    FewWave<KS, FP8> w;
+    FewPages nowPages{}, nextPages{};
+    if (now.valid)
+    {
+        nowPages = w.pages_of(c, now.u, now.i);
+        advance(next, W);
+        if (next.valid)
+        {
+            nextPages = w.pages_of(c, next.u, next.i);
+        }
+    }
+    w.begin(c, a, head.u);
+    if (now.valid)
+    {
+        w.load_keys(c, now.u, now.i, nowPages);
+        w.load_values(c, now.u, now.i, nowPages);
+    }
+    for (bool begun = false;; begun = true) // begun: the head begins in this stretch, behind another
+    {
+        while (now.valid && now.start == head.start)
+        {
+            FewPages afterPages{};
+            Cursor after = next;
+            w.step(
+                c, a, head.u, now.i, nowPages,
+                [&] {
+                    if (next.valid)
+                    {
+                        advance(after, W);
+                        if (after.valid)
+                        {
+                            afterPages = w.pages_of(c, after.u, after.i);
+                        }
+                        w.load_keys(c, next.u, next.i, nextPages);
+                    }
+                },
+                [&] {
+                    if (next.valid)
+                    {
+                        w.load_values(c, next.u, next.i, nextPages);
+                    }
+                });
+            now = next;
+            next = after;
+            nowPages = nextPages;
+            nextPages = afterPages;
+        }
+        FewUnit const& u = head.u;
+        int const count = u.count(), last = min(count, stop - head.start - kHeadCost); // one past the stretch's last chunk of u
+        bool const all = head.i == 0 && last == count;
+        int const slot = 2 * (int) blockIdx.x + (begun ? 1 : 0);
+        size_t const row = (size_t) slot * kFewRows + w.m;
+        meet(w, wave, [&](int t, f32x4 const& y, float negMax, float total) {
+            if (all)
+            {
+                write_few(c, a, u, w, t, y, total);
+            }
+            else if (16 * t < c.d && w.m < u.rows)
+            {
+                *reinterpret_cast<f32x4*>(a.fewPartial + row * c.d + 16 * t + 4 * w.g) = y;
+                if (t == 0 && w.g == 0)
+                {
+                    *reinterpret_cast<f32x2*>(a.fewStats + 2 * row) = f32x2{negMax, total};
+                }
+            }
+        });
+        if (head.i == 0 && threadIdx.x == 0)
+        {
+            int const used = ALIGNED ? (count + start.share - 1) / start.share
+                                     : (head.start + kHeadCost + count - 1) / start.share - (int) blockIdx.x + 1;
+            *reinterpret_cast<i32x2*>(a.fewHeads + 2 * ((size_t) u.b * c.heads + u.h)) = i32x2{slot, used};
+        }
+        head.i = 0;
+        advance(head, count);
+        if (!head.valid)
+        {
+            return;
+        }
+        __syncthreads(); // the meeting's LDS
+        w.begin(c, a, head.u);
+    }
+}
+
+// The sums of a row's stretches: a workgroup a row, L lanes on the values of one, 256 / L of them at a time. Rows that one stretch had are
+// written already.
+template <int L>
+__global__ __launch_bounds__(kThreads) void cached_stretch_join_kernel(CacheArgs const c, AttentionArgs const a)
+{
+    constexpr int kGroups = kThreads / L;
+    __shared__ f32x4 meet[kGroups][L];
+    __shared__ float totals[kGroups];
+    int const row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+    i32x2 const where = *reinterpret_cast<i32x2 const*>(a.fewHeads + 2 * ((size_t) b * c.heads + h));
+    CacheRows const r = cache_rows(c, b);
+    int64_t const rows = (int64_t) r.n * a.group.d;
+    if (row >= rows || rows > kFewRows || where[1] <= 1)
+    {
+        return;
+    }
+    // the first is where the head begins, the others are at the beginning of their stretches
+    int const used = where[1], s0 = where[0];
+    auto slot_of = [&](int s) { return (size_t) (s == 0 ? s0 : (s0 & ~1) + 2 * s) * kFewRows + row; };
+    float least = kNothingSeen;
+    for (int s = lane; s < used; s += kWaveSize)
+    {
+        least = fminf(least, a.fewStats[2 * slot_of(s)]);
+    }
+    least = group_allreduce<kWaveSize>(least, [](float x, float y) { return fminf(x, y); });
+    int const part = threadIdx.x / L, e = 4 * (threadIdx.x & (L - 1));
+    float sum = 0.f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    if (e < c.d)
+    {
+#pragma unroll 4
+        for (int s = part; s < used; s += kGroups)
+        {
+            size_t const slot = slot_of(s);
+            f32x2 const st = *reinterpret_cast<f32x2 const*>(a.fewStats + 2 * slot);
+            float const by = __builtin_amdgcn_exp2f(least - st[0]);
+            sum = fmaf(st[1], by, sum);
+            y += *reinterpret_cast<f32x4 const*>(a.fewPartial + slot * c.d + e) * by;
+        }
+    }
+    meet[part][threadIdx.x & (L - 1)] = y;
+    if (e == 0)
+    {
+        totals[part] = sum;
     }
     __syncthreads();
-    float least4 = kNothingSeen, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-    {
-        least4 = fminf(least4, stats[w][0][m]);
-    }
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-    {
-        total = fmaf(stats[w][1][m], __builtin_amdgcn_exp2f(least4 - stats[w][0][m]), total);
-    }
-    float const by = __builtin_amdgcn_exp2f(least4 - negMax);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-    {
-        o[t] *= by;
-    }
-#pragma unroll
-    for (int half = kWaves / 2; half > 0; half /= 2)
-    {
-        if (wave >= half && wave < 2 * half)
-        {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-            {
-                meet[wave - half][t][lane] = o[t];
-            }
-        }
-        __syncthreads();
-        if (wave < half)
-        {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-            {
-                o[t] += meet[wave][t][lane];
-            }
-        }
-        __syncthreads();
-    }
-    if (wave != 0 || m >= rows)
+    if (threadIdx.x >= L || e >= c.d)
     {
         return;
     }
-    size_t const outRow = (size_t) (r.row0 + token);
-    if (used > 1)
+    sum = totals[0];
+    y = meet[0][threadIdx.x];
+#pragma unroll
+    for (int p = 1; p < kGroups; ++p)
     {
-        size_t const slot = (outRow * a.qHeads + head) * a.slots + split;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-        {
-            if (16 * t < c.d)
-            {
-                *reinterpret_cast<f32x4*>(a.partial + slot * c.d + 16 * t + 4 * g) = o[t];
-            }
-        }
-        if (g == 0)
-        {
-            *reinterpret_cast<f32x2*>(a.stats + 2 * slot) = f32x2{least4, total};
-        }
-        return;
+        sum += totals[p];
+        y += meet[p][threadIdx.x];
     }
-    float const inverse = total == 0.f ? 0.f : 1.f / total; // a row that sees nothing is zeros; a NaN stays one
-    uint8_t* const to = a.out + 2 * (outRow * a.outToken + (int64_t) head * a.outHead);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-    {
-        if (16 * t < c.d)
-        {
-            f16x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-            {
-                y[e] = (f16) (o[t][e] * inverse);
-            }
-            *reinterpret_cast<f16x4*>(to + 2 * (16 * t + 4 * g)) = y;
-        }
-    }
+    float const inverse = sum == 0.f ? 0.f : 1.f / sum;
+    int const token = (int) ((uint32_t) row / a.group), head = h * (int) a.group.d + row - token * (int) a.group.d;
+    *reinterpret_cast<f16x4*>(a.out + 2 * ((int64_t) (r.row0 + token) * a.outToken + (int64_t) head * a.outHead + e))
+        = f16x4{(f16) (y[0] * inverse), (f16) (y[1] * inverse), (f16) (y[2] * inverse), (f16) (y[3] * inverse)};
 }
 
 // ------------------------------------------------------------------------------------------
@@ -409,13 +793,12 @@ struct ManyLds
 };
 
 template <int KS /* 16 of the head's values */, bool FP8>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 8 ? 2 : 1))) void cached_many_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_many_kernel(
     CacheArgs const c, AttentionArgs const a, FastDiv const heads)
 {
     constexpr int DP = padded_head(KS);
     using Lds = ManyLds<DP>;
-    constexpr int kPieces = DP / 16;                     // of 16 bytes in a key
-    constexpr int NL = kChunkKeys * kPieces / kThreads;  // loads a thread of keys, and of values
+    constexpr int NL = DP / 64; // loads a thread of keys, and of values
     constexpr int DV = (KS + 1) / 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     // tiles of a head are a multiple of the heads apart, so that where those divide by 8 they share an XCD's L2
@@ -463,45 +846,39 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
         }
     }
 
-    // this thread's pieces of a chunk: 16 bytes of key (tid + 256 i) / kPieces, 16 keys of value row (tid + 256 i) / 4
+    // This thread's pieces of a chunk: 16 bytes each of key tid / 4, and 16 keys of value rows tid / 4 + 64 l. A wavefront's 16 keys lie in
+    // one page, so its place is scalar arithmetic.
     int32_t const* const table = c.table + (int64_t) b * c.maxPages;
-    int const piece = tid & (kPieces - 1), vGroup = tid & 3;
+    int const ownKey = 16 * wave + (lane >> 2), piece = lane & 3, vGroup = lane & 3, vRow = tid >> 2;
+    // behind the head's end again its last values, times a query of zeros, and rows whose sums are not written
+    uint32_t kAt[NL], vAt[NL];
+#pragma unroll
+    for (int l = 0; l < NL; ++l)
+    {
+        kAt[l] = (uint32_t) ((lane >> 2) * c.d + min(16 * (piece + 4 * l), c.d - 16));
+        vAt[l] = (uint32_t) min(vRow + 64 * l, c.d - 1) * P;
+    }
     auto page_at = [&](int key) { return table[min(key >> c.shift, c.maxPages - 1)]; };
     auto sound = [&](int page) { return (uint32_t) page < (uint32_t) c.pages ? page : 0; };
     struct Pages
     {
-        int k[NL], v;
+        int k, v;
     };
     auto pages_of = [&](int i) {
-        Pages p;
         int const key0 = chunks.key0(i);
-#pragma unroll
-        for (int l = 0; l < NL; ++l)
-        {
-            p.k[l] = page_at(key0 + (tid + kThreads * l) / kPieces);
-        }
-        p.v = page_at(key0 + 16 * vGroup);
-        return p;
+        return Pages{__builtin_amdgcn_readfirstlane(page_at(key0 + 16 * wave)), page_at(key0 + 16 * vGroup)};
     };
     u32x4 kr[NL], vr[NL];
     float kScale = 0.f, vScale = 0.f;
     auto request = [&](int i, Pages const& p) {
         int const key0 = chunks.key0(i);
-        size_t const vPage = page_offset(c, sound(p.v), h);
+        uint8_t const* const keys = c.k + page_offset(c, sound(p.k), h) + (uint32_t) ((key0 + 16 * wave) & (P - 1)) * c.d;
+        uint8_t const* const values = c.v + page_offset(c, sound(p.v), h) + ((key0 + 16 * vGroup) & (P - 1));
 #pragma unroll
         for (int l = 0; l < NL; ++l)
         {
-            int const key = key0 + (tid + kThreads * l) / kPieces, vRow = (tid + kThreads * l) >> 2;
-            kr[l] = u32x4{0, 0, 0, 0};
-            vr[l] = u32x4{0, 0, 0, 0};
-            if (16 * piece < c.d)
-            {
-                kr[l] = *reinterpret_cast<u32x4 const*>(c.k + page_offset(c, sound(p.k[l]), h) + (uint32_t) (key & (P - 1)) * c.d + 16 * piece);
-            }
-            if (vRow < c.d)
-            {
-                vr[l] = *reinterpret_cast<u32x4 const*>(c.v + vPage + (uint32_t) vRow * P + ((key0 + 16 * vGroup) & (P - 1)));
-            }
+            kr[l] = *reinterpret_cast<u32x4 const*>(keys + kAt[l]);
+            vr[l] = *reinterpret_cast<u32x4 const*>(values + vAt[l]);
         }
         if (tid < 4)
         {
@@ -510,23 +887,29 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
             vScale = c.vScale[at];
         }
     };
+    int const kRowAt = (ownKey & 32) + row_of_key(ownKey & 31);
     auto deliver = [&](int i, Pages const& p, int slot) {
-        uint8_t* const keys = lds + slot * Lds::kSlot;
-        uint8_t* const values = keys + Lds::kKeys;
+        uint8_t* const keys = lds + slot * Lds::kSlot + kRowAt * DP * 2;
+        uint8_t* const values = lds + slot * Lds::kSlot + Lds::kKeys + vRow * kChunkKeys * 2;
         int const there = (uint32_t) p.v < (uint32_t) c.pages ? min(max(r.len - chunks.key0(i) - 16 * vGroup, 0), 16) : 0;
-        u32x4 const keep = bytes_below(there);
+        if (__ballot(there < 16) != 0)
+        {
+            u32x4 const keep = bytes_below(there);
+#pragma unroll
+            for (int l = 0; l < NL; ++l)
+            {
+                vr[l] &= keep; // what was never written may be anything, and 0 times it not 0
+            }
+        }
 #pragma unroll
         for (int l = 0; l < NL; ++l)
         {
-            int const key = (tid + kThreads * l) / kPieces, vRow = (tid + kThreads * l) >> 2;
-            int const kRow = (key & 32) + row_of_key(key & 31);
-            uint8_t* const k0 = keys + kRow * DP * 2;
-            *reinterpret_cast<f16x8*>(k0 + 16 * swizzled(kRow, 2 * piece)) = code_values8<FP8>(kr[l][0], kr[l][1]);
-            *reinterpret_cast<f16x8*>(k0 + 16 * swizzled(kRow, 2 * piece + 1)) = code_values8<FP8>(kr[l][2], kr[l][3]);
-            u32x4 const v = vr[l] & keep; // what was never written may be anything, and 0 times it not 0
-            uint8_t* const v0 = values + vRow * kChunkKeys * 2;
-            *reinterpret_cast<f16x8*>(v0 + 16 * swizzled(vRow, 2 * vGroup)) = code_values8<FP8>(v[0], v[1]);
-            *reinterpret_cast<f16x8*>(v0 + 16 * swizzled(vRow, 2 * vGroup + 1)) = code_values8<FP8>(v[2], v[3]);
+            int const at = 2 * (piece + 4 * l);
+            *reinterpret_cast<f16x8*>(keys + 16 * swizzled<2 * DP>(kRowAt, at)) = code_values8<FP8>(kr[l][0], kr[l][1]);
+            *reinterpret_cast<f16x8*>(keys + 16 * swizzled<2 * DP>(kRowAt, at + 1)) = code_values8<FP8>(kr[l][2], kr[l][3]);
+            uint8_t* const v = values + 64 * l * kChunkKeys * 2;
+            *reinterpret_cast<f16x8*>(v + 16 * swizzled<2 * kChunkKeys>(vRow, 2 * vGroup)) = code_values8<FP8>(vr[l][0], vr[l][1]);
+            *reinterpret_cast<f16x8*>(v + 16 * swizzled<2 * kChunkKeys>(vRow, 2 * vGroup + 1)) = code_values8<FP8>(vr[l][2], vr[l][3]);
         }
         if (tid < 4)
         {
@@ -579,22 +962,26 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                     for (int t = 0; t < 2; ++t)
                     {
                         int const kRow = 32 * t + lq;
-                        f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRow * DP * 2 + 16 * swizzled(kRow, 2 * e + half));
+                        f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRow * DP * 2 + 16 * swizzled<2 * DP>(kRow, 2 * e + half));
                         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
                     }
                 }
                 bool const whole = sees_all(least, most, key0) && __ballot(there[0] < 16 || there[1] < 16) == 0;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                    {
-                        s[t][v] = fmaf(s[t][v], f[t][0], f[t][1]);
-                    }
-                }
+// in powers of 2, s * by + add: where all keys are seen and there, by one multiply-add together with the maximum
+                float by[2] = {f[0][0], f[1][0]}, add[2] = {f[0][1], f[1][1]};
                 if (!whole)
                 {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                        {
+                            s[t][v] = fmaf(s[t][v], by[t], add[t]);
+                        }
+                        by[t] = 1.f;
+                        add[t] = 0.f;
+                    }
                     hide(s, seen, key0 + 16 * half);
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
@@ -611,14 +998,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                 }
                 float mx = -__builtin_inff();
 #pragma unroll
-                for (int v = 0; v < 32; ++v)
+                for (int t = 0; t < 2; ++t)
                 {
-                    mx = fmaxf(mx, s[v >> 4][v & 15]);
+                    float own = s[t][0];
+#pragma unroll
+                    for (int v = 1; v < 16; ++v)
+                    {
+                        own = fmaxf(own, s[t][v]);
+                    }
+                    mx = fmaxf(mx, fmaf(own, by[t], add[t]));
                 }
                 sums.move(reduce_step<32>(mx, max_of));
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
                 {
+                    float const base = add[t] + sums.negMax;
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
                     {
@@ -626,7 +1020,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                         {
-                            p[e] = __builtin_amdgcn_exp2f(s[t][8 * w + e] + sums.negMax);
+                            p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * w + e], by[t], base));
                             sums.sum = fmaf(p[e], f[t][2], sums.sum);
                         }
                         f16x8 const weights = weights_f16(p);
@@ -635,7 +1029,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                         {
                             int const vRow = 32 * d + lq;
                             f16x8 const v = *reinterpret_cast<f16x8 const*>(
-                                values + vRow * kChunkKeys * 2 + 16 * swizzled(vRow, 4 * t + 2 * half + w));
+                                values + vRow * kChunkKeys * 2 + 16 * swizzled<2 * kChunkKeys>(vRow, 4 * t + 2 * half + w));
                             sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights, sums.out[d], 0, 0, 0);
                         }
                     }
@@ -705,18 +1099,11 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs const c
         return;
     }
     int const token = (int) ((uint32_t) unit / heads), head = unit - token * (int) heads.d;
-    bool const few = rows <= a.fewLimit;
-    int const span = few ? a.fewSpan : a.manySpan;
-    int i0 = 0, i1 = r.n - 1;
-    if (!few)
-    {
-        int const own = head - (int) ((uint32_t) head / a.group) * group;
-        int const row0 = (token * group + own) / kTileRows * kTileRows;
-        i0 = (int) ((uint32_t) row0 / a.group);
-        i1 = (int) ((uint32_t) (min((int64_t) row0 + kTileRows, rows) - 1) / a.group);
-    }
-    int const used = (chunks_of_tokens(r, i0, i1, a).total + span - 1) / span;
-    if (used <= 1)
+    int const own = head - (int) ((uint32_t) head / a.group) * group;
+    int const row0 = (token * group + own) / kTileRows * kTileRows;
+    int const i0 = (int) ((uint32_t) row0 / a.group), i1 = (int) ((uint32_t) (min((int64_t) row0 + kTileRows, rows) - 1) / a.group);
+    int const used = (chunks_of_tokens(r, i0, i1, a).total + a.manySpan - 1) / a.manySpan;
+    if (used <= 1 || rows <= a.fewLimit)
     {
         return;
     }
@@ -773,12 +1160,11 @@ __global__ __launch_bounds__(kThreads) void cached_join_kernel(CacheArgs const c
 struct Plan
 {
     bool few, many;
-    int fewSpan, fewSplits, manySpan, manySplits;
     int fewLimit;
-    int slots() const
-    {
-        return std::max(few ? fewSplits : 1, many ? manySplits : 1);
-    }
+    int fewWaves;  // of a workgroup a sequence and key head, or
+    int stretches; // how many
+    bool aligned;  // each of one head
+    int manySpan, manySplits;
 };
 
 // Chunks of `most` that a part takes, and how many parts that are at most.
@@ -796,33 +1182,48 @@ Plan plan_of(trtamd_kv_cache_attention_params const& p)
     int const group = p.q_heads / c.kv_heads;
     int64_t const tokens = std::min(c.max_tokens, c.T);
     int64_t const rows = tokens * group;
-    plan.few = rows <= kFewRows || c.B > 1;
+    plan.few = rows <= kFewRows || (c.B > 1 && group <= kFewRows);
     plan.many = rows > kFewRows;
     plan.fewLimit = plan.few ? kFewRows : 0;
     // keys that a row sees at most, and about
     int64_t const capacity = (int64_t) c.max_pages * c.page_tokens;
-    auto const seen = [&](int64_t length) {
-        int64_t const near = p.window ? (int64_t) p.window + tokens : length;
-        return std::min(length, p.window ? near + p.sinks : length);
-    };
+    auto const seen = [&](int64_t length) { return p.window ? std::min(length, p.window + tokens + p.sinks) : length; };
     int64_t const most = ceil_div(seen(capacity), (int64_t) kChunkKeys) + 2;
     int64_t const chunks = ceil_div(seen(p.max_length > 0 ? std::min<int64_t>(p.max_length, capacity) : capacity), (int64_t) kChunkKeys) + (p.window ? 1 : 0);
     int64_t const cus = num_cus(), head = head_steps(c.d);
-    // Few rows: one generation of workgroups, and where there are several sequences, whose lengths differ, parts of no more than 16
-    // chunks. Four chunks are one a wavefront.
-    int64_t const resident = cus * (head <= 4 ? 3 : head <= 8 ? 2 : 1);
-    int64_t const even = ceil_div((int64_t) c.B * c.kv_heads * chunks, resident);
-    share_out(std::max<int64_t>(c.B > 1 ? std::min<int64_t>(even, 16) : even, 4), most, plan.fewSpan, plan.fewSplits);
+    int64_t const units = (int64_t) c.B * c.kv_heads;
+    if (plan.few)
+    {
+        int64_t const resident = cus * (head <= 4 ? 3 : head <= 8 ? 2 : 1); // workgroups of four wavefronts
+        bool const sums = units * most < (int64_t) 1 << 30;                      // of chunks fit 32 bits
+        plan.fewWaves = units <= cus && head <= 8 ? 8 : 4;
+        // Above 128 KB of keys and values a head, one workgroup a head is slower than stretches and their joining.
+        if (chunks * head > 64 && units < 8 * resident && c.B <= 1024 && sums)
+        {
+            plan.stretches = (int) resident;
+            plan.aligned = 4 * units <= resident;
+        }
+    }
     // More rows: whole where there are tiles enough for two a CU.
     int64_t const tiles = ceil_div((int64_t) c.T * group, (int64_t) kTileRows) * c.kv_heads;
     share_out(tiles >= 2 * cus ? most : std::max<int64_t>(ceil_div(tiles * chunks, 2 * cus), 8), most, plan.manySpan, plan.manySplits);
     return plan;
 }
 
+// Sums that go to memory, in floats: those of stretches, and of more rows' parts.
+size_t few_floats(trtamd_kv_cache_attention_params const& p, Plan const& plan)
+{
+    return plan.stretches ? (size_t) plan.stretches * 2 * kFewRows * (p.cache.d + 2) + (((size_t) p.cache.B * p.cache.kv_heads * 2 + 3) & ~(size_t) 3) : 0;
+}
+
+size_t many_floats(trtamd_kv_cache_attention_params const& p, Plan const& plan)
+{
+    return plan.many && plan.manySplits > 1 ? (size_t) p.cache.T * p.q_heads * plan.manySplits * (p.cache.d + 2) : 0;
+}
+
 size_t workspace_of(trtamd_kv_cache_attention_params const& p, Plan const& plan)
 {
-    size_t const slots = (size_t) plan.slots();
-    return slots <= 1 ? 0 : (size_t) p.cache.T * p.q_heads * slots * (p.cache.d + 2) * sizeof(float);
+    return (few_floats(p, plan) + many_floats(p, plan)) * sizeof(float);
 }
 
 int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
@@ -880,14 +1281,46 @@ int launch(hipStream_t stream, trtamd_kv_cache_attention_params const& p, Plan c
     int const group = p.q_heads / k.kv_heads;
     if (plan.few)
     {
-        dim3 const grid((unsigned) k.kv_heads, (unsigned) k.B, (unsigned) plan.fewSplits);
         int const st = by_head(k.d, [&](auto steps) {
-            hipLaunchKernelGGL((cached_few_kernel<decltype(steps)::value, FP8>), grid, dim3(kThreads), 0, stream, c, a);
+            constexpr int S = decltype(steps)::value;
+            if (plan.stretches)
+            {
+                dim3 const grid((unsigned) plan.stretches), block(kStretchWaves * kWaveSize);
+                if (plan.aligned)
+                {
+                    hipLaunchKernelGGL((cached_stretch_kernel<S, FP8, true>), grid, block, 0, stream, c, a, k.B);
+                }
+                else
+                {
+                    hipLaunchKernelGGL((cached_stretch_kernel<S, FP8, false>), grid, block, 0, stream, c, a, k.B);
+                }
+                return check_launch("cached_stretch_kernel");
+            }
+            dim3 const grid((unsigned) k.kv_heads, (unsigned) k.B);
+            if constexpr (S <= 8)
+            {
+                if (plan.fewWaves == 8)
+                {
+                    hipLaunchKernelGGL((cached_few_kernel<S, FP8, 8>), grid, dim3(8 * kWaveSize), 0, stream, c, a);
+                    return check_launch("cached_few_kernel");
+                }
+            }
+            hipLaunchKernelGGL((cached_few_kernel<S, FP8, 4>), grid, dim3(4 * kWaveSize), 0, stream, c, a);
             return check_launch("cached_few_kernel");
         });
         if (st)
         {
             return st;
+        }
+        if (plan.stretches)
+        {
+            dim3 const grid((unsigned) std::min<int64_t>(kFewRows, (int64_t) std::min(k.max_tokens, k.T) * group), (unsigned) k.kv_heads, (unsigned) k.B);
+            auto const run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, c, a); };
+            k.d <= 64 ? run(cached_stretch_join_kernel<16>) : k.d <= 128 ? run(cached_stretch_join_kernel<32>) : run(cached_stretch_join_kernel<64>);
+            if (int const joined = check_launch("cached_stretch_join_kernel"))
+            {
+                return joined;
+            }
         }
     }
     if (plan.many)
@@ -901,11 +1334,9 @@ int launch(hipStream_t stream, trtamd_kv_cache_attention_params const& p, Plan c
             return st;
         }
     }
-    if (plan.slots() > 1)
+    if (plan.many && plan.manySplits > 1)
     {
-        // where only sequences of few rows are shared between workgroups, theirs alone
-        int64_t const tokens = plan.many && plan.manySplits > 1 ? std::min(k.max_tokens, k.T) : std::min(std::min(k.max_tokens, k.T), kFewRows / group);
-        dim3 const grid((unsigned) (tokens * p.q_heads), (unsigned) k.B);
+        dim3 const grid((unsigned) (std::min(k.max_tokens, k.T) * p.q_heads), (unsigned) k.B);
         FastDiv const heads = fast_div((uint32_t) p.q_heads);
         auto const run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, c, a, heads); };
         k.d <= 64 ? run(cached_join_kernel<16>) : k.d <= 128 ? run(cached_join_kernel<32>) : run(cached_join_kernel<64>);
@@ -977,11 +1408,14 @@ extern "C" int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
     a.q = reinterpret_cast<uint8_t const*>(p.q);
     a.out = reinterpret_cast<uint8_t*>(p.out);
     a.qToken = p.q_token_stride, a.qHead = p.q_head_stride, a.outToken = p.out_token_stride, a.outHead = p.out_head_stride;
-    a.partial = static_cast<float*>(p.workspace);
-    a.stats = a.partial + (bytes ? (size_t) c.T * p.q_heads * plan.slots() * c.d : 0);
+    a.fewPartial = static_cast<float*>(p.workspace);
+    a.fewStats = a.fewPartial + (size_t) plan.stretches * 2 * kFewRows * c.d;
+    a.fewHeads = reinterpret_cast<int32_t*>(a.fewStats + (size_t) plan.stretches * 2 * kFewRows * 2);
+    a.partial = a.fewPartial + few_floats(p, plan);
+    a.stats = a.partial + (plan.manySplits > 1 ? (size_t) c.T * p.q_heads * plan.manySplits * c.d : 0);
     a.group = fast_div((uint32_t) (p.q_heads / c.kv_heads));
-    a.qHeads = p.q_heads, a.window = p.window, a.sinks = p.sinks, a.slots = plan.slots();
-    a.fewSpan = plan.fewSpan, a.manySpan = plan.manySpan, a.fewLimit = plan.fewLimit;
+    a.qHeads = p.q_heads, a.window = p.window, a.sinks = p.sinks, a.slots = plan.manySplits;
+    a.manySpan = plan.manySpan, a.fewLimit = plan.fewLimit;
     a.scale = p.scale * 1.44269504088896f;
     return c.data_type == kCacheFp8 ? launch<true>(as_stream(stream), p, plan, a) : launch<false>(as_stream(stream), p, plan, a);
 }

@@ -161,9 +161,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
 #pragma unroll
     for (int l = 0; l < NL; ++l)
     {
-        int const r = (l * kWaves + wave) * kRowsPerLoad + rowInLoad, chunk = swizzled(r, place);
-        kAt[l] = (uint32_t) ((r & 32) + key_of_row(r & 31)) * (uint32_t) a.k.token + 16u * (uint32_t) chunk;
-        vAt[l] = (uint32_t) r * (uint32_t) a.v.token + 16u * (uint32_t) chunk;
+        int const r = (l * kWaves + wave) * kRowsPerLoad + rowInLoad;
+        // both are their own inverses
+        kAt[l] = (uint32_t) ((r & 32) + key_of_row(r & 31)) * (uint32_t) a.k.token + 16u * (uint32_t) swizzled<kRow>(r, place);
+        vAt[l] = (uint32_t) r * (uint32_t) a.v.token + 16u * (uint32_t) swizzled_turned<kRow>(r, place);
     }
     uint8_t const* const kUnit = a.k.p + (int64_t) first * a.k.token + (int64_t) h * a.k.head;
     uint8_t const* const vUnit = a.v.p + (int64_t) first * a.v.token + (int64_t) h * a.v.head;
@@ -185,15 +186,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
         for (int l = 0; l < NL; ++l)
         {
             int const r0 = (l * kWaves + wave) * kRowsPerLoad, r = r0 + rowInLoad;
-            int const chunk = swizzled(r, place); // its own inverse
-            bool const inHead = 8 * chunk < a.d;
+            int const kChunk = swizzled<kRow>(r, place), vChunk = swizzled_turned<kRow>(r, place);
             int const kKey = min(key0 + (r & 32) + key_of_row(r & 31), n - 1), vKey = key0 + r;
-            uint8_t const* const k = kUnit + (int64_t) kKey * a.k.token + 16 * chunk;
+            uint8_t const* const k = kUnit + (int64_t) kKey * a.k.token + 16 * kChunk;
             // 0, the weight of a key behind the sequence, times an infinite value would not be 0
-            uint8_t const* const v = vUnit + (int64_t) vKey * a.v.token + 16 * chunk;
+            uint8_t const* const v = vUnit + (int64_t) vKey * a.v.token + 16 * vChunk;
             uint8_t const* const zeros = reinterpret_cast<uint8_t const*>(kZeros);
-            load_to_lds16(inHead ? k : zeros, to + (uint32_t) (r0 * kRow));
-            load_to_lds16(inHead && vKey < n ? v : zeros, to + (uint32_t) (Lds::kMatrix + r0 * kRow));
+            load_to_lds16(8 * kChunk < a.d ? k : zeros, to + (uint32_t) (r0 * kRow));
+            load_to_lds16(8 * vChunk < a.d && vKey < n ? v : zeros, to + (uint32_t) (Lds::kMatrix + r0 * kRow));
         }
     };
 
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
             for (int t = 0; t < 2; ++t)
             {
                 int const kRowAt = 32 * t + lq;
-                f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRowAt * kRow + 16 * swizzled(kRowAt, 2 * e + half));
+                f16x8 const k = *reinterpret_cast<f16x8 const*>(keys + kRowAt * kRow + 16 * swizzled<kRow>(kRowAt, 2 * e + half));
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[e], s[t], 0, 0, 0);
             }
         }
@@ -267,9 +267,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                 {
                     int const r = 32 * t + 16 * half + 8 * w + tr;
                     i16x4 const lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_i16x4*) (values + r * kRow + 16 * swizzled(r, 4 * d + trChunk) + trByte));
+                        (lds_i16x4*) (values + r * kRow + 16 * swizzled_turned<kRow>(r, 4 * d + trChunk) + trByte));
                     i16x4 const hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_i16x4*) (values + (r + 4) * kRow + 16 * swizzled(r + 4, 4 * d + trChunk) + trByte));
+                        (lds_i16x4*) (values + (r + 4) * kRow + 16 * swizzled_turned<kRow>(r + 4, 4 * d + trChunk) + trByte));
                     i16x8 const both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                     sums.out[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bits_as<f16x8>(both), weights, sums.out[d], 0, 0, 0);
                 }
