@@ -35,37 +35,34 @@ struct CopyArgs
 template <bool FP8>
 constexpr float kTop = FP8 ? 448.f : 127.f;
 
-// Four values, already divided by their scale, as bytes.
+// Four values, divided by their scale, as bytes. None is past the largest by more than three roundings to binary32, and what is that
+// little past it is rounded to it.
 template <bool FP8>
 __device__ inline uint32_t round_codes(f32x4 y)
 {
     if constexpr (FP8)
     {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-        {
-            y[e] = __builtin_amdgcn_fmed3f(y[e], -448.f, 448.f);
-        }
         int const lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
         return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
     }
     else
     {
-        // 1.5 * 2^23 more: rounded to an integer, ties to even, in the lowest byte. What rounds to 128 is brought back before.
+        // 1.5 * 2^23 more: rounded to an integer, ties to even, in the lowest byte. Not as one operation with the product before it.
+#pragma clang fp contract(off)
         uint32_t b[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            b[e] = bits_as<uint32_t>(__builtin_amdgcn_fmed3f(y[e], -127.f, 127.f) + 12582912.f);
+            b[e] = bits_as<uint32_t>(y[e] + 12582912.f);
         }
         return low_bytes(b[0], b[1], b[2], b[3]);
     }
 }
 
-// x is a NaN or an infinity only where inverse is 0 (see scale_of): 0 * it is a NaN, which is 0 as a byte.
 template <bool FP8>
 __device__ inline uint32_t quantize_codes(f16x4 x, float inverse)
 {
+#pragma clang fp contract(off)
     f32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -124,19 +121,51 @@ __device__ inline uint32_t merge_bytes(uint32_t a, uint32_t b, uint32_t take)
     return (a & m) | (b & ~m);
 }
 
-// NV: chunks of 8 values a thread, P * d / 8 / 256 or more.
-template <int NV, bool FP8>
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+constexpr int kRowPad = 16; // rows of bytes in LDS this much further apart: eight of them, 16 bytes each, lie in different banks
+
+// 16 lanes read 8 rows of 16 bytes in LDS, `stride` apart, turned: lane i gets the bytes i of the rows, row 0 first. at: of the first row.
+__device__ inline u32x2 turned_bytes8(uint8_t* at, int stride)
+{
+    int const i = threadIdx.x & 15;
+    return bits_as<u32x2>(__builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*) (at + (i >> 1) * stride + 8 * (i & 1))));
+}
+
+// A page and head, its keys or its values, to W wavefronts, with all new rows in registers between the maximum and the quotients: NV
+// chunks of 8 values a lane. One (four pages a workgroup, side by side in the packed layouts, and no barrier) up to 512 chunks, four
+// above. Values are turned through LDS: they are written there as they come, and 16 tokens of an element are read from it by
+// transposing reads.
+template <int NV, bool FP8, int W>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CopyArgs const a)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t turned[]; // values: [d][P + 4] bytes
-    __shared__ uint32_t tops[kThreads / kWaveSize];
+    extern __shared__ __attribute__((aligned(16))) uint8_t turned[]; // values: [P][d + 16] bytes, W = 1 of two wavefronts
+    __shared__ uint32_t tops[4];
+    static_assert(W == 1 || W == 4, "four wavefronts a workgroup");
     CacheArgs const& c = a.cache;
-    int const b = blockIdx.y, h = blockIdx.z >> 1, which = blockIdx.z & 1;
-    int const P = 1 << c.shift, tid = threadIdx.x;
+    int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = W == 1 ? threadIdx.x & 63 : threadIdx.x; // of the unit
+    int const unit = W == 1 ? (int) blockIdx.z * 4 + wave : blockIdx.z, b = blockIdx.y, h = unit >> 1, which = unit & 1;
+    if (h >= c.heads)
+    {
+        return; // no barrier follows where wavefronts differ
+    }
+    constexpr int kLanes = W * kWaveSize;
+    int const P = 1 << c.shift, stride = c.d + kRowPad;
     CacheRows const r = cache_rows(c, b);
     int const begin = max(r.begin, 0), end = min(r.begin + r.n, r.len);
-    uint8_t const* const src = a.kv[which].p + 2 * (int64_t) h * a.kv[which].head;
+    Strided const from = which ? a.kv[1] : a.kv[0];
+    uint8_t const* const src = from.p + 2 * (int64_t) h * from.head;
     int const n8 = a.chunks.d;
+    uint8_t* const mine = turned + (W == 1 ? wave >> 1 : 0) * P * stride;
+    auto const meet = [] {
+        if constexpr (W == 1)
+        {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        else
+        {
+            __syncthreads();
+        }
+    };
     for (int64_t block = (begin >> c.shift) + blockIdx.x; block * P < end && block < c.maxPages; block += gridDim.x)
     {
         int const page = c.table[(int64_t) b * c.maxPages + block];
@@ -148,166 +177,255 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CopyArgs const
         float* const scaleAt = (which ? c.vScale : c.kScale) + (size_t) page * c.heads + h;
         uint8_t* const codes = (which ? c.v : c.k) + page_offset(c, page, h);
         float const old = lo > 0 ? *scaleAt : 0.f;
+        uint8_t const* const rows = src + 2 * ((int64_t) r.row0 + (first + lo - r.begin)) * from.token;
         f16x8 x[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            uint32_t const at = lane + i * kLanes, row = at / a.chunks, chunk = at - row * n8;
+            x[i] = f16x8{};
+            if ((int) row < hi - lo)
+            {
+                x[i] = *reinterpret_cast<f16x8 const*>(rows + 2 * ((int64_t) row * from.token + 8 * chunk));
+            }
+        }
         u16x2 m = {0, 0};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
         {
-            uint32_t const at = tid + i * kThreads, row = at / a.chunks, chunk = at - row * n8;
-            int const token = lo + (int) row;
-            x[i] = f16x8{};
-            if (token < hi)
-            {
-                int64_t const t = (int64_t) r.row0 + (first + token - r.begin);
-                x[i] = *reinterpret_cast<f16x8 const*>(src + 2 * (t * a.kv[which].token + 8 * chunk));
-            }
             m = max_abs(m, bits_as<u32x4>(x[i]));
         }
-        uint32_t const own = wave_max_bits(m);
-        if ((tid & 63) == 0)
+        uint32_t top = wave_max_bits(m);
+        if constexpr (W == 4)
         {
-            tops[tid >> 6] = own;
+            if ((lane & 63) == 0)
+            {
+                tops[wave] = top;
+            }
+            __syncthreads(); // and everybody has read the scale
+            top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
         }
-        __syncthreads();
-        PageScale const s = page_scale<FP8>(max(max(tops[0], tops[1]), max(tops[2], tops[3])), old);
-        if (tid == 0)
+        PageScale const s = page_scale<FP8>(top, old);
+        if (lane == 0)
         {
-            *scaleAt = s.scale; // everybody has read it
+            *scaleAt = s.scale;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
         {
-            uint32_t const at = tid + i * kThreads, row = at / a.chunks, chunk = at - row * n8;
-            int const token = lo + (int) row;
-            if (token >= hi)
-            {
-                continue;
-            }
+            uint32_t const at = lane + i * kLanes, row = at / a.chunks, chunk = at - row * n8;
             u32x2 w = {quantize_codes<FP8>(f16x4{x[i][0], x[i][1], x[i][2], x[i][3]}, s.inverse),
                 quantize_codes<FP8>(f16x4{x[i][4], x[i][5], x[i][6], x[i][7]}, s.inverse)};
-            w = s.zeros ? u32x2{0, 0} : w;
-            if (which == 0)
+            w = s.zeros ? u32x2{0, 0} : w; // also of a NaN or an infinity
+            if ((int) row < hi - lo)
             {
-                *reinterpret_cast<u32x2*>(codes + (uint32_t) token * c.d + 8 * chunk) = w;
-            }
-            else
-            {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    turned[(8 * chunk + e) * (P + 4) + token] = (uint8_t) (w[e >> 2] >> (8 * (e & 3)));
-                }
+                uint8_t* const to = which ? mine + (lo + row) * stride : codes + (lo + row) * (uint32_t) c.d;
+                *reinterpret_cast<u32x2*>(to + 8 * chunk) = w;
             }
         }
         if (which == 0)
         {
-            for (uint32_t at = tid; s.grown && at < (uint32_t) lo * n8; at += kThreads)
+            for (uint32_t at = lane; s.grown && at < (uint32_t) lo * n8; at += kLanes)
             {
                 u32x2* const p = reinterpret_cast<u32x2*>(codes) + at;
                 *p = u32x2{requantize_codes<FP8>((*p)[0], s.shrink), requantize_codes<FP8>((*p)[1], s.shrink)};
             }
-            __syncthreads(); // tops
+            if constexpr (W == 4)
+            {
+                __syncthreads(); // tops
+            }
             continue;
         }
-        __syncthreads();
-        // 16 tokens of a row at a time: the page and head are this workgroup's, so bytes on either side of the new ones are as well
-        int const groups = P >> 4, from = (s.grown ? 0 : lo) >> 4, to = (hi + 15) >> 4;
-        for (int at = tid; at < c.d * groups; at += kThreads)
+        meet();
+        // Elements 16 e .. + 15 of 16 tokens, four such blocks at a time, side by side in the page. The page and head are this
+        // wavefront's, so bytes on either side of the new ones are as well.
+        int const from16 = (s.grown ? 0 : lo) >> 4, to16 = (hi + 15) >> 4, groups = to16 - from16;
+        for (int at = lane >> 4; at < groups * (c.d >> 4); at += 4 * W)
         {
-            int const row = at >> (c.shift - 4), group = at & (groups - 1);
-            if (group < from || group >= to)
-            {
-                continue;
-            }
-            u32x4* const p = reinterpret_cast<u32x4*>(codes + (uint32_t) row * P) + group;
-            uint32_t const* const t = reinterpret_cast<uint32_t const*>(turned + row * (P + 4) + 16 * group);
+            int const e = at / groups, group = from16 + at - e * groups;
+            uint8_t* const block16 = mine + 16 * group * stride + 16 * e;
+            u32x2 const t0 = turned_bytes8(block16, stride), t1 = turned_bytes8(block16 + 8 * stride, stride);
+            u32x4* const p = reinterpret_cast<u32x4*>(codes + (uint32_t) (16 * e + (lane & 15)) * P + 16 * group);
+            u32x4 w = {t0[0], t0[1], t1[0], t1[1]};
             int const l = min(max(lo - 16 * group, 0), 16), u = min(hi - 16 * group, 16);
-            u32x4 w = {t[0], t[1], t[2], t[3]};
             if (l > 0 || u < 16)
             {
                 uint32_t const isNew = l < u ? (1u << u) - (1u << l) : 0u;
                 u32x4 const was = *p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int k = 0; k < 4; ++k)
                 {
                     // behind the new ones nothing is held: whatever lies there stays
-                    uint32_t held = was[e];
+                    uint32_t held = was[k];
                     if (s.grown)
                     {
-                        held = merge_bytes(requantize_codes<FP8>(held, s.shrink), held, ((1u << l) - 1u) >> (4 * e));
+                        held = merge_bytes(requantize_codes<FP8>(held, s.shrink), held, ((1u << l) - 1u) >> (4 * k));
                     }
-                    w[e] = merge_bytes(w[e], held, isNew >> (4 * e));
+                    w[k] = merge_bytes(w[k], held, isNew >> (4 * k));
                 }
             }
             *p = w;
         }
-        __syncthreads(); // tops and turned
+        meet();
     }
 }
 
 template <bool FP8>
-__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(CopyArgs const a)
+__device__ inline f16x4 scaled_codes(uint32_t w, float scale)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t turned[]; // values: [d][P + 4] bytes
+    f32x4 y;
+    if constexpr (FP8)
+    {
+        auto const lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+        y = {lo[0], lo[1], hi[0], hi[1]};
+    }
+    else
+    {
+        y = {i8_to_f32(w, 0), i8_to_f32(w, 1), i8_to_f32(w, 2), i8_to_f32(w, 3)};
+    }
+    y *= scale;
+    f16x2 const lo = __builtin_convertvector(f32x2{y[0], y[1]}, f16x2), hi = __builtin_convertvector(f32x2{y[2], y[3]}, f16x2);
+    return {lo[0], lo[1], hi[0], hi[1]};
+}
+
+template <bool FP8>
+__device__ inline void store_scaled(uint8_t* to, u32x4 const& w, float scale)
+{
+    f16x4 y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+    {
+        y[k] = scaled_codes<FP8>(w[k], scale);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k += 2)
+    {
+        *reinterpret_cast<f16x8*>(to + 8 * k) = __builtin_shufflevector(y[k], y[k + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// The way back: 4 KB of a page and head a wavefront, tokens of its keys as they lie, or elements of its values, turned through LDS. Four of
+// them a workgroup.
+constexpr int kReadBytes = 4096;
+
+struct ReadArgs
+{
+    CopyArgs copy;
+    int elements; // of a part of the values: a multiple of 16
+    FastDiv parts;
+    int tokens; // of a part of the keys
+    FastDiv pieces; // d / 16
+};
+
+template <bool FP8>
+__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(ReadArgs const ra)
+{
+    constexpr int NV = kReadBytes / 16 / kWaveSize;
+    extern __shared__ __attribute__((aligned(16))) uint8_t turned[]; // four wavefronts' values: [elements][P + 16] bytes each
+    CopyArgs const& a = ra.copy;
     CacheArgs const& c = a.cache;
-    int const b = blockIdx.y, h = blockIdx.z >> 1, which = blockIdx.z & 1;
-    int const P = 1 << c.shift, tid = threadIdx.x;
+    int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int const unit = (int) blockIdx.z * 4 + wave, b = blockIdx.y; // key head, keys or values, part
+    int const pair = (int) ((uint32_t) unit / ra.parts), part = unit - pair * (int) ra.parts.d, h = pair >> 1, which = pair & 1;
+    if (h >= c.heads)
+    {
+        return; // no barrier follows
+    }
+    int const P = 1 << c.shift, stride = P + kRowPad, n16 = ra.pieces.d;
     CacheRows const r = cache_rows(c, b);
-    uint8_t* const out = a.kv[which].p + 2 * (int64_t) h * a.kv[which].head;
-    int const n8 = a.chunks.d;
+    Strided const into = which ? a.kv[1] : a.kv[0];
+    uint8_t* const out = into.p + 2 * (int64_t) h * into.head;
+    uint8_t* const mine = turned + wave * ra.elements * stride;
     // by position, so that rows without a place in the table get their zeros as well
     int64_t const begin = r.begin, end = begin + r.n;
     for (int64_t block = (begin >> c.shift) + blockIdx.x; block * P < end; block += gridDim.x)
     {
         int const page = block >= 0 && block < c.maxPages ? c.table[(int64_t) b * c.maxPages + block] : -1;
         int64_t const first = block * P;
-        int const lo = (int) max(begin - first, (int64_t) 0), hi = (int) min(end - first, (int64_t) P);
+        int lo = (int) max(begin - first, (int64_t) 0), hi = (int) min(end - first, (int64_t) P);
         bool const there = (uint32_t) page < (uint32_t) c.pages;
-        int const at0 = there ? page : 0;
-        float const scale = there ? (which ? c.vScale : c.kScale)[(size_t) at0 * c.heads + h] : 0.f;
-        uint8_t const* const codes = (which ? c.v : c.k) + page_offset(c, at0, h);
-        if (which && there)
+        int const sound = there ? page : 0;
+        float const scale = there ? (which ? c.vScale : c.kScale)[(size_t) sound * c.heads + h] : 0.f;
+        uint8_t const* codes = (which ? c.v : c.k) + page_offset(c, sound, h);
+        uint8_t* const rows = out + 2 * (r.row0 + (first - begin)) * into.token; // of the page's first token, which may not be one of the call's
+        if (which == 0 || !there)
         {
-            int const groups = P >> 4, from = lo >> 4, to = (hi + 15) >> 4;
-            for (int at = tid; at < c.d * groups; at += kThreads)
+            lo = max(lo, part * ra.tokens);
+            hi = min(hi, (part + 1) * ra.tokens);
+            for (int from = lo * n16; from < hi * n16; from += NV * kWaveSize)
             {
-                int const row = at >> (c.shift - 4), group = at & (groups - 1);
-                if (group >= from && group < to)
+                u32x4 w[NV];
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
                 {
-                    u32x4 const w = *(reinterpret_cast<u32x4 const*>(codes + (uint32_t) row * P) + group);
-                    uint32_t* const t = reinterpret_cast<uint32_t*>(turned + row * (P + 4) + 16 * group);
-                    t[0] = w[0], t[1] = w[1], t[2] = w[2], t[3] = w[3];
+                    int const at = from + lane + i * kWaveSize;
+                    w[i] = u32x4{0, 0, 0, 0};
+                    if (there && at < hi * n16)
+                    {
+                        w[i] = reinterpret_cast<u32x4 const*>(codes)[at];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                {
+                    int const at = from + lane + i * kWaveSize, token = (int) ((uint32_t) at / ra.pieces), piece = at - token * n16;
+                    if (at < hi * n16)
+                    {
+                        store_scaled<FP8>(rows + 2 * ((int64_t) token * into.token + 16 * piece), w[i], scale);
+                    }
                 }
             }
-            __syncthreads();
+            continue;
         }
-        for (uint32_t at = tid; at < (uint32_t) (hi - lo) * n8; at += kThreads)
+        int const groups = P >> 4, from16 = lo >> 4, to16 = (hi + 15) >> 4;
+        int const e0 = part * ra.elements, elements = min(ra.elements, c.d - e0);
+        codes += (uint32_t) e0 * P;
+        u32x4 w[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
         {
-            uint32_t const row = at / a.chunks, chunk = at - row * n8;
-            int const token = lo + (int) row;
-            u32x2 w = {0, 0};
-            if (there && which == 0)
+            int const at = lane + i * kWaveSize, group = at & (groups - 1);
+            w[i] = u32x4{0, 0, 0, 0};
+            if (at < elements * groups && group >= from16 && group < to16)
             {
-                w = *reinterpret_cast<u32x2 const*>(codes + (uint32_t) token * c.d + 8 * chunk);
+                w[i] = reinterpret_cast<u32x4 const*>(codes)[at];
             }
-            else if (there)
-            {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    w[e >> 2] |= (uint32_t) turned[(8 * chunk + e) * (P + 4) + token] << (8 * (e & 3));
-                }
-            }
-            f16x8 const v = code_values8<FP8>(w[0], w[1]);
-            f16x8 y;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                y[e] = (f16) ((float) v[e] * scale);
-            }
-            *reinterpret_cast<f16x8*>(out + 2 * ((r.row0 + (first + token - begin)) * a.kv[which].token + 8 * chunk)) = y;
         }
-        __syncthreads(); // turned
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            int const at = lane + i * kWaveSize;
+            if (at < elements * groups)
+            {
+                *reinterpret_cast<u32x4*>(mine + (at >> (c.shift - 4)) * stride + 16 * (at & (groups - 1))) = w[i];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // elements 16 e .. + 15 of 16 tokens, four such blocks at a time, side by side in the rows
+        int const blocks = elements >> 4;
+        int e = lane >> 4, token16 = from16;
+        while (e >= blocks)
+        {
+            e -= blocks;
+            ++token16;
+        }
+        while (token16 < to16)
+        {
+            int const token = 16 * token16 + (lane & 15);
+            uint8_t* const block16 = mine + 16 * e * stride + 16 * token16;
+            u32x2 const t0 = turned_bytes8(block16, stride), t1 = turned_bytes8(block16 + 8 * stride, stride);
+            if (token >= lo && token < hi)
+            {
+                store_scaled<FP8>(rows + 2 * ((int64_t) token * into.token + e0 + 16 * e), u32x4{t0[0], t0[1], t1[0], t1[1]}, scale);
+            }
+            e += 4;
+            while (e >= blocks)
+            {
+                e -= blocks;
+                ++token16;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -346,10 +464,6 @@ dim3 copy_grid(trtamd_kv_cache const& c)
     return dim3((unsigned) std::min<int64_t>(touched, 65536), (unsigned) c.B, (unsigned) c.kv_heads * 2);
 }
 
-size_t turned_bytes(trtamd_kv_cache const& c)
-{
-    return (size_t) c.d * (c.page_tokens + 4);
-}
 
 } // namespace
 
@@ -381,9 +495,9 @@ int cache_check(char const* what, trtamd_kv_cache const& c)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: max_pages=%d pages=%d", what, c.max_pages, c.pages);
     }
-    if (c.B > 65535 || c.kv_heads > 32767)
+    if (c.B > 65535 || c.kv_heads > 16383)
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d kv_heads=%d (at most 65535 and 32767)", what, c.B, c.kv_heads);
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d kv_heads=%d (at most 65535 and 16383)", what, c.B, c.kv_heads);
     }
     if ((int64_t) c.pages * c.kv_heads >= (int64_t) 1 << 31)
     {
@@ -443,19 +557,27 @@ extern "C" int trtamd_kv_cache_write(trtamd_stream_t stream, trtamd_kv_cache_wri
         {{reinterpret_cast<uint8_t*>(const_cast<trtamd_half_t*>(p.k)), p.k_token_stride, p.k_head_stride},
             {reinterpret_cast<uint8_t*>(const_cast<trtamd_half_t*>(p.v)), p.v_token_stride, p.v_head_stride}},
         fast_div((uint32_t) c.d / 8)};
-    int const tokens = std::min(c.page_tokens, std::min(c.max_tokens, c.T));
-    int const perThread = ceil_div(tokens * c.d / 8, kThreads);
-    auto const run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, copy_grid(c), dim3(kThreads), turned_bytes(c), as_stream(stream), a);
+    // of a page at most
+    int const chunks = std::min(c.page_tokens, std::min(c.max_tokens, c.T)) * c.d / 8;
+    dim3 const pages = copy_grid(c);
+    size_t const lds = (size_t) c.page_tokens * (c.d + kRowPad); // values of a page
+    auto const run = [&](auto kernel, int wavefronts) {
+        bool const one = wavefronts == 1;
+        hipLaunchKernelGGL(kernel, dim3(pages.x, pages.y, one ? ceil_div(pages.z, 4u) : pages.z), dim3(kThreads), one ? 2 * lds : lds, as_stream(stream), a);
         return check_launch("kv_cache_write_kernel");
     };
     auto const by_size = [&](auto type) {
         constexpr bool F = decltype(type)::value;
-        return perThread <= 1 ? run(kv_cache_write_kernel<1, F>)
-            : perThread <= 2  ? run(kv_cache_write_kernel<2, F>)
-            : perThread <= 4  ? run(kv_cache_write_kernel<4, F>)
-            : perThread <= 8  ? run(kv_cache_write_kernel<8, F>)
-                              : run(kv_cache_write_kernel<16, F>);
+        if (chunks > 8 * kWaveSize || 2 * lds > 65536)
+        {
+            return chunks <= 16 * kWaveSize ? run(kv_cache_write_kernel<4, F, 4>, 4)
+                : chunks <= 32 * kWaveSize  ? run(kv_cache_write_kernel<8, F, 4>, 4)
+                                            : run(kv_cache_write_kernel<16, F, 4>, 4);
+        }
+        return chunks <= 1 * kWaveSize ? run(kv_cache_write_kernel<1, F, 1>, 1)
+            : chunks <= 2 * kWaveSize  ? run(kv_cache_write_kernel<2, F, 1>, 1)
+            : chunks <= 4 * kWaveSize  ? run(kv_cache_write_kernel<4, F, 1>, 1)
+                                       : run(kv_cache_write_kernel<8, F, 1>, 1);
     };
     return c.data_type == kCacheFp8 ? by_size(std::true_type{}) : by_size(std::false_type{});
 }
@@ -480,8 +602,12 @@ extern "C" int trtamd_kv_cache_read(trtamd_stream_t stream, trtamd_kv_cache_read
         {{reinterpret_cast<uint8_t*>(p.k), p.k_token_stride, p.k_head_stride},
             {reinterpret_cast<uint8_t*>(p.v), p.v_token_stride, p.v_head_stride}},
         fast_div((uint32_t) c.d / 8)};
+    int const elements = std::min(c.d, kReadBytes / c.page_tokens), parts = ceil_div(c.d, elements);
+    ReadArgs const ra = {a, elements, fast_div((uint32_t) parts), ceil_div(c.page_tokens, parts), fast_div((uint32_t) c.d / 16)};
+    dim3 const pages = copy_grid(c);
     auto const run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, copy_grid(c), dim3(kThreads), turned_bytes(c), as_stream(stream), a);
+        hipLaunchKernelGGL(kernel, dim3(pages.x, pages.y, (unsigned) ceil_div((int64_t) pages.z * parts, (int64_t) 4)), dim3(kThreads),
+            4 * (size_t) elements * (c.page_tokens + kRowPad), as_stream(stream), ra);
         return check_launch("kv_cache_read_kernel");
     };
     return c.data_type == kCacheFp8 ? run(kv_cache_read_kernel<true>) : run(kv_cache_read_kernel<false>);

@@ -59,7 +59,7 @@ def test_cache_refused_everywhere(api, change, word):
 
 @pytest.mark.parametrize("change,word", [
     (dict(rows_k=0), "null"), (dict(rows_v=0), "null"), (dict(rows_k=A + 2), "aligned"), (dict(rows_v=A + 8), "aligned"),
-    (dict(rows_k_token_stride=100), "strides"), (dict(rows_v_head_stride=-8), "strides"), (dict(kv_heads=32768), "32767"), (dict(pages=1 << 30), "2^31")])
+    (dict(rows_k_token_stride=100), "strides"), (dict(rows_v_head_stride=-8), "strides"), (dict(kv_heads=16384), "16383"), (dict(pages=1 << 30), "2^31")])
 def test_copies_refuse(api, change, word):
     refused(api, api.kv_cache_write(None, copied(capi.KvCacheWriteParams, **change)), word)
     refused(api, api.kv_cache_read(None, copied(capi.KvCacheReadParams, **change)), word)
