@@ -156,24 +156,27 @@ int by_head(int d, F&& f)
     }
 }
 
-// Scores of keys that a row does not see become -infinity; keys key0 + 16 half + v % 16 + 32 (v / 16) in s[v / 16][v % 16].
-__device__ inline void hide(f32x16 (&s)[2], Seen const& seen, int key0)
+// Ones in the lowest n bits of 16.
+__device__ inline uint32_t low_ones(int n)
 {
-    // behind the sinks one unsigned comparison has both ends
-    uint32_t const from = (uint32_t) (key0 - seen.lo), width = (uint32_t) max(seen.hi - seen.lo, 0);
-    if (key0 >= seen.sinks)
-    {
+    return (1u << min(max(n, 0), 16)) - 1u;
+}
+
+// Scores of keys that a row does not see become -infinity; keys key0 + 32 t + v in s[t][v], of which the first there[t] are there. By bits
+// of a mask: two instructions a score and no scalar registers, where comparisons take three and a pair of them each.
+__device__ inline void hide(f32x16 (&s)[2], Seen const& seen, int key0, int there0, int there1)
+{
 #pragma unroll
-        for (int v = 0; v < 32; ++v)
+    for (int t = 0; t < 2; ++t)
+    {
+        int const from = key0 + 32 * t;
+        uint32_t const mask = ((low_ones(seen.hi - from) & ~low_ones(seen.lo - from)) | low_ones(min(seen.sinks, seen.hi) - from)) & low_ones(t ? there1 : there0);
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
         {
-            s[v >> 4][v & 15] = from + (uint32_t) (32 * (v >> 4) + (v & 15)) < width ? s[v >> 4][v & 15] : -__builtin_inff();
+            uint32_t const keep = (uint32_t) __builtin_amdgcn_sbfe((int) mask, v, 1);
+            s[t][v] = bits_as<float>((bits_as<uint32_t>(s[t][v]) & keep) | (0xff800000u & ~keep));
         }
-        return;
-    }
-#pragma unroll
-    for (int v = 0; v < 32; ++v)
-    {
-        s[v >> 4][v & 15] = seen(key0 + 32 * (v >> 4) + (v & 15)) ? s[v >> 4][v & 15] : -__builtin_inff();
     }
 }
 

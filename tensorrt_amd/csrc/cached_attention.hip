@@ -982,19 +982,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                         by[t] = 1.f;
                         add[t] = 0.f;
                     }
-                    hide(s, seen, key0 + 16 * half);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                    {
-                        if (__ballot(there[t] < 16) != 0)
-                        {
-#pragma unroll
-                            for (int v = 0; v < 16; ++v)
-                            {
-                                s[t][v] = v < there[t] ? s[t][v] : -__builtin_inff();
-                            }
-                        }
-                    }
+                    hide(s, seen, key0 + 16 * half, there[0], there[1]);
                 }
                 float mx = -__builtin_inff();
 #pragma unroll

@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
         }
         if (!(key0 + kChunkKeys <= least.hi && (key0 >= most.lo || key0 + kChunkKeys <= a.sinks)))
         {
-            hide(s, seen, key0 + 16 * half);
+            hide(s, seen, key0 + 16 * half, 16, 16);
         }
         float mx = -__builtin_inff();
 #pragma unroll
