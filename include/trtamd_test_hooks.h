@@ -53,6 +53,11 @@ TRTAMD_API int64_t trtamd_test_fmha_route(int32_t data_type, trtamd_fmha_params 
  * head, bit 16 stores past the caches.  -1: parameters that are refused, or without a launch. */
 TRTAMD_API int trtamd_test_qk_norm_rotary_route(int32_t data_type, trtamd_qk_norm_rotary_params const* params);
 
+/* What trtamd_kv_cache_attention launches for these parameters' sizes. Bits 0-3: wavefronts of a workgroup that takes a sequence and
+ * key head with up to 16 rows, 0 where there is no such launch; bit 4: equal stretches of all sequences instead, bit 5: each of one head;
+ * bit 6: tiles of more rows, and from bit 8 on how many parts their keys are in at most.  -1: sizes that are refused. */
+TRTAMD_API int64_t trtamd_test_kv_cache_attention_route(trtamd_kv_cache_attention_params const* params);
+
 #ifdef __cplusplus
 }
 #endif

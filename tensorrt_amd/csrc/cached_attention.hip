@@ -13,6 +13,7 @@
 #include "attention_rows.hpp"
 #include "host_utils.hpp"
 #include "kv_cache.hpp"
+#include "trtamd_test_hooks.h"
 
 #include <algorithm>
 #include <cmath>
@@ -523,8 +524,9 @@ __device__ inline Stretch stretch_of_workgroup(CacheArgs const& c, AttentionArgs
     int const total = wave_sum_i32(n) * c.heads;
     Stretch s{};
     s.none = true;
-    // a chunk a wavefront at least; ALIGNED: so that the stretches' number with one more for each head is no more than the workgroups'
-    s.share = max((total + wgs - 1) / (ALIGNED ? max(wgs - B * c.heads, 1) : wgs), kStretchWaves);
+    // A chunk a wavefront at least, behind the places in front of a head's first one: every stretch has a chunk. ALIGNED: so that the
+    // stretches' number with one more for each head is no more than the workgroups'.
+    s.share = max((total + wgs - 1) / (ALIGNED ? max(wgs - B * c.heads, 1) : wgs), kStretchWaves + (ALIGNED ? 0 : kHeadCost));
     int const target = ALIGNED ? wg : wg * s.share; // stretches, or chunks, before this one
     if (!ALIGNED && target >= total)
     {
@@ -1192,9 +1194,11 @@ Plan plan_of(trtamd_kv_cache_attention_params const& p)
             plan.aligned = 4 * units <= resident;
         }
     }
-    // More rows: whole where there are tiles enough for two a CU.
-    int64_t const tiles = ceil_div((int64_t) c.T * group, (int64_t) kTileRows) * c.kv_heads;
-    share_out(tiles >= 2 * cus ? most : std::max<int64_t>(ceil_div(tiles * chunks, 2 * cus), 8), most, plan.manySpan, plan.manySplits);
+    // More rows: whole keys where there are tiles enough for two a CU, otherwise parts of 8 chunks or more that make as many; of keys past
+    // max_length no more than four times as many, since their sums have a place each in the workspace.
+    int64_t const tiles = ceil_div((int64_t) c.T * group, (int64_t) kTileRows) * c.kv_heads, parts = ceil_div(2 * cus, std::max<int64_t>(tiles, 1));
+    int64_t const span = std::max(std::max<int64_t>(ceil_div(tiles * chunks, 2 * cus), 8), ceil_div(most, 4 * parts));
+    share_out(tiles >= 2 * cus ? most : span, most, plan.manySpan, plan.manySplits);
     return plan;
 }
 
@@ -1237,6 +1241,14 @@ int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
         return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: T * q_heads of 2^30 or more", what);
     }
     return TRTAMD_STATUS_SUCCESS;
+}
+
+// What plan_of relies on.
+bool sizes_are_sound(trtamd_kv_cache_attention_params const& p)
+{
+    trtamd_kv_cache const& c = p.cache;
+    return c.kv_heads > 0 && p.q_heads > 0 && p.q_heads % c.kv_heads == 0 && c.page_tokens > 0 && c.d > 0 && c.max_pages > 0 && c.B > 0 && c.T > 0
+        && c.max_tokens > 0 && p.window >= 0 && p.sinks >= 0 && p.max_length >= 0;
 }
 
 bool nothing(trtamd_kv_cache const& c)
@@ -1340,18 +1352,18 @@ using namespace trtamd;
 
 extern "C" size_t trtamd_kv_cache_attention_workspace_size(trtamd_kv_cache_attention_params const* params)
 {
-    if (params == nullptr)
+    return params == nullptr || !sizes_are_sound(*params) ? 0 : workspace_of(*params, plan_of(*params));
+}
+
+extern "C" int64_t trtamd_test_kv_cache_attention_route(trtamd_kv_cache_attention_params const* params)
+{
+    if (params == nullptr || !sizes_are_sound(*params))
     {
-        return 0;
+        return -1;
     }
-    trtamd_kv_cache_attention_params const& p = *params;
-    trtamd_kv_cache const& c = p.cache;
-    if (c.kv_heads <= 0 || p.q_heads <= 0 || p.q_heads % c.kv_heads != 0 || c.page_tokens <= 0 || c.d <= 0 || c.max_pages <= 0 || c.B <= 0
-        || c.T <= 0 || c.max_tokens <= 0 || p.window < 0 || p.sinks < 0 || p.max_length < 0)
-    {
-        return 0;
-    }
-    return workspace_of(p, plan_of(p));
+    Plan const p = plan_of(*params);
+    return (p.few && !p.stretches ? p.fewWaves : 0) | (p.stretches ? 16 : 0) | (p.stretches && p.aligned ? 32 : 0) | (p.many ? 64 : 0)
+        | (int64_t) (p.many ? p.manySplits : 0) << 8;
 }
 
 extern "C" int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache_attention_params const* params)

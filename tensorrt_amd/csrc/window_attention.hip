@@ -105,7 +105,7 @@ __device__ void one_row(WindowArgs const& a, int first, int token, int head, int
 }
 
 template <int KS /* 16 of the head's values */>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void window_attention_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 4 : KS <= 8 ? 2 : 1))) void window_attention_kernel(
     WindowArgs const a)
 {
     constexpr int DP = padded_head(KS);

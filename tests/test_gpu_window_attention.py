@@ -151,3 +151,61 @@ def test_agrees_with_the_fused_attention(api):
     api.check(api.fused_mha_run(stream(), 1, C.byref(f)))
     sync()
     assert_fp_close(got, host(out), what="the two attentions")
+
+
+def test_captured(api):
+    """A graph follows the lengths, between eager calls of another problem; rows behind the last sequence stay."""
+    import torch
+    p, other = (Problem([150, 90, 40], 4, 2, 96, seed=s) for s in (1, 2))
+    T = len(p.q)
+    q, k, v, out, dcu = dev(p.q), dev(p.k), dev(p.v), dev_empty(p.q.shape, np.float16, fill=-7), dev(p.cu)
+    a = params(q, k, v, out, dcu, 3, T, p.scale, 20, 5, 3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        api.check(api.window_attention(stream(), C.byref(a)))
+    for lens in ([150, 90, 40], [1, 0, 200], [100, 100, 80], [0, 0, 0]):
+        p.cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        dcu.copy_(dev(p.cu))
+        out.fill_(-7)
+        graph.replay()
+        sync()
+        got = host(out)
+        assert (got[p.cu[-1]:] == -7).all()
+        p.check(got, 20, 5, 3, sample=10)
+        other.check(other.run(api, 20, 5, 3), 20, 5, 3, sample=5)
+
+
+def test_two_streams(api):
+    import torch
+    problems = [Problem([700, 300], 4, 4, 64, seed=s) for s in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in problems]
+    held = []
+    for p in problems:
+        q, k, v, out, dcu = dev(p.q), dev(p.k), dev(p.v), dev_empty(p.q.shape, np.float16, fill=-7), dev(p.cu)
+        held.append((q, k, v, out, dcu, params(q, k, v, out, dcu, 2, 700, p.scale, 100, 100, 0)))
+    sync()
+    for _ in range(3):
+        for h, s in zip(held, streams):
+            api.check(api.window_attention(s.cuda_stream, C.byref(h[5])))
+    sync()
+    for p, h in zip(problems, held):
+        p.check(host(h[3]), 100, 100, 0, sample=20)
+
+
+@pytest.mark.parametrize("strides", [(1 << 25) + 64, 1 << 20])
+def test_far_rows(api, strides):
+    """Rows so far apart that a chunk passes 32-bit offsets, or does not."""
+    import torch
+    d, n = 64, 70
+    r = rng(3)
+    x = r.standard_normal((3, n, 1, d)).astype(np.float16)
+    far = torch.empty((n * strides,), dtype=torch.float16, device="cuda")
+    rows = [torch.as_strided(far, (n, 1, d), (strides, d, 1), i * d) for i in range(3)]
+    for t, y in zip(rows, x):
+        t.copy_(dev(y))
+    out, dcu = dev_empty((n, 1, d), np.float16, fill=-7), dev(np.array([0, n], np.int32))
+    p = Problem([n], 1, 1, d)
+    p.q, p.k, p.v = x
+    api.check(api.window_attention(stream(), C.byref(params(*rows, out, dcu, 1, n, p.scale, 9, 9, 2))))
+    sync()
+    p.check(host(out), 9, 9, 2)
