@@ -280,16 +280,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
     {
         return;
     }
-    // Whatever is not finite leaves a NaN here, and an infinity of a value that is not seen a NaN in its row.
-    float odd = sums.sum * 0.f;
+    float const total = reduce_step<32>(sums.sum, [](float x, float y) { return x + y; });
+    float const inverse = total == 0.f ? 0.f : 1.f / total;
+    f16x4 y[4 * DV];
+    // Whatever is not finite leaves a NaN here: an infinity of a value that is not seen leaves one in its row.
+    float odd = inverse * 0.f;
 #pragma unroll
-    for (int d = 0; d < DV; ++d)
+    for (int i = 0; i < 4 * DV; ++i)
     {
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-        {
-            odd = 32 * d + 2 * (v & 12) + 4 * half + (v & 3) < a.d ? fmaf(sums.out[d][v], 0.f, odd) : odd;
-        }
+        f32x16 const& o = sums.out[i >> 2];
+        int const v = 4 * (i & 3);
+        f16x2 const lo = __builtin_convertvector(f32x2{o[v] * inverse, o[v + 1] * inverse}, f16x2);
+        f16x2 const hi = __builtin_convertvector(f32x2{o[v + 2] * inverse, o[v + 3] * inverse}, f16x2);
+        odd = __builtin_amdgcn_fdot2(lo, f16x2{}, __builtin_amdgcn_fdot2(hi, f16x2{}, odd, false), false);
+        y[i] = f16x4{lo[0], lo[1], hi[0], hi[1]};
     }
     if (__ballot(odd != 0.f) != 0)
     {
@@ -300,25 +304,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
         }
         return;
     }
-    float const total = reduce_step<32>(sums.sum, [](float x, float y) { return x + y; });
     if (wRow + lq >= rowEnd)
     {
         return;
     }
-    float const inverse = total == 0.f ? 0.f : 1.f / total;
-    uint8_t* const to = a.out + (int64_t) (first + token) * a.outToken + (int64_t) head * a.outHead;
+    uint8_t* const to = a.out + (int64_t) (first + token) * a.outToken + (int64_t) head * a.outHead + 8 * half;
 #pragma unroll
-    for (int d = 0; d < DV; ++d)
+    for (int i = 0; i < 4 * DV; ++i)
     {
-#pragma unroll
-        for (int v = 0; v < 16; v += 4)
+        if (8 * i + 4 * half < a.d)
         {
-            int const e = 32 * d + 2 * v + 4 * half;
-            if (e < a.d)
-            {
-                *reinterpret_cast<f16x4*>(to + 2 * e) = f16x4{(f16) (sums.out[d][v] * inverse), (f16) (sums.out[d][v + 1] * inverse),
-                    (f16) (sums.out[d][v + 2] * inverse), (f16) (sums.out[d][v + 3] * inverse)};
-            }
+            *reinterpret_cast<f16x4*>(to + 16 * i) = y[i];
         }
     }
 }
