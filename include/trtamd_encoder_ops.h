@@ -221,7 +221,7 @@ typedef struct trtamd_kv_cache
     int32_t kv_heads;
     int32_t d;                 /* a multiple of 16, at most 256 */
     int32_t B;                 /* sequences, at most 65535 */
-    int32_t max_pages;         /* entries of a sequence in page_table */
+    int32_t max_pages;         /* entries of a sequence in page_table; max_pages * page_tokens at most 2^30 */
     int32_t max_tokens;        /* rows of a sequence in the call, or more */
     int32_t T;                 /* rows of the call's tensors */
 } trtamd_kv_cache;
@@ -248,7 +248,8 @@ typedef struct trtamd_kv_cache_write_params
 
 TRTAMD_API int trtamd_kv_cache_write(trtamd_stream_t stream, trtamd_kv_cache_write_params const* params);
 
-/* The call's rows from the cache, binary16(byte * scale): the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence. */
+/* The call's rows from the cache, binary16(byte * scale): the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each sequence.  (A value
+ * within half a step of the largest binary16 can come back as an infinity; attention does not round it.) */
 typedef struct trtamd_kv_cache_read_params
 {
     trtamd_kv_cache cache;

@@ -56,6 +56,7 @@ __device__ inline Chunks chunks_of(int lo, int hi, int sinks)
     c.first = max(c.sinkChunks, lo / kChunkKeys);
     int const last = hi > lo ? (int) (((int64_t) hi + kChunkKeys - 1) / kChunkKeys) : 0;
     c.total = c.sinkChunks + max(last - c.first, 0);
+    c.first = c.total > 0 ? c.first : 0; // a place that is there, for rows that see nothing
     return c;
 }
 

@@ -499,6 +499,10 @@ int cache_check(char const* what, trtamd_kv_cache const& c)
     {
         return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d kv_heads=%d (at most 65535 and 16383)", what, c.B, c.kv_heads);
     }
+    if ((int64_t) c.max_pages * c.page_tokens > (int64_t) 1 << 30)
+    {
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: max_pages * page_tokens of more than 2^30", what);
+    }
     if ((int64_t) c.pages * c.kv_heads >= (int64_t) 1 << 31)
     {
         return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: pages * kv_heads of 2^31 or more", what);

@@ -37,14 +37,13 @@ struct CacheRows
 
 __device__ inline CacheRows cache_rows(CacheArgs const& c, int b)
 {
-    int const lo = max(c.cu[b], 0), hi = min(c.cu[b + 1], c.T);
-    int const all = max(c.cu[b + 1] - lo, 0);
-    int const length = max(c.lengths[b], 0);
+    int const lo = min(max(c.cu[b], 0), c.T), next = max(c.cu[b + 1], lo), hi = min(next, c.T);
+    int const all = next - lo, length = max(c.lengths[b], 0);
     CacheRows r;
     r.row0 = lo;
-    r.n = min(max(hi - lo, 0), c.maxTokens);
+    r.n = min(hi - lo, c.maxTokens);
     r.begin = length - all;
-    r.len = (int) min((int64_t) length, (int64_t) c.maxPages << c.shift);
+    r.len = min(length, c.maxPages << c.shift);
     return r;
 }
 

@@ -116,8 +116,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
     constexpr int NL = kChunkKeys / kRowsPerLoad / kWaves;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int const b = blockIdx.z;
-    int const first = max(a.cu[b], 0);
-    int const n = min(max(min(a.cu[b + 1], a.T) - first, 0), a.maxTokens);
+    int const first = min(max(a.cu[b], 0), a.T);
+    int const n = min(min(max(a.cu[b + 1], first), a.T) - first, a.maxTokens);
     int const group = a.group.d;
     int const rows = n * group;
     int const fromEnd = (int) (blockIdx.x / a.kvHeads), h = (int) (blockIdx.x - fromEnd * a.kvHeads.d);

@@ -46,7 +46,7 @@ CACHE = [
     (dict(d=0), "d=0"), (dict(d=72), "d=72"), (dict(d=272), "d=272"), (dict(d=-16), "d=-16"), (dict(kv_heads=0), "kv_heads=0"),
     (dict(B=-1), "B=-1"), (dict(T=-1), "T=-1"), (dict(max_tokens=-1), "max_tokens=-1"), (dict(max_pages=-1), "max_pages=-1"),
     (dict(max_pages=0), "max_pages=0"), (dict(pages=0), "pages=0"), (dict(B=65536), "65535"),
-    (dict(k_scale=0), "null"), (dict(v_scale=0), "null"), (dict(page_table=0), "null"), (dict(lengths=0), "null"),
+    (dict(max_pages=(1 << 26) + 1), "2^30"), (dict(pages=1 << 30), "2^31"), (dict(k_scale=0), "null"), (dict(v_scale=0), "null"), (dict(page_table=0), "null"), (dict(lengths=0), "null"),
     (dict(cu_seqlens=0), "null"), (dict(k_scale=A + 2), "aligned"), (dict(page_table=A + 1), "aligned"), (dict(lengths=A + 2), "aligned")]
 
 

@@ -268,6 +268,28 @@ def test_rows_left_out_stay(api, more):
     check_attention(cache, cu, q, got, 0.125, **more)
 
 
+@pytest.mark.parametrize("lengths,cu,T", [
+    ([2 ** 31 - 1, 100, -5], [0, 2, 4, 6], 6), ([64, 64, 64], [3, 1, 6, 2], 6), ([64, 64, 64], [-7, 2, 2 ** 31 - 1, 5], 6),
+    ([2 ** 31 - 1] * 3, [0, 20, 40, 60], 60), ([64, 2 ** 30, 33], [50, 10, 45, 60], 60)])
+def test_tables_of_no_sense(api, lengths, cu, T):
+    """Lengths and rows that no cache has: everything stays within the call's tensors and the pool, and what is out of them stays."""
+    cache = filled(api, "int8", 16, 2, 64, [64, 64, 64])
+    cache.lengths = np.array(lengths, np.int32)
+    cache.dlengths.copy_(dev(cache.lengths))
+    kv, q = new_rows(cache.r, T, 2, 64), cache.r.standard_normal((T, 4, 64)).astype(np.float16)
+    n = max(1, min(T, 40))
+    for window in (0, 10):
+        out = attend(api, cache, np.array(cu), q, 0.125, window=window, T=T, max_tokens=n)
+        assert np.isfinite(out).all()
+    k, v = read(api, cache, np.array(cu), T=T, max_tokens=n)
+    assert (k[T] == -7).all() and (v[T] == -7).all()
+    c, keep = cache.described(cu, T=T, max_tokens=n)
+    t = dev(kv)
+    s = dict(k_token_stride=256, k_head_stride=128, v_token_stride=256, v_head_stride=128)
+    api.check(api.kv_cache_write(stream(), C.byref(capi.KvCacheWriteParams(cache=c, k=ptr(t), v=ptr(t) + 128, **s))))
+    sync()
+
+
 @pytest.mark.parametrize("dtype", ["int8", "fp8"])
 def test_scales_far_apart(api, dtype):
     """Pages whose values are 2^20 times others': the weights keep their digits whatever the scales are; a page of zeros counts too."""
