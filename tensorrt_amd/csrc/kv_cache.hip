@@ -134,7 +134,8 @@ __device__ inline u32x2 turned_bytes8(uint8_t* at, int stride)
 // A page and head, its keys or its values, to W wavefronts, with all new rows in registers between the maximum and the quotients: NV
 // chunks of 8 values a lane. One (four pages a workgroup, side by side in the packed layouts, and no barrier) up to 512 chunks, four
 // above. Values are turned through LDS: they are written there as they come, and 16 tokens of an element are read from it by
-// transposing reads.
+// transposing reads. 16621 tokens of 16 heads of 64 in pages of 32: 22.5 us (102 MB, 4.5 TB/s; vector instructions 55 % of the cycles); a
+// workgroup a page, values turned byte by byte, 48. Pages of 64 x 128 to one wavefront each 19.7, to four 16.6. One token 3.6, a launch.
 template <int NV, bool FP8, int W>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CopyArgs const a)
 {
@@ -305,7 +306,7 @@ __device__ inline void store_scaled(uint8_t* to, u32x4 const& w, float scale)
 }
 
 // The way back: 4 KB of a page and head a wavefront, tokens of its keys as they lie, or elements of its values, turned through LDS. Four of
-// them a workgroup.
+// them a workgroup. The same 16621 tokens 20.7 us (4.9 TB/s); a workgroup a page 45.
 constexpr int kReadBytes = 4096;
 
 struct ReadArgs

@@ -6,6 +6,11 @@
 // 128 rows of a key head a workgroup, (token, query head) with the heads of a group side by side, 32 a wavefront
 // (attention_rows.hpp). Keys and values come in chunks of 64 straight into LDS, in two slots; of the keys in front of a tile's
 // windows only the chunks with sinks. Values lie in LDS as in memory and become the second product's operand by transposing reads.
+// What bounds it: long windows the matrix and the vector instructions (34 and 35 % of the cycles, in turns), short ones the trips to memory
+// of a workgroup's few chunks. 8001 tokens of 16 heads of 128 on 4, 1024 keys back and 4 sinks: 260 us with branches on the head size
+// between the products, 99 without, 88 with rows of LDS in all 64 banks and masks as bits (717 TFLOP/s); all 8001 keys, causal, 293 (894). 128
+// sequences, 16621 tokens, 16 heads of 64, 64 keys on either side: 43 us (3.1 TB/s), 2 to 4 workgroups a CU at once; a third slot of LDS
+// instead of the fourth workgroup 47, both, with 34 registers spilled, 99.
 #include "attention_rows.hpp"
 #include "host_utils.hpp"
 #include "trtamd_encoder_ops.h"
