@@ -1182,7 +1182,9 @@ Plan plan_of(trtamd_kv_cache_attention_params const& p)
     int const group = p.q_heads / c.kv_heads;
     int64_t const tokens = std::min(c.max_tokens, c.T);
     int64_t const rows = tokens * group;
-    plan.few = rows <= kFewRows || (c.B > 1 && group <= kFewRows);
+    // Where some sequences may have more rows, few where others may have up to 16: not where the tensors' rows are as many as if all had
+    // the most (two launches without work, 9 us), though tensors may be longer than their sequences; the tiles take any then.
+    plan.few = rows <= kFewRows || (group <= kFewRows && c.T <= (c.B - 1) * tokens + kFewRows / group);
     plan.many = rows > kFewRows;
     plan.fewLimit = plan.few ? kFewRows : 0;
     // keys that a row sees at most, and about

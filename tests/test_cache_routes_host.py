@@ -37,7 +37,9 @@ def route(api, **k):
     # a window bounds what there is to share
     (dict(length=100000, window=300), dict(waves=8, stretches=False)), (dict(length=100000, window=3000), dict(stretches=True)),
     # rows of a key head: 16 and more
-    (dict(n=4), dict(tiles=False)), (dict(n=5), dict(tiles=True, waves=0, stretches=False)), (dict(B=2, n=5), dict(tiles=True, stretches=True)),
+    (dict(n=4), dict(tiles=False)), (dict(n=5), dict(tiles=True, waves=0, stretches=False)), (dict(B=2, n=5, T=9), dict(tiles=True, stretches=True)),
+    (dict(B=2, n=5), dict(tiles=True, stretches=False, waves=0)), (dict(B=8, n=512, T=4096), dict(tiles=True, stretches=False, waves=0)),
+    (dict(B=8, n=512, T=3000), dict(tiles=True, stretches=True)),
     (dict(n=1, heads=136), dict(tiles=True, waves=0)), (dict(B=3, n=1, heads=136), dict(tiles=True, waves=0, stretches=False)),
     # tiles enough for the chip: whole keys; otherwise parts
     (dict(B=4, n=1024, length=9000), dict(tiles=True, parts=1)), (dict(n=64, length=100000), dict(tiles=True)), (dict(n=8192, length=8192), dict(parts=1))])

@@ -375,6 +375,16 @@ def test_pool_past_4_gib(api):
         check_attention(small, cu, q, host(out), 0.1, sample=16)
 
 
+def test_tensors_longer_than_their_sequences(api):
+    """As many rows as if all sequences had the most, though two have one: nobody is left out."""
+    cache = filled(api, "int8", 32, 2, 64, [300, 200, 90])
+    cu = np.array([0, 50, 51, 52])
+    q = cache.r.standard_normal((150, 8, 64)).astype(np.float16)
+    got = attend(api, cache, cu, q, 0.125, T=150)
+    check_attention(cache, cu, q, got, 0.125, sample=40)
+    assert (got[52:] == -7).all()
+
+
 def test_calls_again_give_the_same_bits(api):
     cache = filled(api, "fp8", 16, 2, 128, [3000, 700])
     for new in ([1, 1], [200, 100]):
