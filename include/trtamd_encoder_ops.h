@@ -218,7 +218,7 @@ typedef struct trtamd_kv_cache
     int32_t data_type;         /* of k and v: 2 = INT8, 6 = FP8 E4M3 (nvinfer1::DataType values) */
     int32_t pages;             /* in the pool */
     int32_t page_tokens;       /* 16, 32, 64 or 128 */
-    int32_t kv_heads;
+    int32_t kv_heads;          /* at most 16383; pages * kv_heads < 2^31 */
     int32_t d;                 /* a multiple of 16, at most 256 */
     int32_t B;                 /* sequences, at most 65535 */
     int32_t max_pages;         /* entries of a sequence in page_table; max_pages * page_tokens at most 2^30 */
@@ -274,7 +274,7 @@ typedef struct trtamd_kv_cache_attention_params
     trtamd_half_t const* q;
     trtamd_half_t* out;
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-    int32_t q_heads;        /* a multiple of kv_heads */
+    int32_t q_heads;        /* a multiple of kv_heads; T * q_heads < 2^30 */
     float scale;            /* of the scores; finite and not negative */
     int32_t window;         /* tokens that a row sees, itself the last of them; 0: all */
     int32_t sinks;          /* 0 or more */
@@ -309,10 +309,10 @@ typedef struct trtamd_window_attention_params
     int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
     int32_t const* cu_seqlens; /* [B + 1] */
     int32_t B;                 /* sequences, at most 65535 */
-    int32_t T;                 /* rows of the tensors */
+    int32_t T;                 /* rows of the tensors; T * q_heads < 2^30 */
     int32_t max_tokens;        /* of a sequence, or more */
     int32_t q_heads;           /* a multiple of kv_heads */
-    int32_t kv_heads;
+    int32_t kv_heads;          /* at most 65535 */
     int32_t d;                 /* a multiple of 8, at most 256 */
     float scale;               /* finite and not negative */
     int32_t left, right;       /* -1 or more */

@@ -376,9 +376,10 @@ int window_check(trtamd_window_attention_params const& p)
     {
         return TRTAMD_STATUS_SUCCESS;
     }
-    if (p.B > 65535 || (int64_t) p.T * p.q_heads >= (int64_t) 1 << 30)
+    if (p.B > 65535 || (int64_t) p.T * p.q_heads >= (int64_t) 1 << 30 || p.kv_heads > 65535) // a launch has 2^32 threads
     {
-        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d (at most 65535), T * q_heads of 2^30 or more", what, p.B);
+        return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: B=%d kv_heads=%d (at most 65535), T * q_heads=%lld (less than 2^30)", what, p.B, p.kv_heads,
+            (long long) p.T * p.q_heads);
     }
     for (void const* x : {(void const*) p.q, (void const*) p.k, (void const*) p.v, (void const*) p.out, (void const*) p.cu_seqlens})
     {

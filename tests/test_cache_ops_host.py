@@ -91,7 +91,7 @@ def window(**change):
     (dict(sinks=-1), "sinks=-1"), (dict(q=0), "null"), (dict(k=0), "null"), (dict(v=0), "null"), (dict(out=0), "null"),
     (dict(cu_seqlens=0), "null"), (dict(q=A + 8), "aligned"), (dict(out=A + 2), "aligned"), (dict(cu_seqlens=A + 2), "aligned"),
     (dict(k_token_stride=68), "strides"), (dict(v_head_stride=-64), "strides"), (dict(B=65536), "65535"),
-    (dict(T=1 << 29, max_tokens=1 << 29), "2^30")])
+    (dict(T=1 << 29, max_tokens=1 << 29), "2^30"), (dict(q_heads=65536, kv_heads=65536, T=1), "65535")])
 def test_window_refuses(api, change, word):
     refused(api, api.window_attention(None, window(**change)), word, "window_attention")
 
