@@ -324,20 +324,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
     }
 }
 
+// LDS that a workgroup asks for where it needs `need` bytes. Fewer workgroups than the CUs could hold at once are not spread evenly by
+// themselves: some CUs get as many as fit and others none. With no more than their share fitting they are: 16 sequences of up to 512, 12
+// heads of 64, all keys (some 360 tiles) 20.0 us without, 17.1 with two a CU; 32 of up to 384 in windows (760) 17.4, three 15.7; 8
+// (190) 10.7, one 9.7.
+constexpr int kCuLds = 160 << 10, kMostLds = kCuLds / 2 + 1024;
+size_t spreading_lds(size_t need, int64_t workgroups, int cus)
+{
+    int64_t const share = std::max<int64_t>((workgroups + cus - 1) / cus, 1);
+    return share >= 4 ? need : std::max(need, (size_t) (kCuLds / (share + 1) + 1024));
+}
+
 template <int KS>
-int launch(hipStream_t stream, dim3 grid, WindowArgs const& a)
+int launch(hipStream_t stream, dim3 grid, int64_t tiles, WindowArgs const& a)
 {
     constexpr int kBytes = WindowLds<padded_head(KS)>::kTotal;
-    if constexpr (kBytes > 65536)
+    static hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(window_attention_kernel<KS>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        std::max(kBytes, kMostLds));
+    if (e != hipSuccess)
     {
-        static hipError_t const e = hipFuncSetAttribute(
-            reinterpret_cast<void const*>(window_attention_kernel<KS>), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        if (e != hipSuccess)
-        {
-            return set_error(TRTAMD_STATUS_FAILURE, "window_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
-        }
+        return set_error(TRTAMD_STATUS_FAILURE, "window_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(window_attention_kernel<KS>, grid, dim3(kThreads), kBytes, stream, a);
+    hipLaunchKernelGGL(window_attention_kernel<KS>, grid, dim3(kThreads), spreading_lds(kBytes, tiles, num_cus()), stream, a);
     return check_launch("window_attention_kernel");
 }
 
@@ -437,5 +445,7 @@ extern "C" int trtamd_window_attention(trtamd_stream_t stream, trtamd_window_att
     int64_t const tiles = ceil_div((int64_t) std::min(p.max_tokens, p.T) * group, (int64_t) kTileRows);
     a.near = p.d == padded_head(head_steps(p.d)) && std::max(a.k.token, a.v.token) < (int64_t) 1 << 25;
     dim3 const grid((unsigned) (tiles * p.kv_heads), 1, (unsigned) p.B);
-    return by_head(p.d, [&](auto steps) { return launch<decltype(steps)::value>(as_stream(stream), grid, a); });
+    // about as many tiles as there are: one of each sequence is half full
+    int64_t const there = ((int64_t) p.T * group / kTileRows + (p.B + 1) / 2) * p.kv_heads;
+    return by_head(p.d, [&](auto steps) { return launch<decltype(steps)::value>(as_stream(stream), grid, there, a); });
 }
