@@ -34,17 +34,17 @@ struct AttentionArgs
     uint8_t const* q; // FP16
     uint8_t* out;
     int64_t qToken, qHead, outToken, outHead; // elements
-    float* partial;   // [row][slot][d], the sums that parts of a row's keys have in cached_many_kernel
-    float* stats;     // [row][slot][2]: minus the maximum, sum of the weights
+    float* partial;    // [row][slot][d], the sums that parts of a row's keys have in cached_many_kernel
+    float* stats;      // [row][slot][2]: minus the maximum, sum of the weights
     float* fewPartial; // [stretch][2][16][d]
-    float* fewStats;  // [stretch][2][16][2]
+    float* fewStats;   // [stretch][2][16][2]
     int32_t* fewHeads; // [B][key heads][2]: the first of a head's sums in fewPartial, and how many
-    FastDiv group;    // query heads of a key head
+    FastDiv group;     // query heads of a key head
     int32_t qHeads;
     int32_t window, sinks;
     int32_t slots;    // of a row in partial
     int32_t manySpan; // chunks of 64 keys that a workgroup takes
-    int32_t fewLimit; // sequences of up to so many rows are cached_few_kernel's
+    int32_t fewLimit; // sequences of up to so many rows are the other kernels'
     float scale;      // in powers of 2
 };
 
