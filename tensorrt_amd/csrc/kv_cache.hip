@@ -153,6 +153,10 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(CopyArgs const
     int const P = 1 << c.shift, stride = c.d + kRowPad;
     CacheRows const r = cache_rows(c, b);
     int const begin = max(r.begin, 0), end = min(r.begin + r.n, r.len);
+    if (begin >= end)
+    {
+        return; // the whole workgroup: a page that the sequence only reads may be another one's that writes it
+    }
     Strided const from = which ? a.kv[1] : a.kv[0];
     uint8_t const* const src = from.p + 2 * (int64_t) h * from.head;
     int const n8 = a.chunks.d;

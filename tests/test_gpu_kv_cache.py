@@ -393,3 +393,33 @@ def test_calls_again_give_the_same_bits(api):
         first = attend(api, cache, cu, q, 0.1)
         for _ in range(3):
             assert np.array_equal(first, attend(api, cache, cu, q, 0.1))
+
+
+@pytest.mark.parametrize("dtype,P,d", [("int8", 16, 64), ("fp8", 64, 128), ("int8", 128, 256), ("fp8", 128, 256)])
+@pytest.mark.parametrize("behind", [False, True])
+def test_sequences_without_rows_write_nothing(api, dtype, P, d, behind):
+    """Idle sequences, of no rows or with all of theirs behind T, whose last page, partly filled, is a page that another sequence of the call
+    appends to, loud enough to double its scale; and idle ones whose table names pages with scales that no write leaves. One
+    wavefront a page and head, and four (128 x 256)."""
+    H, writers = 2, 12
+    old = [P // 2 + 1 + b % (P // 2 - 4) for b in range(writers)]
+    cache = Cache(dtype, P, H, d, 3 * writers, 3 * writers, 2, seed=P + d)
+    cache.grow(old + [0] * (2 * writers))
+    cu = np.concatenate([[0], np.cumsum(cache.lengths)])
+    write(api, cache, new_rows(cache.r, int(cu[-1]), H, d), cu)
+    idle, odd = np.arange(writers, 2 * writers), np.arange(2 * writers, 3 * writers)
+    cache.table[idle] = cache.table[:writers]
+    cache.lengths[idle] = np.array(old) - np.arange(writers) % 3
+    cache.table[odd, 0] = cache.free[:writers]
+    cache.lengths[odd] = P // 2
+    for x in (cache.ks, cache.vs):
+        x[cache.table[odd, 0]] = np.array([-1.0, -0.0, np.inf, 1e-40], np.float32)[np.arange(writers) % 4, None]
+    cache.upload()
+    for new in (1, 2):
+        cache.grow([new] * writers + [0] * (2 * writers))
+        cu = np.concatenate([[0], np.cumsum([new] * writers + [2 if behind else 0] * (2 * writers))])
+        kv = new_rows(cache.r, int(cu[-1]), H, d) * np.float16(8 ** new)
+        write(api, cache, kv, cu, T=new * writers)
+        cache.check()
+        for which in ("ks", "vs"):
+            assert np.array_equal(host(getattr(cache, "d" + which)).view(np.uint32), getattr(cache, which).view(np.uint32))
