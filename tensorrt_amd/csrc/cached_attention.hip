@@ -66,8 +66,9 @@ __device__ inline bool sees_all(Seen const& least, Seen const& most, int key0)
     return key0 + kChunkKeys <= least.hi && (key0 >= most.lo || key0 + kChunkKeys <= least.sinks);
 }
 
-// What a page's scales are to its scores and weights. No values of 0 or below 2^-126 (a scale of 0 times a score of -infinity is no
-// number), but what is a NaN stays one.
+// What a page's scales are to its scores and weights. No score factor of 0 or below 2^-126 (0 times a score of -infinity is no number), but
+// what is a NaN stays one. The inverse is finite whatever the scale is: a weight of 0 is multiplied by it where no row sees the page, and
+// scales of pages that were never written may be any.
 struct PageFactors
 {
     float score, log2Value, inverse;
@@ -79,8 +80,8 @@ __device__ inline PageFactors page_factors(float kScale, float vScale, float sca
     float const s = kScale * scale;
     f.score = s < 0x1p-126f ? 0x1p-126f : s;
     // the values of a scale of 0 are zeros: any scale does, and the least one leaves the maximum to the others
-    f.log2Value = vScale == 0.f ? -32.f : __builtin_amdgcn_logf(vScale);
-    f.inverse = vScale > 0.f ? 1.f / vScale : 0x1p32f;
+    f.log2Value = fabsf(vScale) < 0x1p-126f ? -32.f : __builtin_amdgcn_logf(vScale);
+    f.inverse = vScale >= 0x1p-126f ? 1.f / vScale : 0x1p32f;
     return f;
 }
 

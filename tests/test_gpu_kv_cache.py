@@ -423,3 +423,31 @@ def test_sequences_without_rows_write_nothing(api, dtype, P, d, behind):
         cache.check()
         for which in ("ks", "vs"):
             assert np.array_equal(host(getattr(cache, "d" + which)).view(np.uint32), getattr(cache, which).view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype,P", [("int8", 16), ("fp8", 32)])
+@pytest.mark.parametrize("what", [1e-40, np.nan, np.inf, -1.0, 0.0])
+def test_scales_of_pages_that_no_row_sees(api, dtype, P, what):
+    """Pages behind a sequence's end that the table names already, and page 0, which stands in for pages that are gone: whatever their
+    scales are, subnormal numbers included, no row is touched by them."""
+    H, heads, d = 2, 4, 64
+    lens = [40, 70, 150, 1]
+    cache = Cache(dtype, P, H, d, 40, len(lens), 16, seed=P)
+    cache.free.remove(0)
+    cache.grow(lens)
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    write(api, cache, new_rows(cache.r, int(cu[-1]), H, d), cu)
+    for b, n in enumerate(lens):
+        behind = -(-n // P)
+        cache.table[b, behind:behind + 3] = cache.free[3 * b:3 * b + 3]
+    cache.table[2, 1:3] = -1
+    unwritten = np.setdiff1d(np.arange(40), [cache.table[b, i] for b, n in enumerate(lens) for i in range(-(-n // P))])
+    assert 0 in unwritten and cache.table[0, -(-40 // P)] in unwritten
+    cache.ks[unwritten], cache.vs[unwritten] = what, what
+    cache.upload()
+    for new in ([2, 1, 4, 1], [20, 40, 30, 1]):
+        cu = np.concatenate([[0], np.cumsum(new)])
+        q = cache.r.standard_normal((int(cu[-1]), heads, d)).astype(np.float16)
+        for window, max_length in ((0, 0), (0, 2), (30, 0)):
+            got = attend(api, cache, cu, q, 0.125, window=window, max_length=max_length)
+            check_attention(cache, cu, q, got, 0.125, window, sample=40)
