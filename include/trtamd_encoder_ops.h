@@ -264,7 +264,7 @@ TRTAMD_API int trtamd_kv_cache_read(trtamd_stream_t stream, trtamd_kv_cache_read
  * tokens j <= p, with a window only those with j > p - window, and the first `sinks` tokens whatever the window is.
  *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j),  k_j and v_j what the cache's bytes stand for.
  * Products of the bytes' values are exact, sums, maxima and exponentials binary32; the weights of the second product are rounded
- * to binary16 once, half to even.  A row that sees nothing is zeros.  Query head h reads head h / (q_heads / kv_heads) of the cache.
+ * to binary16 once, half to even, the largest at 2^7 or more: by 2^-11 of themselves, or 2^-32 of the largest where that is more.  A row that sees nothing is zeros.  Query head h reads head h / (q_heads / kv_heads) of the cache.
  * A result can differ in its last bits between calls of other sizes or estimates, not between calls of the same.
  * q: row t, head h at q + t * q_token_stride + h * q_head_stride, multiples of 8 elements, d values in a row; out alike.  What is
  * written overlaps nothing that is read, but out may be q with the same strides. */
@@ -292,7 +292,7 @@ TRTAMD_API int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
  * Attention in windows, over packed sequences in FP16: row i of a sequence sees the rows i - left .. i + right and the first `sinks`
  * rows, of them none behind i + right; left or right -1: all on that side (right = 0: causal).
  *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j)
- * Sums, maxima and exponentials are binary32, the weights of the second product rounded to binary16 once, half to even.  Rows that
+ * Sums, maxima and exponentials are binary32, the weights of the second product rounded to binary16 once, as above.  Rows that
  * are not seen do not take part whatever they hold, infinities and NaNs included (a NaN or an infinity anywhere near makes the
  * rows around it slow).  A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
  * max_tokens-th on, are left out: neither read nor written.  Row t, head h of q at q + t * q_token_stride + h * q_head_stride, d

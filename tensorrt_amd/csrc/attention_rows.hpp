@@ -15,6 +15,10 @@ namespace trtamd
 
 constexpr int kChunkKeys = 64;
 constexpr float kNothingSeen = 3.402823466e+38f; // minus the maximum of no scores, finite
+// Weights reach the second product in binary16, which has 2^-14 to 65504 with all its digits. The largest is held between 2^7 and 2^15 (a
+// maximum moves the sums only where it passes the last one by 2^8), so that one of 2^-21 of it still has them and one of 2^-32 does not
+// vanish: many keys that only add up to something behind one loud one. With the largest from 1 on, 8191 keys of 2^-26 each came out as nothing.
+constexpr float kWeightsTop = 7.f;
 
 // The key of a block of 32 that LDS row m of the block holds, and the row that holds key k.
 __device__ inline int key_of_row(int m)
@@ -82,7 +86,7 @@ template <int DV>
 struct RowSums
 {
     f32x16 out[DV]; // O^T: elements 32 d + 8 (v / 4) + 4 h + v % 4 of query lane % 32
-    float negMax;   // minus the maximum that the weights are relative to, in powers of 2
+    float negMax;   // kWeightsTop minus the maximum that the weights are relative to, in powers of 2
     float sum;      // of this lane's keys
 
     __device__ void clear()
@@ -104,7 +108,7 @@ struct RowSums
     // this chunk's scores, of both halves.
     __device__ void move(float mx)
     {
-        float const negNew = fminf(-mx, kNothingSeen);
+        float const negNew = fminf(kWeightsTop - mx, kNothingSeen);
         if (__ballot(negNew < negMax - 8.f) != 0)
         {
             float const to = fminf(negNew, negMax);

@@ -5,7 +5,8 @@
 // Bytes become binary16 exactly, so the products' operands are the bytes' values and the scales go elsewhere: a page's key scale into
 // the multiplication that brings its scores to powers of 2, its value scale into the exponent, s + log2(value scale), where it costs
 // nothing: the weights P' = p * value scale are what the second product wants, and p = P' / value scale is summed by one multiply-add.
-// The running maximum is that of the weights P', so that they fill binary16's range whatever the scales are.
+// The running maximum is that of the weights P', so that the largest lies where binary16 has the most digits below it (kWeightsTop) whatever
+// the scales are.
 //
 // Rows of one key head, (token, query head) with the heads of a group side by side, share the keys. Up to 16 of them (decoding, a few
 // drafted tokens) go to `cached_few_kernel` or `cached_stretch_kernel`, which are bound by reading the cache; more to
@@ -35,7 +36,7 @@ struct AttentionArgs
     uint8_t* out;
     int64_t qToken, qHead, outToken, outHead; // elements
     float* partial;    // [row][slot][d], the sums that parts of a row's keys have in cached_many_kernel
-    float* stats;      // [row][slot][2]: minus the maximum, sum of the weights
+    float* stats;      // [row][slot][2]: negMax (attention_rows.hpp), sum of the weights
     float* fewPartial; // [stretch][2][16][d]
     float* fewStats;   // [stretch][2][16][2]
     int32_t* fewHeads; // [B][key heads][2]: the first of a head's sums in fewPartial, and how many
@@ -287,7 +288,7 @@ struct FewWave
             mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
         }
         mx = reduce_step<32>(reduce_step<16>(mx, max_of), max_of);
-        float const negNew = fminf(-mx, kNothingSeen);
+        float const negNew = fminf(kWeightsTop - mx, kNothingSeen);
         if (__ballot(negNew < negMax - 8.f) != 0)
         {
             float const to = fminf(negNew, negMax), by = __builtin_amdgcn_exp2f(to - negMax);
@@ -330,7 +331,7 @@ struct FewWave
 };
 
 // The sums of a workgroup's W wavefronts meet in LDS, as they are; then each thread adds some elements up over the wavefronts and gives
-// them to store(tile, sums, minus the maximum, sum of the weights).
+// them to store(tile, sums, negMax, sum of the weights).
 template <int KS, bool FP8, int W>
 struct FewMeeting
 {
