@@ -14,7 +14,8 @@ namespace trtamd
 {
 
 constexpr int kChunkKeys = 64;
-constexpr float kNothingSeen = 3.402823466e+38f; // minus the maximum of no scores, finite
+constexpr float kLargest = 3.402823466e+38f;     // binary32
+constexpr float kNothingSeen = kLargest;         // minus the maximum of no scores, finite
 // Weights reach the second product in binary16, which has 2^-14 to 65504 with all its digits. The largest is held between 2^7 and 2^15 (a
 // maximum moves the sums only where it passes the last one by 2^8), so that one of 2^-21 of it still has them and one of 2^-32 does not
 // vanish: many keys that only add up to something behind one loud one. With the largest from 1 on, 8191 keys of 2^-26 each came out as nothing.

@@ -67,8 +67,8 @@ __device__ inline bool sees_all(Seen const& least, Seen const& most, int key0)
     return key0 + kChunkKeys <= least.hi && (key0 >= most.lo || key0 + kChunkKeys <= least.sinks);
 }
 
-// What a page's scales are to its scores and weights. No score factor of 0 or below 2^-126 (0 times a score of -infinity is no number), but
-// what is a NaN stays one. The inverse is finite whatever the scale is: a weight of 0 is multiplied by it where no row sees the page, and
+// What a page's scales are to its scores and weights. No score factor of 0 or below 2^-126 (0 times a score of -infinity is no number), nor an
+// infinite one (times a score of 0), but what is a NaN stays one. The inverse is finite whatever the scale is: a weight of 0 is multiplied by it where no row sees the page, and
 // scales of pages that were never written may be any.
 struct PageFactors
 {
@@ -79,7 +79,7 @@ __device__ inline PageFactors page_factors(float kScale, float vScale, float sca
 {
     PageFactors f;
     float const s = kScale * scale;
-    f.score = s < 0x1p-126f ? 0x1p-126f : s;
+    f.score = s < 0x1p-126f ? 0x1p-126f : s > kLargest ? kLargest : s;
     // the values of a scale of 0 are zeros: any scale does, and the least one leaves the maximum to the others
     f.log2Value = fabsf(vScale) < 0x1p-126f ? -32.f : __builtin_amdgcn_logf(vScale);
     f.inverse = vScale >= 0x1p-126f ? 1.f / vScale : 0x1p32f;
@@ -1430,6 +1430,6 @@ extern "C" int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
     a.group = fast_div((uint32_t) (p.q_heads / c.kv_heads));
     a.qHeads = p.q_heads, a.window = p.window, a.sinks = p.sinks, a.slots = plan.manySplits;
     a.manySpan = plan.manySpan, a.fewLimit = plan.fewLimit;
-    a.scale = p.scale * 1.44269504088896f;
+    a.scale = std::min(p.scale * 1.44269504088896f, kLargest);
     return c.data_type == kCacheFp8 ? launch<true>(as_stream(stream), p, plan, a) : launch<false>(as_stream(stream), p, plan, a);
 }

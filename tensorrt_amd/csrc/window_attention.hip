@@ -437,8 +437,8 @@ extern "C" int trtamd_window_attention(trtamd_stream_t stream, trtamd_window_att
     a.left = p.left < 0 ? INT32_MAX : p.left;
     a.right = p.right < 0 ? INT32_MAX : p.right;
     a.sinks = p.sinks;
-    // a scale of 0 times a score of -infinity is no number
-    a.scale = std::max(p.scale * 1.44269504088896f, 0x1p-126f);
+    // a scale of 0 times a score of -infinity is no number, nor is an infinite one times 0
+    a.scale = std::min(std::max(p.scale * 1.44269504088896f, 0x1p-126f), kLargest);
     int const group = p.q_heads / p.kv_heads;
     a.group = fast_div((uint32_t) group);
     a.kvHeads = fast_div((uint32_t) p.kv_heads);

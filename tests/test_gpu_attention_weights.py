@@ -1,14 +1,12 @@
 """Weights far below the largest one: a loud first token that the rows look at for want of anything else, with a value of zero, and
-thousands of quiet keys whose weights only add up to something. Attention over the cache and in windows, against binary64."""
-import ctypes as C
-
+thousands of quiet keys whose weights only add up to something. Attention over the cache and in windows, against binary64. And scales of the
+scores near the largest binary32."""
 import numpy as np
 import pytest
 
-from cache_helpers import Cache, TOP, assert_within, round_codes
-from helpers import dev, dev_empty, host, rng
+from cache_helpers import Cache, assert_within, round_codes, values
 from tensorrt_amd import capi
-from test_gpu_kv_cache import attend
+from test_gpu_kv_cache import attend, check_attention, filled
 from test_gpu_window_attention import Problem
 
 pytestmark = pytest.mark.gpu
@@ -61,7 +59,6 @@ def test_over_the_cache(api, dtype, rows, max_length):
     scale = np.float32(1 / 32)
     q[0, :, 0] = depths / np.log2(np.e)
     depths = q[0, :, 0].astype(np.float64) * np.log2(np.e)
-    from cache_helpers import values
     want, tol = expected(depths, values(v, dtype).astype(np.float64)[1:] * 2.0 ** -6)
     got = attend(api, cache, np.array([0, 1]), q, scale, max_length=max_length)
     assert_within(got[0], want, tol)
@@ -81,3 +78,20 @@ def test_in_windows(api, heads):
     want, tol = expected(depths, p.v[1:, 0].astype(np.float64))
     for h in range(heads):
         assert_within(got[-len(DEPTHS):, h], want, tol, f"head {h}")
+
+
+@pytest.mark.parametrize("scale", [1e37, 3.4e38])
+def test_scales_near_the_largest(api, scale):
+    """Scores of zero stay zero whatever they are scaled by, times a page's scale too: rows whose query is zero weigh all keys alike."""
+    cache = filled(api, "int8", 16, 1, D, [100, 7])
+    cache.ks[cache.table[0, 2:4]], cache.ks[cache.table[0, 4]] = 100, 0
+    cache.upload()
+    for new in ([2, 2], [40, 7]):
+        cu = np.concatenate([[0], np.cumsum(new)])
+        q = np.zeros((int(cu[-1]), 2, D), np.float16)
+        check_attention(cache, cu, q, attend(api, cache, cu, q, scale), np.float32(1))
+    p = Problem([70, 5], 2, 1, D, seed=6)
+    p.q[:], p.scale = 0, scale
+    got = p.run(api, 20, 3, 1)
+    p.scale = 1.0
+    p.check(got, 20, 3, 1)
