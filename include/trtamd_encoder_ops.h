@@ -284,7 +284,8 @@ typedef struct trtamd_kv_cache_attention_params
     size_t workspace_bytes; /* trtamd_kv_cache_attention_workspace_size(params) or more */
 } trtamd_kv_cache_attention_params;
 
-/* Of the parameters' sizes alone: no pointer is looked at.  0: none is needed, or the sizes are refused. */
+/* Of the parameters' sizes alone: no pointer is looked at.  0: none is needed, or the call refuses the sizes (trtamd_last_error() then
+ * says why). */
 TRTAMD_API size_t trtamd_kv_cache_attention_workspace_size(trtamd_kv_cache_attention_params const* params);
 TRTAMD_API int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache_attention_params const* params);
 

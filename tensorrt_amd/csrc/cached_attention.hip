@@ -1232,19 +1232,16 @@ size_t workspace_of(trtamd_kv_cache_attention_params const& p, Plan const& plan)
     return (few_floats(p, plan) + many_floats(p, plan)) * sizeof(float);
 }
 
-int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
+// What plan_of relies on, and the size query: no pointer is looked at.
+int attention_sizes_check(char const* what, trtamd_kv_cache_attention_params const& p)
 {
-    if (int const st = cache_check(what, p.cache))
+    if (int const st = cache_sizes_check(what, p.cache))
     {
         return st;
     }
     if (p.q_heads <= 0 || p.q_heads % p.cache.kv_heads != 0)
     {
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: q_heads=%d (a multiple of kv_heads=%d)", what, p.q_heads, p.cache.kv_heads);
-    }
-    if (!(p.scale >= 0.f) || !std::isfinite(p.scale))
-    {
-        return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: scale %g (finite and not negative)", what, p.scale);
     }
     if (p.window < 0 || p.sinks < 0 || p.max_length < 0)
     {
@@ -1257,17 +1254,19 @@ int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
     return TRTAMD_STATUS_SUCCESS;
 }
 
-// What plan_of relies on.
-bool sizes_are_sound(trtamd_kv_cache_attention_params const& p)
+int attention_check(char const* what, trtamd_kv_cache_attention_params const& p)
 {
-    trtamd_kv_cache const& c = p.cache;
-    return c.kv_heads > 0 && p.q_heads > 0 && p.q_heads % c.kv_heads == 0 && c.page_tokens > 0 && c.d > 0 && c.max_pages > 0 && c.B > 0 && c.T > 0
-        && c.max_tokens > 0 && p.window >= 0 && p.sinks >= 0 && p.max_length >= 0;
-}
-
-bool nothing(trtamd_kv_cache const& c)
-{
-    return c.B == 0 || c.T == 0 || c.max_tokens == 0;
+    int st = attention_sizes_check(what, p);
+    st = st ? st : cache_check(what, p.cache);
+    if (st)
+    {
+        return st;
+    }
+    if (!(p.scale >= 0.f) || !std::isfinite(p.scale))
+    {
+        return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: scale %g (finite and not negative)", what, p.scale);
+    }
+    return TRTAMD_STATUS_SUCCESS;
 }
 
 template <int KS, bool FP8>
@@ -1366,12 +1365,16 @@ using namespace trtamd;
 
 extern "C" size_t trtamd_kv_cache_attention_workspace_size(trtamd_kv_cache_attention_params const* params)
 {
-    return params == nullptr || !sizes_are_sound(*params) ? 0 : workspace_of(*params, plan_of(*params));
+    if (params == nullptr || attention_sizes_check("kv_cache_attention_workspace_size", *params) || no_tokens(params->cache))
+    {
+        return 0;
+    }
+    return workspace_of(*params, plan_of(*params));
 }
 
 extern "C" int64_t trtamd_test_kv_cache_attention_route(trtamd_kv_cache_attention_params const* params)
 {
-    if (params == nullptr || !sizes_are_sound(*params))
+    if (params == nullptr || attention_sizes_check("kv_cache_attention_route", *params) || no_tokens(params->cache))
     {
         return -1;
     }
@@ -1398,7 +1401,7 @@ extern "C" int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
             return set_error(TRTAMD_STATUS_BAD_PARAM, "kv_cache_attention: strides must be multiples of 8 elements, and not negative");
         }
     }
-    if (nothing(p.cache))
+    if (no_tokens(p.cache))
     {
         return TRTAMD_STATUS_SUCCESS;
     }

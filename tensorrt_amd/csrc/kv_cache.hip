@@ -447,7 +447,7 @@ int copy_check(char const* what, trtamd_kv_cache const& c, void const* k, void c
             return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: strides must be multiples of 8 elements, and not negative", what);
         }
     }
-    if (c.B == 0 || c.T == 0 || c.max_tokens == 0)
+    if (no_tokens(c))
     {
         return TRTAMD_STATUS_SUCCESS;
     }
@@ -472,7 +472,7 @@ dim3 copy_grid(trtamd_kv_cache const& c)
 
 } // namespace
 
-int cache_check(char const* what, trtamd_kv_cache const& c)
+int cache_sizes_check(char const* what, trtamd_kv_cache const& c)
 {
     if (c.data_type != kCacheInt8 && c.data_type != kCacheFp8)
     {
@@ -492,9 +492,9 @@ int cache_check(char const* what, trtamd_kv_cache const& c)
         return set_error(TRTAMD_STATUS_BAD_PARAM, "%s: B=%d T=%d max_tokens=%d max_pages=%d pages=%d", what, c.B, c.T, c.max_tokens,
             c.max_pages, c.pages);
     }
-    if (c.B == 0 || c.T == 0 || c.max_tokens == 0)
+    if (no_tokens(c))
     {
-        return TRTAMD_STATUS_SUCCESS; // a call without a token: its tensors may have no address
+        return TRTAMD_STATUS_SUCCESS;
     }
     if (c.max_pages == 0 || c.pages == 0)
     {
@@ -511,6 +511,16 @@ int cache_check(char const* what, trtamd_kv_cache const& c)
     if ((int64_t) c.pages * c.kv_heads >= (int64_t) 1 << 31)
     {
         return set_error(TRTAMD_STATUS_NOT_SUPPORTED, "%s: pages * kv_heads of 2^31 or more", what);
+    }
+    return TRTAMD_STATUS_SUCCESS;
+}
+
+int cache_check(char const* what, trtamd_kv_cache const& c)
+{
+    int const st = cache_sizes_check(what, c);
+    if (st || no_tokens(c)) // a call without a token: its tensors may have no address
+    {
+        return st;
     }
     for (void const* p : {(void const*) c.k, (void const*) c.v, (void const*) c.k_scale, (void const*) c.v_scale,
              (void const*) c.page_table, (void const*) c.lengths, (void const*) c.cu_seqlens})
@@ -558,7 +568,7 @@ extern "C" int trtamd_kv_cache_write(trtamd_stream_t stream, trtamd_kv_cache_wri
     {
         return st;
     }
-    if (c.B == 0 || c.T == 0 || c.max_tokens == 0)
+    if (no_tokens(c))
     {
         return TRTAMD_STATUS_SUCCESS;
     }
@@ -603,7 +613,7 @@ extern "C" int trtamd_kv_cache_read(trtamd_stream_t stream, trtamd_kv_cache_read
     {
         return st;
     }
-    if (c.B == 0 || c.T == 0 || c.max_tokens == 0)
+    if (no_tokens(c))
     {
         return TRTAMD_STATUS_SUCCESS;
     }

@@ -24,7 +24,14 @@ struct CacheArgs
     int32_t pages, shift /* log2(page_tokens) */, heads, d, maxPages, maxTokens, T;
 };
 
-// Refuses what no call takes; 0 where it is sound.
+// A call with nothing to do.
+inline bool no_tokens(trtamd_kv_cache const& c)
+{
+    return c.B == 0 || c.T == 0 || c.max_tokens == 0;
+}
+
+// Refuses what no call takes; 0 where it is sound. Of the sizes alone, and of everything.
+int cache_sizes_check(char const* what, trtamd_kv_cache const& c);
 int cache_check(char const* what, trtamd_kv_cache const& c);
 CacheArgs cache_args(trtamd_kv_cache const& c);
 

@@ -118,3 +118,20 @@ def test_workspace_follows_sizes_alone(api):
     gone = dict(k=0, v=0, k_scale=0, v_scale=0, page_table=0, lengths=0, cu_seqlens=0, q=0, out=0, workspace=0, workspace_bytes=0)
     assert api.kv_cache_attention_workspace_size(attention(max_pages=1 << 12, max_length=0, **gone)) == size
     assert api.kv_cache_attention_workspace_size(attention(q_heads=3)) == 0
+
+
+SIZES = [(change, word) for change, word in CACHE if word not in ("null", "aligned")] + [
+    (dict(kv_heads=16384, q_heads=16384), "16383"), (dict(d=300), "d=300"), (dict(d=24), "d=24"), (dict(d=2 ** 31 - 1), "d="), (dict(q_heads=0), "q_heads=0"),
+    (dict(q_heads=3), "q_heads=3"), (dict(q_heads=-2), "q_heads=-2"), (dict(window=-1), "window=-1"), (dict(sinks=-1), "sinks=-1"),
+    (dict(max_length=-1), "max_length=-1"), (dict(T=1 << 28), "2^30")]
+
+
+@pytest.mark.parametrize("change,word", SIZES)
+def test_no_workspace_for_sizes_that_are_refused(api, change, word):
+    """0 where the call refuses the sizes, and the error says which, with pages enough to need a workspace; no pointer is looked at."""
+    gone = dict(k=0, v=0, k_scale=0, v_scale=0, page_table=0, lengths=0, cu_seqlens=0, q=0, out=0, workspace=0)
+    more = {**dict(max_pages=1 << 12, max_length=0), **gone, **change}
+    refused(api, api.kv_cache_attention(None, attention(**more)), word, "kv_cache_attention")
+    assert api.kv_cache_attention_workspace_size(attention(**more)) == 0
+    assert word in api.last_error_str() and "workspace_size" in api.last_error_str()
+    assert api.test_kv_cache_attention_route(attention(**more)) == -1
