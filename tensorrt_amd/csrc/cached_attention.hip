@@ -1275,11 +1275,9 @@ int launch_many(hipStream_t stream, dim3 grid, CacheArgs const& c, AttentionArgs
     constexpr int kBytes = ManyLds<padded_head(KS)>::kTotal;
     if constexpr (kBytes > 65536)
     {
-        static hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(cached_many_kernel<KS, FP8>),
-            hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        if (e != hipSuccess)
+        if (int const st = reserve_lds<cached_many_kernel<KS, FP8>>("kv_cache_attention", kBytes))
         {
-            return set_error(TRTAMD_STATUS_FAILURE, "kv_cache_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
+            return st;
         }
     }
     hipLaunchKernelGGL((cached_many_kernel<KS, FP8>), grid, dim3(kThreads), kBytes, stream, c, a, heads);

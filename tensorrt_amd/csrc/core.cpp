@@ -1,4 +1,5 @@
-// Library-wide state of the C-ABI layer: version, the per-thread error text and the tuning switches.
+// Library-wide state of the C-ABI layer: version, the per-thread error text, the tuning switches and the
+// kernels whose LDS limit is raised.
 #include "host_utils.hpp"
 
 #include "trtamd_test_hooks.h"
@@ -7,6 +8,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <vector>
 
 namespace trtamd
 {
@@ -85,6 +87,29 @@ int set_error(int status, char const* fmt, ...)
     vsnprintf(gLastError, sizeof(gLastError), fmt, ap);
     va_end(ap);
     return status;
+}
+
+int ensure_lds(void const* key, char const* name, int ldsBytes)
+{
+    static std::mutex mtx;
+    static std::vector<void const*> done;
+    std::lock_guard<std::mutex> lock(mtx);
+    for (void const* p : done)
+    {
+        if (p == key)
+        {
+            return TRTAMD_STATUS_SUCCESS;
+        }
+    }
+    hipError_t const e = hipFuncSetAttribute(key, hipFuncAttributeMaxDynamicSharedMemorySize, ldsBytes);
+    if (e != hipSuccess)
+    {
+        (void) hipGetLastError();
+        return set_error(TRTAMD_STATUS_FAILURE, "%s: cannot reserve %d bytes of LDS: %s", name, ldsBytes,
+            hipGetErrorString(e));
+    }
+    done.push_back(key);
+    return TRTAMD_STATUS_SUCCESS;
 }
 } // namespace trtamd
 

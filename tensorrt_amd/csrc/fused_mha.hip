@@ -28,10 +28,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
-#include <atomic>
-#include <mutex>
 #include <type_traits>
-#include <vector>
 
 namespace trtamd
 {
@@ -2260,43 +2257,12 @@ __global__ __launch_bounds__(kWavesStream* kWaveSize) __attribute__((amdgpu_wave
 // host side
 // ------------------------------------------------------------------------------------------
 
-// Raising the dynamic LDS limit is a per-function attribute, set once per process and kernel: at the first launch,
-// or ahead of it by trtamd_fused_mha_prepare.
-int ensure_lds(void const* key, char const* name, int ldsBytes)
-{
-    static std::mutex mtx;
-    static std::vector<void const*> done;
-    std::lock_guard<std::mutex> lock(mtx);
-    for (void const* p : done)
-    {
-        if (p == key)
-        {
-            return TRTAMD_STATUS_SUCCESS;
-        }
-    }
-    hipError_t const e = hipFuncSetAttribute(key, hipFuncAttributeMaxDynamicSharedMemorySize, ldsBytes);
-    if (e != hipSuccess)
-    {
-        (void) hipGetLastError();
-        return set_error(TRTAMD_STATUS_FAILURE, "%s: cannot reserve %d bytes of LDS: %s", name, ldsBytes,
-            hipGetErrorString(e));
-    }
-    done.push_back(key);
-    return TRTAMD_STATUS_SUCCESS;
-}
-
 template <auto KERNEL>
 int launch_fmha(char const* name, hipStream_t stream, FmhaArgs const& args, int ldsBytes, int waves)
 {
-    static std::atomic<bool> reserved{false}; // known without the lock from the second launch on
-    if (!reserved.load(std::memory_order_acquire))
+    if (int const st = reserve_lds<KERNEL>(name, ldsBytes))
     {
-        int const st = ensure_lds(reinterpret_cast<void const*>(KERNEL), name, ldsBytes);
-        if (st != TRTAMD_STATUS_SUCCESS)
-        {
-            return st;
-        }
-        reserved.store(true, std::memory_order_release);
+        return st;
     }
     unsigned const blocks = (unsigned) args.B * args.N * args.qSplit;
     if constexpr (std::is_invocable_v<decltype(KERNEL), FmhaArgs>)

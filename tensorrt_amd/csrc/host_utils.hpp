@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -57,6 +58,26 @@ int tuning(Tuning which);
 
 // Compute units of the current device, asked once per process (256 when the query fails).
 int num_cus();
+
+// Raising the dynamic LDS limit is a per-function attribute, set once per process and kernel: at the first launch, or ahead of it by
+// trtamd_fused_mha_prepare.  What fails is tried again by the next call.
+int ensure_lds(void const* key, char const* name, int ldsBytes);
+
+// The same for launches, which know without the lock from the second on.
+template <auto KERNEL>
+int reserve_lds(char const* name, int ldsBytes)
+{
+    static std::atomic<bool> reserved{false};
+    if (!reserved.load(std::memory_order_acquire))
+    {
+        if (int const st = ensure_lds(reinterpret_cast<void const*>(KERNEL), name, ldsBytes))
+        {
+            return st;
+        }
+        reserved.store(true, std::memory_order_release);
+    }
+    return TRTAMD_STATUS_SUCCESS;
+}
 
 template <typename T>
 constexpr T ceil_div(T a, T b)

@@ -339,11 +339,9 @@ template <int KS>
 int launch(hipStream_t stream, dim3 grid, int64_t tiles, WindowArgs const& a)
 {
     constexpr int kBytes = WindowLds<padded_head(KS)>::kTotal;
-    static hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(window_attention_kernel<KS>), hipFuncAttributeMaxDynamicSharedMemorySize,
-        std::max(kBytes, kMostLds));
-    if (e != hipSuccess)
+    if (int const st = reserve_lds<window_attention_kernel<KS>>("window_attention", std::max(kBytes, kMostLds)))
     {
-        return set_error(TRTAMD_STATUS_FAILURE, "window_attention: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
+        return st;
     }
     hipLaunchKernelGGL(window_attention_kernel<KS>, grid, dim3(kThreads), spreading_lds(kBytes, tiles, num_cus()), stream, a);
     return check_launch("window_attention_kernel");
