@@ -451,3 +451,32 @@ def test_scales_of_pages_that_no_row_sees(api, dtype, P, what):
         for window, max_length in ((0, 0), (0, 2), (30, 0)):
             got = attend(api, cache, cu, q, 0.125, window=window, max_length=max_length)
             check_attention(cache, cu, q, got, 0.125, window, sample=40)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "fp8"])
+@pytest.mark.parametrize("lengths,cu,T", [
+    ([2 ** 31 - 1, 100, -5], [0, 2, 4, 6], 6), ([64, 64, 64], [3, 1, 6, 2], 6), ([64, 64, 64], [-7, 2, 2 ** 31 - 1, 5], 6),
+    ([2 ** 31 - 1] * 3, [0, 20, 40, 60], 60), ([64, 2 ** 30, 33], [50, 10, 45, 60], 60), ([-2 ** 31, 70, 2 ** 31 - 1], [0, 2 ** 31 - 1, 1, 30], 60)])
+def test_writes_of_no_sense_stay_in_their_pages(api, dtype, lengths, cu, T):
+    """Lengths and rows that no cache has: pages that no table entry names, and what lies behind the pool and the scales, stay as they were."""
+    import torch
+    cache = filled(api, dtype, 16, 2, 64, [64, 64, 64], spare=5)
+    cache.lengths = np.array(lengths, np.int32)
+    cache.dlengths.copy_(dev(cache.lengths))
+    pool = [cache.dk, cache.dv, cache.dks, cache.dvs]
+    guarded = [torch.cat([x.flatten().view(torch.uint8), torch.full((4096,), 0x5A, dtype=torch.uint8, device="cuda")]) for x in pool]
+    before = [host(x) for x in guarded]
+    kv = new_rows(cache.r, T, 2, 64)
+    c, keep = cache.described(np.array(cu), T=T, max_tokens=min(T, 40))
+    c.k, c.v, c.k_scale, c.v_scale = (ptr(x) for x in guarded)
+    t = dev(kv)
+    s = dict(k_token_stride=256, k_head_stride=128, v_token_stride=256, v_head_stride=128)
+    api.check(api.kv_cache_write(stream(), C.byref(capi.KvCacheWriteParams(cache=c, k=ptr(t), v=ptr(t) + 128, **s))))
+    sync()
+    others = np.setdiff1d(np.arange(cache.pages), cache.table)
+    assert len(others) == 5
+    for x, was, shape in zip(guarded, before, (cache.k.shape, cache.v.shape, cache.ks.shape, cache.vs.shape)):
+        now = host(x)
+        assert np.array_equal(now[-4096:], was[-4096:])
+        pages = [y[:-4096].reshape(shape[0], -1)[others] for y in (now, was)]
+        assert np.array_equal(*pages)

@@ -209,3 +209,27 @@ def test_far_rows(api, strides):
     api.check(api.window_attention(stream(), C.byref(params(*rows, out, dcu, 1, n, p.scale, 9, 9, 2))))
     sync()
     p.check(host(out), 9, 9, 2)
+
+
+@pytest.mark.parametrize("d", [64, 72, 128])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+def test_infinities_that_are_seen(api, what, d):
+    """A value that a row sees and that is infinite: its element is that infinity, of its sign, in every row that sees it, and no other
+    element is touched; two of opposite signs are no number."""
+    p = Problem([150, 90], 4, 2, d, seed=12)
+    for t, h, e, x in ((30, 0, 5, what), (64, 1, 0, what), (150 + 70, 0, d - 1, what), (100, 0, 7, what), (103, 0, 7, -what)):
+        p.v[t, h, e] = x
+    for left, right, sinks in ((10, 10, 0), (20, 0, 40), (-1, -1, 0)):
+        got = p.run(api, left, right, sinks).astype(np.float64)
+        for lo, hi in zip(p.cu[:-1], p.cu[1:]):
+            n = int(hi - lo)
+            for i in range(n):
+                ok = visible_keys(i, n, None if left < 0 else left, None if right < 0 else right, sinks)
+                for h in range(4):
+                    k, v = p.k[lo:hi, h // 2], p.v[lo:hi, h // 2].astype(np.float64)
+                    with np.errstate(invalid="ignore"):
+                        odd = np.where(ok[:, None] & ~np.isfinite(v), v, 0).sum(0)
+                    sound = odd == 0
+                    want, tol = attention_reference(p.q[lo + i, h], k, np.ones(n), np.where(np.isfinite(v), v, 0), np.ones(n), ok, p.scale)
+                    assert np.array_equal(got[lo + i, h][~sound], odd[~sound], equal_nan=True), (lo + i, h)
+                    assert_within(got[lo + i, h][sound], want[sound], tol[sound], f"row {lo + i} head {h}")
