@@ -204,7 +204,13 @@ TRTAMD_API int trtamd_qk_norm_rotary(
  * max_pages pages, and pages whose number is not in 0 .. pages - 1 (not written; read as zeros; not attended to, so that
  * pages that a window has left behind can go back to the pool with -1 in their place).
  *
- * No page may be written for two sequences, or two rows, of a call; reading them may be shared.
+ * No page may be written for two sequences, or two rows, of a call; reading them may be shared, also with a sequence that writes: one
+ * without rows in the call writes nothing.
+ *
+ * max_tokens and T may be bounds, of a captured call for one, and every row is served; but attention's kernels are chosen by them. Where T
+ * is about B * max_tokens, every sequence is taken to have as many rows, and a lone one then waits for its keys 64 at a time (a row over
+ * 131070 keys, 8 key heads of 128: 54 us with max_tokens = T = 1, 1.0 ms with 512, 3.9 ms with 8192).  Capture steps of single tokens apart
+ * from those of prompts.
  * ------------------------------------------------------------------------------------------ */
 typedef struct trtamd_kv_cache
 {
@@ -264,7 +270,9 @@ TRTAMD_API int trtamd_kv_cache_read(trtamd_stream_t stream, trtamd_kv_cache_read
  * tokens j <= p, with a window only those with j > p - window, and the first `sinks` tokens whatever the window is.
  *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j),  k_j and v_j what the cache's bytes stand for.
  * Products of the bytes' values are exact, sums, maxima and exponentials binary32; the weights of the second product are rounded
- * to binary16 once, half to even, the largest at 2^7 or more: by 2^-11 of themselves, or 2^-32 of the largest where that is more.  A row that sees nothing is zeros.  Query head h reads head h / (q_heads / kv_heads) of the cache.
+ * to binary16 once, half to even, each times its page's v_scale and the largest at 2^7 or more: by 2^-11 of themselves, or 2^-32 of the
+ * largest where that is more.
+ * A score of minus infinity weighs nothing.  A row that sees nothing is zeros.  Query head h reads head h / (q_heads / kv_heads) of the cache.
  * A result can differ in its last bits between calls of other sizes or estimates, not between calls of the same.
  * q: row t, head h at q + t * q_token_stride + h * q_head_stride, multiples of 8 elements, d values in a row; out alike.  What is
  * written overlaps nothing that is read, but out may be q with the same strides. */
@@ -295,7 +303,7 @@ TRTAMD_API int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
  *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j)
  * Sums, maxima and exponentials are binary32, the weights of the second product rounded to binary16 once, as above.  Rows that
  * are not seen do not take part whatever they hold, infinities and NaNs included (a NaN or an infinity anywhere near makes the
- * rows around it slow).  A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
+ * rows around it slow, some hundred times where all are).  A score of minus infinity weighs nothing.  A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
  * max_tokens-th on, are left out: neither read nor written.  Row t, head h of q at q + t * q_token_stride + h * q_head_stride, d
  * values in a row, multiples of 8 elements; k, v and out alike: the attention plugins' packing ([token][head][q|k|v][d]) as well
  * as tensors of their own.  What is written overlaps nothing that is read.  No counterpart in the reference's plugins.

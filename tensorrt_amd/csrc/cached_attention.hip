@@ -110,9 +110,7 @@ __device__ inline u32x4 bytes_below(int n)
 // t, so that its scores are those of the keys 16 g .. 16 g + 15 of row m, and 16 bytes of the same keys of element 16 i + m of the
 // values. 16 keys lie in one page, so a lane has one page for the keys and one for the values and the factors of a chunk. The next
 // chunk's keys are requested as soon as this one's are used, its values likewise: 16 KB a wavefront (heads of 128) are always on
-// their way, two wavefronts a SIMD (a third one, at six spilled registers, was 7 % slower). With three sets of inputs, so that nothing
-// is still in the last-level cache: 131070 keys of 8 heads of 128 49 us (268 MB, 5.5 TB/s; a copy moves 5.2). Page sizes and the kind of bytes make no
-// difference. Matrix cores 6 %, vector instructions 35 % of the cycles.
+// their way, two wavefronts a SIMD (a third one, at six spilled registers, was 7 % slower). Page sizes and the kind of bytes make no difference.
 // ------------------------------------------------------------------------------------------
 
 // A sequence and key head, the same for a wavefront.
@@ -408,7 +406,8 @@ __device__ inline void write_few(CacheArgs const& c, AttentionArgs const& a, Few
     }
 }
 
-// One workgroup a sequence and key head, its W wavefronts' sums meeting in LDS.
+// One workgroup a sequence and key head, its W wavefronts' sums meeting in LDS. 1000 keys of 16 heads of 64: 8.0 us with 8 wavefronts, tables,
+// pages and two chunks a wavefront behind each other; with 16 it was 6 % slower.
 template <int KS, bool FP8, int W>
 __global__ __launch_bounds__(W* kWaveSize) __attribute__((amdgpu_waves_per_eu(KS <= 4 ? 3 : KS <= 8 ? 2 : 1))) void cached_few_kernel(
     CacheArgs const c, AttentionArgs const a)
@@ -465,8 +464,9 @@ __global__ __launch_bounds__(W* kWaveSize) __attribute__((amdgpu_waves_per_eu(KS
 // end, whose sums go to memory, and the stretch in which a head begins says which those are. Where heads are few (ALIGNED) every stretch
 // is of one head: the meeting of the wavefronts and the next head's queries would be paid for twice by some.
 // 64 sequences of 400 to 8000 keys, 8 heads of 128, in all: parts of 16 chunks of each head 90 us; stretches 85, with the wavefronts' sums
-// met by all of them at once 82.5, with heads that count 3 to 6 chunks more 77.5 (12: 81); 64 sequences of 4000 109 -> 99, of which 94
-// are this kernel (5.6 TB/s). Aligned, 16 sequences of up to 2000 17.5 -> 14.5.
+// met by all of them at once 82.5, with heads that count 3 to 6 chunks more 77.5 (12: 81); 64 sequences of 4000 109 -> 99 to 101, of which 94
+// are this kernel (5.6 TB/s). Aligned, 16 sequences of up to 2000 17.5 -> 14.8; 131070 keys of 8 heads of 128 49 us with three sets of inputs, so
+// that nothing is still in the last-level cache (268 MB, 5.5 TB/s; a copy moves 5.1), matrix cores 7 %, vector instructions 35 % of the cycles.
 constexpr int kStretchWaves = 4;
 constexpr int kHeadCost = 4; // chunks that a head counts more, for its queries and the wavefronts' meeting: so many places come before its first
 
@@ -792,7 +792,7 @@ __global__ __launch_bounds__(kThreads) void cached_stretch_join_kernel(CacheArgs
 // More rows: 128 a workgroup, 32 a wavefront (attention_rows.hpp). Chunks of 64 keys become binary16 on their way into LDS, in two
 // slots: the next chunk's bytes are requested before this one's products and converted behind them. Values come [d][key], so both
 // operands are read as they lie, 16 bytes a lane.
-// 4 x 1024 rows over 8192 keys before them, 32 heads of 128 on 8: 683 us, 856 TFLOP/s (the library's 8192^3 product 1140 to 1180). Matrix
+// 4 x 1024 rows over 8192 keys before them, 32 heads of 128 on 8: 693 us, 849 TFLOP/s (the library's 8192^3 product 1110 to 1180). Matrix
 // cores 37 % of the cycles and vector instructions 44 % (270 a wavefront and chunk: 160 of them the softmax and the conversion), which take
 // turns. With branches on the head size between the products 4970: every accumulator was moved at each. Tiles of 256 rows, whose keys are
 // converted once for twice the rows, 705; four tiles' worth of parts instead of two 3 to 10 % slower where tiles are few.
@@ -981,7 +981,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
                     }
                 }
                 bool const whole = sees_all(least, most, key0) && __ballot(there[0] < 16 || there[1] < 16) == 0;
-// in powers of 2, s * by + add: where all keys are seen and there, by one multiply-add together with the maximum
+                // in powers of 2, s * by + add: where all keys are seen and there, by one multiply-add together with the maximum
                 float by[2] = {f[0][0], f[1][0]}, add[2] = {f[0][1], f[1][1]};
                 if (!whole)
                 {

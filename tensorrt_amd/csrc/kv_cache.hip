@@ -469,7 +469,6 @@ dim3 copy_grid(trtamd_kv_cache const& c)
     return dim3((unsigned) std::min<int64_t>(touched, 65536), (unsigned) c.B, (unsigned) c.kv_heads * 2);
 }
 
-
 } // namespace
 
 int cache_sizes_check(char const* what, trtamd_kv_cache const& c)

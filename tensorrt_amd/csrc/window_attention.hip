@@ -8,8 +8,8 @@
 // windows only the chunks with sinks. Values lie in LDS as in memory and become the second product's operand by transposing reads.
 // What bounds it: long windows the matrix and the vector instructions (34 and 35 % of the cycles, in turns), short ones the trips to memory
 // of a workgroup's few chunks. 8001 tokens of 16 heads of 128 on 4, 1024 keys back and 4 sinks: 260 us with branches on the head size
-// between the products, 99 without, 88 with rows of LDS in all 64 banks and masks as bits (717 TFLOP/s); all 8001 keys, causal, 293 (894). 128
-// sequences, 16621 tokens, 16 heads of 64, 64 keys on either side: 43 us (3.1 TB/s), 2 to 4 workgroups a CU at once; a third slot of LDS
+// between the products, 99 without, 91 with rows of LDS in all 64 banks and masks as bits (694 TFLOP/s); all 8001 keys, causal, 302 (869). 128
+// sequences, 16621 tokens, 16 heads of 64, 64 keys on either side: 44 us (3.1 TB/s), 2 to 4 workgroups a CU at once; a third slot of LDS
 // instead of the fourth workgroup 47, both, with 34 registers spilled, 99.
 #include "attention_rows.hpp"
 #include "host_utils.hpp"
@@ -59,7 +59,8 @@ struct WindowLds
 };
 
 // One row over the keys it sees and no others, a lane's elements lane, lane + 64, ..: what rows take that have infinities or NaNs
-// near them, where a weight of 0 in the products above is not enough.
+// near them, where a weight of 0 in the products above is not enough. A key is a trip to memory: 8001 tokens of 16 heads of 128 in windows of
+// 1024, all of them NaN, 38 ms.
 template <int DP>
 __device__ void one_row(WindowArgs const& a, int first, int token, int head, int kvHead, Seen const& seen)
 {
@@ -326,8 +327,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(KS <= 
 
 // LDS that a workgroup asks for where it needs `need` bytes. Fewer workgroups than the CUs could hold at once are not spread evenly by
 // themselves: some CUs get as many as fit and others none. With no more than their share fitting they are: 16 sequences of up to 512, 12
-// heads of 64, all keys (some 360 tiles) 20.0 us without, 17.1 with two a CU; 32 of up to 384 in windows (760) 17.4, three 15.7; 8
-// (190) 10.7, one 9.7.
+// heads of 64, all keys (some 360 tiles) 20.0 us without, 17.2 with two a CU; 32 of up to 384 in windows (760) 17.1, three 15.4; 8
+// (190) 10.7, one 9.9.
 constexpr int kCuLds = 160 << 10, kMostLds = kCuLds / 2 + 1024;
 size_t spreading_lds(size_t need, int64_t workgroups, int cus)
 {
