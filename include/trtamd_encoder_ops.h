@@ -303,7 +303,8 @@ TRTAMD_API int trtamd_kv_cache_attention(trtamd_stream_t stream, trtamd_kv_cache
  *   out = binary16(sum_j w_j v_j / sum_j w_j),  w_j = exp(scale * q k_j)
  * Sums, maxima and exponentials are binary32, the weights of the second product rounded to binary16 once, as above.  Rows that
  * are not seen do not take part whatever they hold, infinities and NaNs included (a NaN or an infinity anywhere near makes the
- * rows around it slow, some hundred times where all are).  A score of minus infinity weighs nothing.  A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
+ * rows around it slow, some hundred times where all are).  A score of minus infinity weighs nothing.
+ * A query head h reads head h / (q_heads / kv_heads) of k and v.  Rows at or behind T, and a sequence's rows from the
  * max_tokens-th on, are left out: neither read nor written.  Row t, head h of q at q + t * q_token_stride + h * q_head_stride, d
  * values in a row, multiples of 8 elements; k, v and out alike: the attention plugins' packing ([token][head][q|k|v][d]) as well
  * as tensors of their own.  What is written overlaps nothing that is read.  No counterpart in the reference's plugins.

@@ -67,9 +67,9 @@ __device__ inline bool sees_all(Seen const& least, Seen const& most, int key0)
     return key0 + kChunkKeys <= least.hi && (key0 >= most.lo || key0 + kChunkKeys <= least.sinks);
 }
 
-// What a page's scales are to its scores and weights. No score factor of 0 or below 2^-126 (0 times a score of -infinity is no number), nor an
-// infinite one (times a score of 0), but what is a NaN stays one. The inverse is finite whatever the scale is: a weight of 0 is multiplied by it where no row sees the page, and
-// scales of pages that were never written may be any.
+// What a page's scales are to its scores and weights. No score factor of 0 or below 2^-126 (0 times a score of -infinity is no number), nor
+// an infinite one (times a score of 0), but what is a NaN stays one. The inverse is finite whatever the scale is: a weight of 0 is
+// multiplied by it where no row sees the page, and scales of pages that were never written may be any.
 struct PageFactors
 {
     float score, log2Value, inverse;

@@ -1,10 +1,10 @@
 """Weights far below the largest one: a loud first token that the rows look at for want of anything else, with a value of zero, and
 thousands of quiet keys whose weights only add up to something. Attention over the cache and in windows, against binary64. And scales of the
-scores near the largest binary32."""
+scores near the largest binary32, and scores of minus infinity."""
 import numpy as np
 import pytest
 
-from cache_helpers import Cache, assert_within, round_codes, values
+from cache_helpers import Cache, assert_within, attention_reference, round_codes, values, visible_keys
 from tensorrt_amd import capi
 from test_gpu_kv_cache import attend, check_attention, filled
 from test_gpu_window_attention import Problem
@@ -95,3 +95,33 @@ def test_scales_near_the_largest(api, scale):
     got = p.run(api, 20, 3, 1)
     p.scale = 1.0
     p.check(got, 20, 3, 1)
+
+
+def test_scores_of_minus_infinity(api):
+    """They weigh nothing: keys that a window sees are as if it did not, and a row that has no other is zeros."""
+    p = Problem([150, 20], 4, 2, D, seed=3)
+    p.q[:, :, 5] = np.abs(p.q[:, :, 5]) + np.float16(0.5)
+    gone = np.zeros(170, bool)
+    gone[[3, 40, 41, 64, 149, 155]] = True
+    gone[90:120] = True
+    p.k[gone, :, 5] = -np.inf
+    got = p.run(api, 10, 10, 0)
+    assert (got[100:110] == 0).all()
+    for lo, hi in zip(p.cu[:-1], p.cu[1:]):
+        n = int(hi - lo)
+        k = np.where(gone[lo:hi, None, None], 0, p.k[lo:hi])
+        for i in range(n):
+            ok = visible_keys(i, n, 10, 10, 0) & ~gone[lo:hi]
+            for h in range(4):
+                want, tol = attention_reference(p.q[lo + i, h], k[:, h // 2], np.ones(n), p.v[lo:hi, h // 2], np.ones(n), ok, p.scale)
+                assert_within(got[lo + i, h], want, tol, f"row {lo + i} head {h}")
+    cache = filled(api, "int8", 16, 1, D, [100])
+    cache.k[:] = 5
+    cache.upload()
+    for rows in (1, 40):
+        q = np.zeros((rows, 2, D), np.float16)
+        q[:, 1, 5] = -np.inf
+        q[:, 1] += 1
+        got = attend(api, cache, np.array([0, rows]), q, 0.125)
+        assert (got[:, 1] == 0).all()
+        check_attention(cache, np.array([0, rows]), q[:, :1], got[:, :1], 0.125)
